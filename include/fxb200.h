@@ -46,7 +46,8 @@ const char* fxb_last_error(void);
 
 /* Reads (and with clear != 0 resets) the device error word that kernels set
  * when a bounded wait expires (bit 1 GEMM, 2 attention, 4 gather, 8 cross-
- * entropy). Synchronises
+ * entropy), or when the page table or pool of a KV cache does not fit a call
+ * (bit 16). Synchronises
  * the current device. No reference counterpart (the reference has no bounded
  * waits). */
 int fxb_device_error(int32_t* code, int32_t clear);
@@ -58,7 +59,8 @@ int fxb_num_sms(int32_t* out);
 uint64_t fxb_launch_count(void);
 
 /* ABI self-check for bindings: sizeof(fxb_gemm_args) for which == 0,
- * sizeof(fxb_attn_args) for which == 1, 0 otherwise. */
+ * sizeof(fxb_attn_args) for which == 1, sizeof(fxb_tree_attn_args) for
+ * which == 2, sizeof(fxb_kv_args) for which == 3, 0 otherwise. */
 size_t fxb_abi_struct_size(int32_t which);
 
 /* ------------------------------------------------------------------ RMSNorm */
@@ -343,6 +345,118 @@ int fxb_gather_windows(int32_t dtype, const void* X, int64_t R, int32_t F, const
  * The bias gradient db = g.sum(0) of ml/fxgpu/fused_linear.py:95. */
 int fxb_colsum(int32_t dtype, const void* g, int64_t rows, int32_t cols, float* out,
                int32_t accumulate, void* stream);
+
+/* ------------------------------------------------------------------ generation over a paged KV cache
+ *
+ * Not in the reference, whose sampler re-runs the whole window for every
+ * token (ml/fxlm/sample.py:63-73). The cache is a pool of P pages of `page`
+ * token slots each (page a power of two, 16..256). Sequence (batch row) s
+ * holds its tokens in order in the pages table[s, 0..n_pages[s]); ref[p]
+ * counts the rows that hold page p, and a page is free when its count is 0.
+ * A page held by more than one row is full and is only read. Lengths, tables
+ * and counts live on the device and every call is capturable in a CUDA graph.
+ * Wrong contents of these arrays (a page id outside the pool where a page is
+ * needed, a pool without enough free pages, a path that does not ascend) do
+ * not fault: the access is skipped and bit 16 of the device error word is set
+ * (fxb_device_error). */
+
+/* Attention of the nodes of a token tree over the cache, which also writes
+ * the nodes' keys and values:
+ *   o[b,t,h] = sum_j p_j v_j,  p = softmax_j(scale * q[b,t,h] . k_j)
+ * over j in the cache slots [0, lens[b]) of row b and the nodes j < n_nodes[b]
+ * with bit j of mask[b,t] set; h's key head is h / (Hq/Hkv). A row without
+ * any j, and rows t >= n_nodes[b], are written as zeros. k[b,j], v[b,j] of the
+ * nodes j < n_nodes[b] go to the cache slots lens[b] + j (which have to be
+ * held). T == 1 is plain decoding of one token.
+ * What lies in slots from lens[b] on, in nodes from n_nodes[b] on and in nodes
+ * that the mask hides does not reach a row's output, whatever its value. */
+typedef struct fxb_tree_attn_args {
+  int32_t dtype;            /* FXB_DTYPE_* of every tensor */
+  int32_t B, T, Hq, Hkv, D; /* T <= 64; Hq a multiple of Hkv; D = 64 or 128 */
+  int32_t page, P, W;       /* slots per page, pages of the pool, entries of a table row */
+  float scale;
+  /* element strides, unit stride on D; strides multiples of 16 bytes, 16-byte aligned bases */
+  const void* q; int64_t q_sb, q_st, q_sh;             /* (B,T,Hq,D) */
+  const void* k; int64_t k_sb, k_st, k_sh;             /* (B,T,Hkv,D) */
+  const void* v; int64_t v_sb, v_st, v_sh;
+  void* o;       int64_t o_sb, o_st, o_sh;             /* (B,T,Hq,D) */
+  void* k_pages; int64_t kp_sp, kp_sh, kp_st;          /* (P,Hkv,page,D) */
+  void* v_pages; int64_t vp_sp, vp_sh, vp_st;
+  const int32_t* table; int64_t table_sb;              /* (B,W) */
+  const int32_t* lens;                                 /* (B,) */
+  const int32_t* n_nodes;                              /* (B,) in [0,T] */
+  const int64_t* mask; int64_t mask_sb;                /* (B,T) */
+  void* workspace; int64_t workspace_bytes;            /* fxb_tree_attn_workspace bytes */
+} fxb_tree_attn_args;
+
+/* Workspace bytes of fxb_tree_attn on the current device (partial results of
+ * sequences that several thread blocks share), 16-byte aligned. Its first
+ * fxb_tree_attn_workspace_zeroed(...) bytes have to be zero before its first
+ * use; every call leaves them zero. One workspace per stream. */
+size_t fxb_tree_attn_workspace(int32_t dtype, int32_t B, int32_t T, int32_t Hq, int32_t Hkv, int32_t D);
+size_t fxb_tree_attn_workspace_zeroed(int32_t dtype, int32_t B, int32_t T, int32_t Hq, int32_t Hkv,
+                                      int32_t D);
+int fxb_tree_attn(const fxb_tree_attn_args* args, void* stream);
+
+/* Verification of drafted tokens. Row b is a tree of n_nodes[b] <= T <= 64
+ * nodes, parents[b,c] < c; node 0 is the last committed token, the others
+ * carry drafted tokens. p[b,i,:] is the target's distribution after node i.
+ * The walk starts at node 0 and tries the children c of the current node in
+ * index order: c is accepted, and becomes the current node, when
+ *   with q (q[b,i,:]: the distribution from which each child of node i was
+ *   drawn independently):  u[b,c] * q(x_c) < w(x_c), else
+ *       w = max(w - q, 0) / sum(max(w - q, 0)),    w = p at first;
+ *   without q (drafts that were not drawn at random):
+ *       u[b,c] * m < w(x_c), else m = max(m - w(x_c), 0), w(x_c) = 0,
+ *       w = p and m = 1 at first.
+ * When no child is accepted, the next token is drawn from w (from p where w is
+ * empty) by inversion with u[b,0]: the first token at which the running sum
+ * exceeds floor(u * total). So accepted tokens and the next one are
+ * distributed as if drawn from the target.
+ * Sums are taken over floor(w * 2^36) in 64-bit integers, so results do not
+ * depend on the order of summation; values that are not above 0 (NaN among
+ * them) count as 0, values above 1 as 1.
+ * path (B,T): the accepted nodes in order, node 0 first, then -1; n_path (B):
+ * their number; next (B): the drawn token, -1 for n_nodes == 0 or an empty row. */
+int fxb_verify_tree(const int64_t* tokens, const int32_t* parents, const int32_t* n_nodes,
+                    const float* p, int64_t p_sb, int64_t p_st, const float* q, int64_t q_sb,
+                    int64_t q_st, const float* u, int32_t* path, int32_t* n_path, int64_t* next,
+                    int32_t B, int32_t T, int32_t V, void* stream);
+
+/* The cache of all layers, as fxb_kv_commit and fxb_kv_fork see it. */
+typedef struct fxb_kv_args {
+  int32_t elem_size;        /* bytes of one element (2 or 4); D * elem_size a multiple of 16 */
+  int32_t L, P, H, page, D;
+  void* k; int64_t k_sl, k_sp, k_sh, k_st;             /* (L,P,H,page,D), strides as above */
+  void* v; int64_t v_sl, v_sp, v_sh, v_st;
+  int32_t S, W;
+  int32_t* table; int64_t table_ss;                    /* (S,W) */
+  int32_t* n_pages;                                    /* (S,) */
+  int32_t* lens;                                       /* (S,) */
+  int32_t* ref;                                        /* (P,) */
+} fxb_kv_args;
+
+/* Commits a path of each row and makes room: token i < n_path[s] moves from
+ * slot lens[s] + path[s,i] to slot lens[s] + i in every layer (path ascends
+ * strictly; path == NULL: nothing moves and n_path counts as 0), then
+ * lens_out[s] = lens[s] + n_path[s], and where room[s] > 0 (room may be NULL)
+ * the row is given pages for lens_out[s] + room[s] slots: the lowest-numbered
+ * free ones, rows in order. If the pool lacks them no row is given any (bit 16
+ * of the device error word). lens_out must not be lens. */
+int fxb_kv_commit(const fxb_kv_args* args, const int32_t* path, int64_t path_ss, int32_t T,
+                  const int32_t* n_path, const int32_t* room, int32_t* lens_out, void* stream);
+
+/* Row s becomes a fork of row parents[s] as it was before the call (s itself:
+ * it stays; -1: it is emptied). Full pages are shared. A last page that is
+ * only partly filled passes to one heir (the row itself, else the first row
+ * that forks from it); the others get a copy of its filled slots in a page of
+ * their own, the lowest-numbered pages that were free before the call, rows in
+ * order. Pages held beyond the length, and pages that no row holds any more,
+ * become free. If the pool lacks pages, or a parent is outside [-1, S),
+ * nothing changes (bit 16 of the device error word). workspace:
+ * fxb_kv_fork_workspace bytes, 16-byte aligned. */
+size_t fxb_kv_fork_workspace(int32_t S, int32_t W);
+int fxb_kv_fork(const fxb_kv_args* args, const int32_t* parents, void* workspace, void* stream);
 
 #ifdef __cplusplus
 }

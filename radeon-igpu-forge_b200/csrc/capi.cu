@@ -136,7 +136,7 @@ int encode_tiled(CUtensorMap* map, CUtensorMapDataType dt, uint32_t rank, const 
 
 extern "C" {
 
-int fxb_version(void) { return 200; }  // 0.2.0: fxb_gemm_args.workspace
+int fxb_version(void) { return 300; }  // 0.3.0: generation over a paged KV cache
 
 const char* fxb_last_error(void) { return fxb::t_last_error.c_str(); }
 
@@ -162,6 +162,8 @@ uint64_t fxb_launch_count(void) { return fxb::g_launches.load(std::memory_order_
 size_t fxb_abi_struct_size(int32_t which) {
   if (which == 0) return sizeof(fxb_gemm_args);
   if (which == 1) return sizeof(fxb_attn_args);
+  if (which == 2) return sizeof(fxb_tree_attn_args);
+  if (which == 3) return sizeof(fxb_kv_args);
   return 0;
 }
 

@@ -64,6 +64,34 @@ class AttnArgs(ctypes.Structure):
     ]
 
 
+class TreeAttnArgs(ctypes.Structure):
+    """Mirror of fxb_tree_attn_args."""
+    _fields_ = [
+        ("dtype", _i32), ("B", _i32), ("T", _i32), ("Hq", _i32), ("Hkv", _i32), ("D", _i32),
+        ("page", _i32), ("P", _i32), ("W", _i32), ("scale", _f32),
+        ("q", _vp), ("q_sb", _i64), ("q_st", _i64), ("q_sh", _i64),
+        ("k", _vp), ("k_sb", _i64), ("k_st", _i64), ("k_sh", _i64),
+        ("v", _vp), ("v_sb", _i64), ("v_st", _i64), ("v_sh", _i64),
+        ("o", _vp), ("o_sb", _i64), ("o_st", _i64), ("o_sh", _i64),
+        ("k_pages", _vp), ("kp_sp", _i64), ("kp_sh", _i64), ("kp_st", _i64),
+        ("v_pages", _vp), ("vp_sp", _i64), ("vp_sh", _i64), ("vp_st", _i64),
+        ("table", _vp), ("table_sb", _i64), ("lens", _vp), ("n_nodes", _vp),
+        ("mask", _vp), ("mask_sb", _i64),
+        ("workspace", _vp), ("workspace_bytes", _i64),
+    ]
+
+
+class KvArgs(ctypes.Structure):
+    """Mirror of fxb_kv_args."""
+    _fields_ = [
+        ("elem_size", _i32), ("L", _i32), ("P", _i32), ("H", _i32), ("page", _i32), ("D", _i32),
+        ("k", _vp), ("k_sl", _i64), ("k_sp", _i64), ("k_sh", _i64), ("k_st", _i64),
+        ("v", _vp), ("v_sl", _i64), ("v_sp", _i64), ("v_sh", _i64), ("v_st", _i64),
+        ("S", _i32), ("W", _i32), ("table", _vp), ("table_ss", _i64),
+        ("n_pages", _vp), ("lens", _vp), ("ref", _vp),
+    ]
+
+
 # name -> (restype, argtypes); every symbol declared in include/fxb200.h
 SIGNATURES = {
     "fxb_version": (ctypes.c_int, []),
@@ -98,6 +126,14 @@ SIGNATURES = {
     "fxb_attn_fwd": (ctypes.c_int, [ctypes.POINTER(AttnArgs), _vp]),
     "fxb_attn_bwd_workspace": (ctypes.c_size_t, [_i32, _i32, _i32, _i32]),
     "fxb_attn_bwd": (ctypes.c_int, [ctypes.POINTER(AttnArgs), _vp]),
+    "fxb_tree_attn_workspace": (ctypes.c_size_t, [_i32] * 6),
+    "fxb_tree_attn_workspace_zeroed": (ctypes.c_size_t, [_i32] * 6),
+    "fxb_tree_attn": (ctypes.c_int, [ctypes.POINTER(TreeAttnArgs), _vp]),
+    "fxb_verify_tree": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp,
+                                       _vp, _vp, _i32, _i32, _i32, _vp]),
+    "fxb_kv_commit": (ctypes.c_int, [ctypes.POINTER(KvArgs), _vp, _i64, _i32, _vp, _vp, _vp, _vp]),
+    "fxb_kv_fork_workspace": (ctypes.c_size_t, [_i32, _i32]),
+    "fxb_kv_fork": (ctypes.c_int, [ctypes.POINTER(KvArgs), _vp, _vp, _vp]),
     "fxb_embedding_fwd": (ctypes.c_int, [_i32, _vp, _vp, _vp, _vp, _i64, _i64, _i32, _i64, _vp]),
     "fxb_embedding_bwd": (ctypes.c_int, [_i32, _vp, _vp, _vp, _vp, _i64, _i64, _i32, _i64, _vp]),
     "fxb_axpy": (ctypes.c_int, [_i32, _vp, _i32, _vp, _vp, _i32, _i64, _vp]),
@@ -180,8 +216,10 @@ def device_error(clear=True):
 
 # bits of the device error word (csrc/common.cuh)
 DERR_NAMES = {1: "gemm (tensor-core pipeline or tail-split wait)", 2: "attention pipeline",
-              4: "gather pipeline", 8: "cross-entropy row copy"}
+              4: "gather pipeline", 8: "cross-entropy row copy",
+              16: "KV cache: page ids, free pages, lengths or paths that do not fit the call"}
 DERR_GEMM_WAIT = 1
+DERR_PAGES = 16
 
 # called with the word when a check finds it non-zero, before raising
 # (fxb200.ops registers the reset of its GEMM workspaces' arrival counters)
@@ -198,5 +236,8 @@ def raise_on_device_error(where=""):
         for fn in _ON_DEVICE_ERROR:
             fn(code)
         what = ", ".join(n for b, n in DERR_NAMES.items() if code & b) or "unknown"
+        if code == DERR_PAGES:
+            raise RuntimeError(f"libfxb200: a KV cache call did not fit{' ' + where if where else ''} "
+                               f"(device error word {code}: {what}); the step's results are invalid")
         raise RuntimeError(f"libfxb200: a kernel's bounded wait expired{' ' + where if where else ''} "
                            f"(device error word {code}: {what}); the step's results are invalid")

@@ -22,6 +22,12 @@ __all__ = [
     "GPTConfig",
     "GraphedStep",
     "GraphedFunction",
+    "tree_attention",
+    "tree_masks",
+    "kv_commit",
+    "kv_reserve",
+    "kv_fork",
+    "verify_tree",
 ]
 
 
@@ -50,4 +56,10 @@ def __getattr__(name):
     if name in ("GPT", "GPTConfig"):
         from . import model as _m
         return getattr(_m, name)
+    if name in ("tree_attention", "tree_masks", "kv_commit", "kv_reserve", "kv_fork"):
+        from . import paged as _m
+        return getattr(_m, name)
+    if name == "verify_tree":
+        from .speculate import verify_tree
+        return verify_tree
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

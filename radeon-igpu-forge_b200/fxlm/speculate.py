@@ -1,0 +1,60 @@
+"""fxlm.speculate: verification of drafted tokens against the target's probabilities."""
+import torch
+
+from fxb200 import _lib
+from .paged import MAX_NODES, _i32
+
+
+def _probs(t, name, shape):
+    if t.dtype != torch.float32 or not t.is_cuda:
+        raise TypeError(f"{name} must be a cuda fp32 tensor, got {t.dtype} on {t.device}")
+    if tuple(t.shape) != shape or (shape[-1] > 1 and t.stride(-1) != 1):
+        raise ValueError(f"{name} must be {shape} with unit stride on the vocabulary, got {tuple(t.shape)}")
+    return t.data_ptr(), t.stride(0), t.stride(1)
+
+
+def verify_tree(tokens, parents, n_nodes, target_probs, u, draft_probs=None):
+    """Walk each row's tree of drafted tokens; returns (path, n_path, next_token).
+
+    tokens (B, T) int64, parents (B, T) int32 with parents[b, c] < c, n_nodes
+    (B,) int32: node 0 is the last committed token, the others are drafts.
+    target_probs (B, T, V) fp32: the target's distribution after each node;
+    draft_probs (the same, or None): the distribution from which the children
+    of each node were drawn independently. u (B, T) fp32 in [0, 1): u[b, c]
+    decides on node c, u[b, 0] draws the next token. With draft_probs child c
+    is accepted when u * q(x) < w(x), and a rejection leaves
+    w = max(w - q, 0) / sum; without, children are taken with their probability
+    under what the rejected ones left over. In both the accepted tokens and the
+    next one are distributed as draws from the target. Sums are exact (64-bit
+    integers in units of 2^-36), so the result is the same on every run.
+
+    path (B, T) int32: accepted nodes, node 0 first, then -1; n_path (B,) int32;
+    next_token (B,) int64, -1 where n_nodes is 0 or the row has no mass.
+    """
+    if tokens.dim() != 2:
+        raise ValueError(f"tokens must be (B,T), got {tuple(tokens.shape)}")
+    B, T = tokens.shape
+    if not 1 <= T <= MAX_NODES:
+        raise ValueError(f"T={T}: 1 to {MAX_NODES} nodes")
+    if tokens.dtype != torch.int64 or not tokens.is_cuda:
+        raise TypeError("tokens must be a cuda int64 tensor")
+    if not tokens.is_contiguous():
+        raise ValueError("tokens must be contiguous")
+    V = target_probs.shape[-1]
+    pp, p_sb, p_st = _probs(target_probs, "target_probs", (B, T, V))
+    qp, q_sb, q_st = (None, 0, 0) if draft_probs is None else _probs(draft_probs, "draft_probs", (B, T, V))
+    par, nn = _i32(parents, "parents", (B, T)), _i32(n_nodes, "n_nodes", (B,))
+    if u.dtype != torch.float32 or not u.is_cuda:
+        raise TypeError("u must be a cuda fp32 tensor")
+    if tuple(u.shape) != (B, T) or not u.is_contiguous():
+        raise ValueError(f"u must be contiguous ({B},{T}), got {tuple(u.shape)}")
+    dev = tokens.device
+    path = torch.empty((B, T), device=dev, dtype=torch.int32)
+    n_path = torch.empty((B,), device=dev, dtype=torch.int32)
+    nxt = torch.empty((B,), device=dev, dtype=torch.int64)
+    if B == 0:
+        return path, n_path, nxt
+    _lib.check(_lib.load().fxb_verify_tree(
+        tokens.data_ptr(), par, nn, pp, p_sb, p_st, qp, q_sb, q_st, u.data_ptr(), path.data_ptr(),
+        n_path.data_ptr(), nxt.data_ptr(), B, T, V, _lib.stream_ptr(dev)), "fxb_verify_tree")
+    return path, n_path, nxt

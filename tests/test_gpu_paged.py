@@ -1,0 +1,712 @@
+"""GPU tests of generation over a paged KV cache: tree attention, verification
+of drafted tokens, committing and forking sequences.
+
+Attention is compared with a 64-bit computation of the same formula on the same
+rounded inputs. Its error bound is the formula's: with A = sum_j p_j |v_j|, u
+the unit roundoff of the dtype and e the error of a score, rounding the
+probabilities to the dtype (16-bit types) and the result once gives at most
+u (A + |o|), a score's error moves p by a factor of at most 1 + 2 e, and
+probabilities below the smallest fp16 number vanish. Verification and the page
+operators give whole numbers and copies: they have to be equal.
+"""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+@pytest.fixture(scope="module")
+def dev():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    return torch.device("cuda")
+
+
+@pytest.fixture(autouse=True)
+def _clean_error_word(dev):
+    """Every test must leave the device error word at 0 (those that set it read and clear it)."""
+    yield
+    from fxb200 import _lib
+    code = _lib.device_error(clear=True)
+    assert code == 0, f"device error word {code}"
+
+
+# ------------------------------------------------------------------ tree attention
+def random_tree(B, T, rng):
+    par = np.full((B, T), -1, np.int32)
+    for b in range(B):
+        for i in range(1, T):
+            par[b, i] = rng.randint(max(0, i - 4), i)
+    return torch.from_numpy(par)
+
+
+def make(dev, dtype, B, T, Hq, Hkv, D, lens, page, seed, n_nodes=None, layout="fused", spread=1.5):
+    from fxlm import tree_masks
+    g = torch.Generator(device=dev).manual_seed(seed)
+    rng = np.random.RandomState(seed)
+
+    def randn(*s):
+        return torch.randn(*s, generator=g, device=dev, dtype=F32)
+
+    held = [-(-(n + T) // page) for n in lens]
+    W = max(held) + 1
+    P = sum(held) + 2
+    order = rng.permutation(P)[:sum(held)]
+    table, at = np.full((B, W), -1, np.int32), 0
+    for b, h in enumerate(held):
+        table[b, :h] = order[at:at + h]
+        at += h
+    if layout == "nhd":  # (P, page, H, D) storage seen as (P, H, page, D); separate q, k, v
+        kp, vp = (randn(P, page, Hkv, D).to(dtype).transpose(1, 2) for _ in range(2))
+        q, k, v = ((randn(B, T, h, D) * spread).to(dtype) for h in (Hq, Hkv, Hkv))
+    else:  # keys and values interleaved in one pool; q, k, v slices of one projection
+        pool = randn(P, Hkv, 2, page, D).to(dtype)
+        kp, vp = pool[:, :, 0], pool[:, :, 1]
+        qkv = (randn(B, T, Hq + 2 * Hkv, D) * spread).to(dtype)
+        q, k, v = qkv.split([Hq, Hkv, Hkv], dim=2)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    n_nodes = [T] * B if n_nodes is None else n_nodes
+    return dict(q=q, k=k, v=v, k_pages=kp, v_pages=vp, page_table=torch.from_numpy(table).to(dev),
+                ctx_lens=i32(lens), n_nodes=i32(n_nodes), tree_mask=tree_masks(random_tree(B, T, rng)).to(dev))
+
+
+def attention_64(a, scale=None):
+    """(o, bound of the error) by the formula in 64 bits, one node at a time."""
+    q, k, v, kp, vp = (a[n] for n in ("q", "k", "v", "k_pages", "v_pages"))
+    B, T, Hq, D = q.shape
+    Hkv, page = k.shape[2], kp.shape[2]
+    G = Hq // Hkv
+    scale = 1 / math.sqrt(D) if scale is None else scale
+    u = {BF16: 2.0 ** -8, F16: 2.0 ** -11, F32: 2.0 ** -24}[q.dtype]
+    p_round = 0.0 if q.dtype == F32 else 1.0
+    o = torch.zeros(B, T, Hq, D, dtype=torch.float64, device=q.device)
+    tol = torch.zeros_like(o)
+    for b in range(B):
+        n, L = int(a["n_nodes"][b]), int(a["ctx_lens"][b])
+        pages = a["page_table"][b, :-(-L // page)].long()
+        for t in range(n):
+            m = int(a["tree_mask"][b, t])
+            see = [j for j in range(n) if (m >> j) & 1]
+            for h in range(Hkv):
+                kk = torch.cat([kp[pages, h].reshape(-1, D)[:L], k[b, see, h]]).double()
+                vv = torch.cat([vp[pages, h].reshape(-1, D)[:L], v[b, see, h]]).double()
+                if not len(kk):
+                    continue
+                qq = q[b, t, h * G:(h + 1) * G].double()
+                p = torch.softmax(qq @ kk.T * scale, -1)
+                r, A = p @ vv, p @ vv.abs()
+                e = D * 2.0 ** -23 * float((qq.abs() @ kk.abs().T).max()) * scale + 2.0 ** -20
+                low = 2.0 ** -24 * len(kk) * vv.abs().max() if q.dtype == F16 else 0.0
+                o[b, t, h * G:(h + 1) * G] = r
+                tol[b, t, h * G:(h + 1) * G] = 1.02 * u * (p_round * A + r.abs()) + 2 * e * A + low
+    return o, tol
+
+
+def check(a, scale=None, **kw):
+    from fxlm import tree_attention
+    ref, tol = attention_64(a, scale)
+    before = a["k_pages"].clone(), a["v_pages"].clone()
+    o = tree_attention(**a, scale=scale, **kw)
+    torch.cuda.synchronize()
+    bad = (o.double() - ref).abs() > tol
+    assert torch.isfinite(o).all()
+    assert not bad.any(), f"{int(bad.sum())} of {bad.numel()} off, worst {((o.double() - ref).abs() / (tol + 1e-30)).max()}"
+    # the nodes' keys and values stand behind the sequences, nothing else changed
+    page = a["k_pages"].shape[2]
+    for pool, was, new in ((a["k_pages"], before[0], a["k"]), (a["v_pages"], before[1], a["v"])):
+        for b in range(a["q"].shape[0]):
+            for j in range(int(a["n_nodes"][b])):
+                at = int(a["ctx_lens"][b]) + j
+                was[int(a["page_table"][b, at // page]), :, at % page] = new[b, j]
+        assert torch.equal(pool.view(torch.int16 if pool.element_size() == 2 else torch.int32),
+                           was.view(torch.int16 if pool.element_size() == 2 else torch.int32))
+    return o
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("B,T,Hq,Hkv,D,lens,page", [
+    (1, 1, 1, 1, 64, [0], 16),                       # one token, empty cache
+    (1, 1, 12, 12, 64, [1], 16),
+    (2, 1, 4, 2, 128, [15, 16], 16),                 # the node opens a page, or not
+    (3, 2, 3, 1, 64, [17, 127, 128], 32),
+    (4, 5, 12, 12, 64, [63, 64, 65, 0], 64),
+    (2, 7, 8, 1, 128, [255, 257], 128),
+    (2, 16, 10, 5, 64, [1000, 31], 16),
+    (3, 17, 6, 2, 128, [129, 640, 5], 256),
+    (2, 33, 8, 2, 64, [511, 70], 64),
+    (1, 64, 16, 2, 128, [300], 32),                  # 512 rows on a key head
+    (2, 64, 2, 2, 64, [1, 900], 128),
+    (9, 3, 7, 7, 128, [0, 1, 2, 3, 100, 200, 300, 33, 8], 16),
+])
+def test_attention_shapes(dev, dtype, B, T, Hq, Hkv, D, lens, page):
+    check(make(dev, dtype, B, T, Hq, Hkv, D, lens, page, seed=B * 100 + T))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("T,G,Hkv,D,L", [(1, 1, 2, 64, 9001), (2, 4, 1, 128, 20011), (9, 8, 2, 128, 5003),
+                                         (64, 1, 3, 64, 4099)])
+def test_attention_long(dev, dtype, T, G, Hkv, D, L):
+    check(make(dev, dtype, 1, T, Hkv * G, Hkv, D, [L], 64, seed=T))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("T,Hq,Hkv", [(5, 4, 4), (24, 8, 2)])
+def test_attention_uneven_rows_and_layout(dev, dtype, T, Hq, Hkv):
+    # lengths from none to long, rows with fewer nodes and with none; pages stored token-major
+    a = make(dev, dtype, 6, T, Hq, Hkv, 64, [0, 3000, 1, 77, 512, 129], 32, seed=3,
+             n_nodes=[T, 1, 0, T - 1, 2, T], layout="nhd")
+    o = check(a)
+    for b, n in enumerate(a["n_nodes"].tolist()):
+        assert not o[b, n:].any()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("T,G", [(6, 1), (40, 4)])
+def test_attention_masks(dev, dtype, T, G):
+    # masks that are no trees: rows that see nothing, only a later node, everything, bit 63 of T=64 trees
+    a = make(dev, dtype, 3, T, 2 * G, 2, 64, [0, 5, 200], 16, seed=5)
+    g = torch.Generator().manual_seed(1)
+    m = torch.randint(-(2 ** 62), 2 ** 62, (3, T), generator=g)
+    m[:, 0] = 0
+    m[:, 1] = 1 << (T - 1)
+    m[:, 2] = -1
+    a["tree_mask"] = m.to(dev)
+    o = check(a)
+    assert not o[0, 0].any()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("T,G,D", [(4, 1, 64), (4, 8, 128), (30, 4, 128)])
+def test_attention_hidden_values(dev, dtype, T, G, D):
+    # infinities and NaN where no visible key is: behind the sequences, in nodes that do not
+    # exist, and in a node that only its own branch sees
+    B, lens = 3, [0, 70, 333]
+    clean = make(dev, dtype, B, T, G * 2, 2, D, lens, 32, seed=11, n_nodes=[T - 1] * B)
+    ref, tol = attention_64(clean)
+    a = dict(clean, k_pages=clean["k_pages"].clone(), v_pages=clean["v_pages"].clone(),
+             q=clean["q"].clone(), k=clean["k"].clone(), v=clean["v"].clone())
+    page = 32
+    for pool, bad in ((a["k_pages"], float("nan")), (a["v_pages"], float("inf"))):
+        for b in range(B):
+            held = a["page_table"][b][a["page_table"][b] >= 0].long()
+            for slot in range(lens[b], len(held) * page):
+                pool[held[slot // page], :, slot % page] = bad
+        free = sorted(set(range(pool.shape[0])) - set(a["page_table"].flatten().tolist()))
+        pool[free] = bad
+    for x in (a["q"], a["k"], a["v"]):
+        x[:, T - 1] = float("nan")
+    hide = 1  # node 1: only itself and its descendants see it
+    a["k"][:, hide] = float("inf")
+    a["v"][:, hide] = float("-inf")
+    a["v"][:, hide, :, 3] = float("nan")
+    from fxlm import tree_attention
+    o = tree_attention(**a).double()
+    sees = ((a["tree_mask"] >> hide) & 1).bool()
+    sees[:, T - 1] = False
+    assert not sees[:, 0].any() and sees[:, hide].all()
+    assert ((o - ref).abs() <= tol)[~sees].all()
+    assert not torch.isfinite(o[sees]).any(-1).all()
+
+
+def test_attention_value_infinity_reaches_who_sees_it(dev):
+    # an infinite value in a visible node, with finite keys: the formula's infinity in that element alone
+    from fxlm import tree_attention
+    for dtype in (BF16, F32):
+        for T, G in ((4, 1), (30, 4)):
+            a = make(dev, dtype, 1, T, 2 * G, 2, 64, [50], 32, seed=2)
+            a["v"] = a["v"].clone()
+            ref, tol = attention_64(a)
+            a["v"][0, 1, :, 5] = float("inf")
+            o = tree_attention(**a).double()
+            sees = ((a["tree_mask"][0] >> 1) & 1).bool()
+            hit = torch.zeros_like(o, dtype=torch.bool)
+            hit[0, sees, :, 5] = True
+            assert (o[hit] == float("inf")).all()
+            assert ((o - ref).abs() <= tol)[~hit].all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("T,G", [(3, 1), (20, 8)])
+def test_attention_peaked_scores(dev, dtype, T, G):
+    # large scores whose maximum rises along the sequence: every rescaling of the running sums is taken
+    a = make(dev, dtype, 1, T, G, 1, 64, [777], 64, seed=4)
+    pages, page = a["page_table"][0].long(), 64
+    up = torch.linspace(0, 24, 777, device=dev)
+    for j in range(777):
+        a["k_pages"][pages[j // page], :, j % page] = (a["k_pages"][pages[j // page], :, j % page].float()
+                                                       * 0.1 + up[j]).to(dtype)
+    a["q"] = torch.full_like(a["q"], 0.125)
+    check(a)
+    check(a, scale=0.5)
+
+
+def test_attention_no_dependence_on_the_past(dev):
+    # the same call twice is the same result bit for bit, other calls in between or not
+    from fxlm import tree_attention
+    a = make(dev, BF16, 5, 6, 8, 2, 128, [3000, 1, 700, 64, 9000], 64, seed=1)
+    b = make(dev, BF16, 2, 64, 8, 1, 64, [2000, 900], 16, seed=2)
+    first = tree_attention(**a).clone()
+    for _ in range(3):
+        tree_attention(**b)
+        assert torch.equal(tree_attention(**a), first)
+
+
+def test_attention_other_stream_and_graph(dev):
+    from fxb200 import ops
+    from fxlm import tree_attention
+    a = make(dev, BF16, 3, 4, 8, 8, 64, [500, 900, 3], 32, seed=6)
+    want = tree_attention(**a).clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = tree_attention(**a)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+    g = torch.cuda.CUDAGraph()
+    ws = {}
+    with ops.graph_workspaces(ws), torch.cuda.graph(g):
+        out = tree_attention(**a)
+    for _ in range(3):
+        out.zero_()
+        g.replay()
+        tree_attention(**a)
+        assert torch.equal(out, want)
+    # lengths are read on the device: a replay after they changed is the new result
+    a["ctx_lens"].copy_(torch.tensor([17, 880, 0], dtype=torch.int32))
+    g.replay()
+    assert torch.equal(out, tree_attention(**a))
+
+
+@pytest.mark.parametrize("T,G,dtype", [(2, 1, BF16), (32, 1, BF16), (2, 1, F32)])
+def test_attention_far_pages(dev, T, G, dtype):
+    # pages beyond 2^32 bytes and 2^31 elements of the pool
+    page, D, H = 64, 128, 4
+    P = 2 ** 31 // (page * D * H) + 40
+    pool = torch.zeros(P, H, page, D, device=dev, dtype=dtype)
+    a = make(dev, dtype, 2, T, H * G, H, D, [150, 1], page, seed=8)
+    far = torch.arange(P - 10, P, device=dev)
+    near = a["page_table"].clone()
+    for k in ("k_pages", "v_pages"):
+        src = a[k]
+        one = pool if k == "k_pages" else pool.clone()
+        for i in range(src.shape[0]):
+            one[far[i]] = src[i]
+        a[k] = one
+    a["page_table"] = torch.where(near >= 0, (near + P - 10).int(), -1).int()
+    ref, tol = attention_64(a)
+    from fxlm import tree_attention
+    o = tree_attention(**a)
+    assert ((o.double() - ref).abs() <= tol).all()
+    assert torch.equal(a["k_pages"][int(a["page_table"][1, 0]), :, 1], a["k"][1, 0])
+
+
+def test_attention_pages_that_do_not_fit(dev):
+    from fxb200 import _lib
+    from fxlm import tree_attention
+    a = make(dev, BF16, 2, 3, 4, 4, 64, [40, 20], 16, seed=9)
+    good = tree_attention(**a)
+    for change in ({"page_table": torch.where(a["page_table"] == a["page_table"][0, 1], 10 ** 6, a["page_table"]).int()},
+                   {"page_table": torch.where(a["page_table"] == a["page_table"][0, 1], -5, a["page_table"]).int()},
+                   {"ctx_lens": torch.tensor([10 ** 8, 20], dtype=torch.int32, device=dev)},
+                   {"ctx_lens": torch.tensor([-3, 20], dtype=torch.int32, device=dev)},
+                   {"n_nodes": torch.tensor([70, 3], dtype=torch.int32, device=dev)}):
+        o = tree_attention(**dict(a, **change))
+        assert torch.equal(o[1], good[1])
+        with pytest.raises(RuntimeError, match="KV cache"):
+            _lib.raise_on_device_error()
+
+
+# ------------------------------------------------------------------ verification
+def verify_plain(tokens, par, n, p, u, q):
+    """One row, one step at a time: fp32 for single values, Python integers for sums."""
+    f = np.float32
+
+    def fixed(w):
+        return int(min(w, f(1)) * f(2 ** 36)) if w > 0 else 0
+
+    def fixed_row(w):
+        w = np.where(w > 0, w, f(0)).clip(max=f(1))
+        return (w * f(2 ** 36)).astype(np.int64)
+
+    V = p.shape[1]
+    if n == 0:
+        return [], -1
+    path, cur = [0], 0
+    w, scale, mass, empty = p[0].copy(), f(1), f(1), False
+    for c in range(1, n):
+        if par[c] != cur or empty:
+            continue
+        x = int(tokens[c])
+        inside = 0 <= x < V
+        a = w[x] if inside and w[x] > 0 else f(0)
+        if q is None:
+            a = min(a, f(1))
+            take = f(u[c]) * mass < a
+        else:
+            take = f(u[c]) * (q[cur][x] if inside else f(0)) < a * scale
+        if take:
+            cur = c
+            path.append(c)
+            w, scale, mass = p[c].copy(), f(1), f(1)
+        elif q is None:
+            mass = max(mass - a, f(0))
+            if inside:
+                w[x] = 0
+        else:
+            w = w * scale - q[cur]
+            w = np.where(w > 0, w, f(0))
+            total = int(fixed_row(w).sum())
+            if total:
+                scale = f(1) / (f(total) * f(2.0 ** -36))
+            else:
+                empty = True
+    fr = fixed_row(w)
+    if fr.sum() == 0:
+        fr = fixed_row(p[cur])
+    total = int(fr.sum())
+    if total == 0:
+        return path, -1
+    thr = (total * int(min(max(u[0], 0), 1 - 2.0 ** -24) * 2 ** 24)) >> 24
+    return path, int(np.searchsorted(np.cumsum(fr), thr, side="right"))
+
+
+def verify_inputs(B, T, V, draft, seed, chain=False, peak=3.0):
+    rng = np.random.RandomState(seed)
+    par = random_tree(B, T, rng).numpy()
+    if chain:
+        par[:, 1:] = np.arange(T - 1)
+    g = torch.Generator().manual_seed(seed)
+    logits = torch.randn(B, T, V, generator=g) * peak
+    p = torch.softmax(logits, -1)
+    q = torch.softmax(logits * 0.7 + torch.randn(B, T, V, generator=g), -1)
+    src = (q if draft else p).double().numpy()
+    tokens = np.zeros((B, T), np.int64)
+    for b in range(B):
+        for c in range(1, T):
+            w = src[b, par[b, c]]
+            tokens[b, c] = rng.choice(V, p=w / w.sum())
+    u = torch.rand(B, T, generator=g)
+    n = rng.randint(0, T + 1, B).astype(np.int32)
+    n[0] = T
+    return torch.from_numpy(tokens), torch.from_numpy(par), torch.from_numpy(n), p, u, (q if draft else None)
+
+
+def verify_check(dev, tokens, par, n, p, u, q):
+    from fxlm import verify_tree
+    to = lambda x: None if x is None else x.to(dev)  # noqa: E731
+    path, n_path, nxt = verify_tree(to(tokens), to(par), to(n), to(p), to(u), draft_probs=to(q))
+    lengths = []
+    for b in range(tokens.shape[0]):
+        want, tok = verify_plain(tokens[b].numpy(), par[b].numpy(), int(n[b]), p[b].numpy(), u[b].numpy(),
+                                 None if q is None else q[b].numpy())
+        got = path[b].tolist()
+        assert got == want + [-1] * (tokens.shape[1] - len(want)), (b, got, want)
+        assert int(n_path[b]) == len(want) and int(nxt[b]) == tok, (b, int(nxt[b]), tok)
+        lengths.append(len(want))
+    return lengths
+
+
+@pytest.mark.parametrize("draft", [False, True])
+@pytest.mark.parametrize("B,T,V,chain", [(1, 1, 5, False), (1, 2, 33, True), (7, 9, 257, True), (16, 33, 1000, False),
+                                         (5, 64, 4097, False), (3, 8, 32768, True), (2, 5, 50257, False),
+                                         (2, 3, 131075, False), (70, 4, 100, False)])
+def test_verify(dev, B, T, V, chain, draft):
+    lengths = verify_check(dev, *verify_inputs(B, T, V, draft, seed=B * T + V, chain=chain))
+    if B * T > 60 and T > 2:
+        assert max(lengths) > 1 and min(lengths) <= 1
+
+
+def test_verify_many_rejections(dev):
+    # drafts that the target hardly ever takes: long chains of residuals, and rows whose children all fail
+    tokens, par, n, p, u, q = verify_inputs(12, 20, 300, True, seed=4)
+    par[:, 1:] = 0
+    g = torch.Generator().manual_seed(9)
+    q = torch.softmax(torch.randn(12, 20, 300, generator=g) * 2, -1)
+    tokens = torch.multinomial(q[:, 0], 20, replacement=True, generator=g)
+    verify_check(dev, tokens, par, torch.full_like(n, 20), p, u, q)
+
+
+@pytest.mark.parametrize("draft", [False, True])
+def test_verify_degenerate_rows(dev, draft):
+    B, T, V = 8, 4, 70
+    tokens, par, n, p, u, q = verify_inputs(B, T, V, draft, seed=6)
+    n[:] = T
+    par[:, 1:] = 0
+    p[0] = 0                                     # no mass at all
+    p[1] = float("nan")
+    p[2] = 0; p[2, :, 69] = 1                    # everything on the last token
+    p[3] = 0; p[3, :, 0] = 1
+    tokens[4, 1:] = torch.tensor([-1, V, 2 ** 40])   # tokens outside the vocabulary
+    tokens[5, 1:] = tokens[5, 1]                 # the same draft three times
+    p[5] = p[5, :, torch.randperm(V)]
+    u[6] = 0
+    u[7] = 1 - 2.0 ** -24
+    if draft:
+        q[5] = p[5]                              # residuals that are empty up to rounding
+        q[2] = 0; q[2, :, 69] = 1
+    verify_check(dev, tokens, par, n, p, u, q)
+    # parents that point forward or outside are never reached
+    par[0, 1:] = torch.tensor([5, -7, 3])
+    verify_check(dev, tokens, par, n, p, u, q)
+
+
+def test_verify_strided_rows(dev):
+    from fxlm import verify_tree
+    tokens, par, n, p, u, q = verify_inputs(4, 6, 333, True, seed=3)
+    both = torch.empty(4, 6, 2, 340)
+    both[:, :, 0, 3:336], both[:, :, 1, 3:336] = p, q
+    both = both.to(dev)
+    want = verify_tree(tokens.to(dev), par.to(dev), n.to(dev), p.to(dev), u.to(dev), draft_probs=q.to(dev))
+    got = verify_tree(tokens.to(dev), par.to(dev), n.to(dev), both[:, :, 0, 3:336], u.to(dev),
+                      draft_probs=both[:, :, 1, 3:336])
+    for x, y in zip(want, got):
+        assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("draft", [False, True])
+def test_verify_keeps_the_target_distribution(dev, draft):
+    # the token after the root (accepted draft or drawn) follows the target, whatever was drafted:
+    # 5 standard deviations of a binomial count, over 8 tokens
+    from fxlm import verify_tree
+    B, T, V = 40000, 4, 8
+    g = torch.Generator(device=dev).manual_seed(5)
+    p0 = torch.softmax(torch.randn(V, generator=g, device=dev) * 1.5, -1)
+    q0 = torch.softmax(torch.randn(V, generator=g, device=dev) * 1.5, -1)
+    par = torch.tensor([[-1, 0, 0, 0]], dtype=torch.int32, device=dev).expand(B, T).contiguous()
+    tokens = torch.multinomial(q0.expand(B, V), T, replacement=True, generator=g)
+    if not draft:
+        tokens[:, 1:] = torch.topk(q0, 3).indices
+    p = p0.expand(B, T, V)
+    path, n_path, nxt = verify_tree(tokens, par, torch.full((B,), T, dtype=torch.int32, device=dev),
+                                    p, torch.rand(B, T, generator=g, device=dev),
+                                    draft_probs=q0.expand(B, T, V) if draft else None)
+    first = torch.where(n_path > 1, tokens.gather(1, path[:, 1:2].clamp(min=0).long())[:, 0], nxt)
+    count = torch.bincount(first, minlength=V).double()
+    sigma = (B * p0.double() * (1 - p0.double())).sqrt()
+    assert ((count - B * p0.double()).abs() <= 5 * sigma).all()
+    assert (n_path > 1).float().mean() > 0.2
+
+
+# ------------------------------------------------------------------ pages
+class PlainPages:
+    """The page table as lists, one row and one page at a time."""
+
+    def __init__(self, c):
+        self.k, self.v = c["k"].clone(), c["v"].clone()
+        self.W, self.page = c["table"].shape[1], c["page"]
+        self.lens = c["lens"].tolist()
+        self.rows = [c["table"][s, :h].tolist() for s, h in enumerate(c["n_pages"].tolist())]
+        self.ref = c["ref"].tolist()
+
+    def free(self):
+        return [p for p, r in enumerate(self.ref) if r == 0]
+
+    def commit(self, path, n_path, room):
+        P = self.page
+        for s, row in enumerate(self.rows):
+            n = n_path[s] if path is not None else 0
+            for i in range(n):
+                a, b = self.lens[s] + path[s][i], self.lens[s] + i
+                for x in (self.k, self.v):
+                    x[:, row[b // P], :, b % P] = x[:, row[a // P], :, a % P].clone()
+            self.lens[s] += n
+        want = [max(0, min(self.W, -(-(self.lens[s] + r) // P)) - len(self.rows[s])) if r > 0 else 0
+                for s, r in enumerate(room)]
+        free = self.free()
+        if sum(want) > len(free):
+            return False
+        for s, w in enumerate(want):
+            for _ in range(w):
+                p = free.pop(0)
+                self.rows[s].append(p)
+                self.ref[p] = 1
+        return True
+
+    def fork(self, parents):
+        P, free = self.page, self.free()
+        kept = {p for s, p in enumerate(parents) if p == s}
+        rows, lens = [], []
+        copies = []
+        for s, p in enumerate(parents):
+            n = self.lens[p] if p >= 0 else 0
+            row = list(self.rows[p][:-(-n // P)]) if p >= 0 else []
+            if n % P and p != s:
+                if p in kept:
+                    if not free:
+                        return False
+                    new = free.pop(0)
+                    copies.append((row[-1], new, n % P))
+                    row[-1] = new
+                else:
+                    kept.add(p)
+            rows.append(row)
+            lens.append(n)
+        for a, b, n in copies:
+            for x in (self.k, self.v):
+                x[:, b, :, :n] = x[:, a, :, :n]
+        self.rows, self.lens = rows, lens
+        self.ref = [0] * len(self.ref)
+        for row in rows:
+            for p in row:
+                self.ref[p] += 1
+        return True
+
+
+def cache(dev, dtype, S, L, H, D, page, lens, extra, P=None, seed=0, W=None):
+    g = torch.Generator(device=dev).manual_seed(seed)
+    rng = np.random.RandomState(seed)
+    held = [-(-(n + extra) // page) for n in lens]
+    P = sum(held) + S + 4 if P is None else P
+    W = max(held) + 5 if W is None else W
+    order, at = rng.permutation(P), 0
+    table, ref = np.full((S, W), -1, np.int32), np.zeros(P, np.int32)
+    for s, h in enumerate(held):
+        table[s, :h] = order[at:at + h]
+        ref[order[at:at + h]] = 1
+        at += h
+    both = torch.randn(L, P, 2, H, page, D, generator=g, device=dev).to(dtype)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    return dict(k=both[:, :, 0], v=both[:, :, 1], table=torch.from_numpy(table).to(dev), n_pages=i32(held),
+                lens=i32(lens), ref=torch.from_numpy(ref).to(dev), page=page)
+
+
+def same(c, want, lens):
+    torch.cuda.synchronize()
+    assert lens.tolist() == want.lens
+    assert c["n_pages"].tolist() == [len(r) for r in want.rows]
+    assert c["ref"].tolist() == want.ref
+    W = want.W
+    assert c["table"].tolist() == [r + [-1] * (W - len(r)) for r in want.rows]
+    assert torch.equal(c["k"], want.k) and torch.equal(c["v"], want.v)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("S,L,H,D,page,lens,T", [
+    (1, 1, 1, 64, 16, [0], 1), (1, 3, 2, 64, 16, [15], 8), (4, 2, 3, 128, 32, [0, 31, 32, 100], 9),
+    (3, 12, 12, 64, 16, [500, 7, 64], 64), (6, 1, 5, 8, 64, [1, 2, 3, 63, 64, 65], 17),
+    (2, 2, 2, 128, 256, [250, 300], 33)])
+def test_commit(dev, dtype, S, L, H, D, page, lens, T):
+    from fxlm import kv_commit
+    rng = np.random.RandomState(T)
+    c = cache(dev, dtype, S, L, H, D, page, lens, T, seed=T)
+    want = PlainPages(c)
+    n = [int(rng.randint(0, T + 1)) for _ in range(S)]
+    n[-1] = T if S > 1 else n[-1]
+    path = [sorted(rng.permutation(T)[:k].tolist()) + [-1] * (T - k) for k in n]
+    room = [int(rng.choice([0, 1, page, 3 * page])) for _ in range(S)]
+    room[0] = T
+    assert want.commit(path, n, room)
+    old = c["lens"].clone()
+    lens_out = kv_commit(c["k"], c["v"], c["table"], c["n_pages"], c["lens"], c["ref"],
+                         torch.tensor(path, dtype=torch.int32, device=dev),
+                         torch.tensor(n, dtype=torch.int32, device=dev),
+                         room=torch.tensor(room, dtype=torch.int32, device=dev))
+    same(c, want, lens_out)
+    assert torch.equal(c["lens"], old)
+
+
+@pytest.mark.parametrize("S,P", [(1, 5), (600, 4000), (3, 70001)])
+def test_reserve(dev, S, P):
+    from fxlm import kv_reserve
+    rng = np.random.RandomState(S)
+    lens = [int(rng.randint(0, 40)) for _ in range(S)] if S > 1 else [0]
+    c = cache(dev, BF16, S, 1, 1, 8, 16, lens, 0, P=P, seed=S, W=max(5, P // 10))
+    want = PlainPages(c)
+    room = [int(rng.randint(0, 50)) for _ in range(S)] if S > 1 else [80]
+    assert want.commit(None, None, room)
+    kv_reserve(c["table"], c["n_pages"], c["lens"], c["ref"], torch.tensor(room, dtype=torch.int32, device=dev), 16)
+    same(c, want, c["lens"])
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("S,L,H,D,page,lens,parents", [
+    (1, 1, 1, 64, 16, [5], [0]), (2, 2, 3, 64, 16, [5, 40], [1, 1]), (2, 1, 1, 64, 16, [0, 16], [1, 0]),
+    (5, 3, 2, 128, 32, [33, 64, 7, 0, 100], [4, 4, 0, 2, 2]), (4, 2, 2, 64, 128, [100, 300, 128, 5], [1, 2, 3, 0]),
+    (6, 12, 12, 64, 16, [500, 3, 9, 77, 16, 1], [0, 0, -1, 0, 3, -1]), (3, 1, 1, 8, 256, [1, 2, 3], [-1, -1, -1])])
+def test_fork(dev, dtype, S, L, H, D, page, lens, parents):
+    from fxlm import kv_fork
+    c = cache(dev, dtype, S, L, H, D, page, lens, 3, seed=S + L)
+    want = PlainPages(c)
+    par = torch.tensor(parents, dtype=torch.int32, device=dev)
+    for _ in range(3):  # forks of forks: shared pages, freed pages that come back
+        assert want.fork(parents)
+        kv_fork(c["k"], c["v"], c["table"], c["n_pages"], c["lens"], c["ref"], par)
+        same(c, want, c["lens"])
+
+
+def test_fork_many_rows(dev):
+    from fxlm import kv_fork
+    rng = np.random.RandomState(2)
+    S = 700
+    c = cache(dev, BF16, S, 2, 1, 16, 16, [int(rng.randint(0, 60)) for _ in range(S)], 2, P=6000, seed=1)
+    want = PlainPages(c)
+    parents = [int(rng.randint(-1, S)) for _ in range(S)]
+    assert want.fork(parents)
+    kv_fork(c["k"], c["v"], c["table"], c["n_pages"], c["lens"], c["ref"],
+            torch.tensor(parents, dtype=torch.int32, device=dev))
+    same(c, want, c["lens"])
+
+
+def test_calls_that_do_not_fit_change_nothing(dev):
+    from fxb200 import _lib
+    from fxlm import kv_commit, kv_fork, kv_reserve
+    c = cache(dev, BF16, 3, 2, 2, 64, 16, [20, 30, 7], 2, P=6, seed=1, W=6)  # 5 pages held, one free
+    want = PlainPages(c)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    args = (c["table"], c["n_pages"], c["lens"], c["ref"])
+
+    def refused():
+        with pytest.raises(RuntimeError, match="KV cache"):
+            _lib.raise_on_device_error()
+        same(c, want, c["lens"])
+
+    kv_reserve(*args, i32([0, 20, 20]), 16)              # two pages wanted
+    refused()
+    kv_fork(c["k"], c["v"], *args, i32([0, 0, 0]))       # two copies wanted
+    refused()
+    kv_fork(c["k"], c["v"], *args, i32([0, 3, 2]))       # no such row
+    refused()
+    kv_fork(c["k"], c["v"], *args, i32([0, -2, 2]))
+    refused()
+    kv_reserve(*args, i32([100, 0, 0]), 16)              # longer than a row of the table: 6 - 2 pages wanted
+    refused()
+    for path in ([[1, 0], [0, 1], [0, 1]], [[0, 0], [0, 1], [0, 1]], [[0, 2], [0, 1], [0, 1]], [[-1, 1], [0, 1], [0, 1]]):
+        kv_commit(c["k"], c["v"], *args, i32(path), i32([2, 0, 0]))
+        got = c["k"].clone()
+        with pytest.raises(RuntimeError, match="KV cache"):
+            _lib.raise_on_device_error()
+        del got
+    kv_reserve(*args, i32([0, 3, 0]), 16)                # one page: fits
+    assert want.commit(None, None, [0, 3, 0])
+    assert c["ref"].tolist() == want.ref
+
+
+def test_page_calls_in_a_graph(dev):
+    from fxlm import kv_commit, kv_fork
+    c = cache(dev, BF16, 3, 2, 2, 64, 16, [20, 30, 7], 8, P=40, seed=1)
+    want = PlainPages(c)
+    path = torch.tensor([[0, 2, 5, -1]] * 3, dtype=torch.int32, device=dev)
+    n = torch.tensor([3, 2, 0], dtype=torch.int32, device=dev)
+    room = torch.full((3,), 8, dtype=torch.int32, device=dev)
+    par = torch.tensor([1, 1, 0], dtype=torch.int32, device=dev)
+    args = (c["k"], c["v"], c["table"], c["n_pages"], c["lens"], c["ref"])
+    path8 = torch.cat([path, torch.full((3, 4), -1, dtype=torch.int32, device=dev)], 1)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        new = kv_commit(*args, path8, n, room=room)
+        c["lens"].copy_(new)
+        kv_fork(*args, par)
+    for _ in range(3):
+        assert want.commit(path8.tolist(), n.tolist(), room.tolist())
+        assert want.fork(par.tolist())
+        # fork drops the room that commit made: give it back before the next replay
+        g.replay()
+        same(c, want, c["lens"])
+        from fxlm import kv_reserve
+        kv_reserve(c["table"], c["n_pages"], c["lens"], c["ref"], room, 16)
+        want.commit(None, None, room.tolist())

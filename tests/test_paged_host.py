@@ -1,0 +1,158 @@
+"""CPU: refusals of the generation operators (C ABI and Python wrappers) and
+the host-side helpers of fxlm.paged. No kernel runs here."""
+import ctypes
+
+import pytest
+import torch
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from fxb200 import _lib
+    return _lib.load()
+
+
+def err():
+    from fxb200 import _lib
+    return _lib.last_error()
+
+
+def tree_args(**kw):
+    from fxb200 import _lib
+    a = _lib.TreeAttnArgs()
+    a.dtype, a.B, a.T, a.Hq, a.Hkv, a.D, a.page, a.P, a.W, a.scale = 2, 1, 4, 4, 2, 64, 16, 8, 4, 0.125
+    a.q = a.k = a.v = a.o = a.k_pages = a.v_pages = 256
+    a.table = a.lens = a.n_nodes = a.mask = 256
+    a.table_sb, a.mask_sb = 4, 4
+    for n in ("q", "k", "v", "o"):
+        for s in ("sb", "st", "sh"):
+            setattr(a, f"{n}_{s}", 64)
+    for n in ("kp", "vp"):
+        for s in ("sp", "sh", "st"):
+            setattr(a, f"{n}_{s}", 64)
+    for n, x in kw.items():
+        setattr(a, n, x)
+    return a
+
+
+def test_struct_layouts_match(lib):
+    from fxb200 import _lib
+    assert lib.fxb_abi_struct_size(2) == ctypes.sizeof(_lib.TreeAttnArgs)
+    assert lib.fxb_abi_struct_size(3) == ctypes.sizeof(_lib.KvArgs)
+
+
+@pytest.mark.parametrize("change,word", [
+    (dict(D=96), "head_dim 96"), (dict(T=65), "T=65"), (dict(T=0), "T=0"), (dict(Hq=5), "Hq=5"), (dict(B=0), "B=0"),
+    (dict(page=24), "page 24"), (dict(page=512), "page 512"), (dict(page=8), "page 8"), (dict(P=0), "P=0"),
+    (dict(W=0), "W=0"), (dict(table_sb=3), "row stride"), (dict(mask_sb=3), "row stride"), (dict(q=264), "aligned"),
+    (dict(k_pages=0), "aligned"), (dict(mask=0), "NULL"), (dict(q_sh=12), "strides"), (dict(vp_st=-64), "strides"),
+    (dict(scale=0.0), "scale"), (dict(scale=float("inf")), "scale"), (dict(scale=float("nan")), "scale")])
+def test_tree_attn_refuses(lib, change, word):
+    assert lib.fxb_tree_attn(ctypes.byref(tree_args(**change)), None) == -1
+    assert word in err()
+
+
+def test_tree_attn_refuses_dtype_and_null(lib):
+    assert lib.fxb_tree_attn(ctypes.byref(tree_args(dtype=7)), None) == -2
+    assert lib.fxb_tree_attn(None, None) == -1
+
+
+def kv_args(**kw):
+    from fxb200 import _lib
+    a = _lib.KvArgs()
+    a.elem_size, a.L, a.P, a.H, a.page, a.D, a.S, a.W = 2, 2, 8, 2, 16, 64, 2, 4
+    a.k = a.v = a.table = a.n_pages = a.lens = a.ref = 256
+    a.table_ss = 4
+    for n in ("k", "v"):
+        for s in ("sl", "sp", "sh", "st"):
+            setattr(a, f"{n}_{s}", 64)
+    for n, x in kw.items():
+        setattr(a, n, x)
+    return a
+
+
+@pytest.mark.parametrize("change,word", [
+    (dict(page=20), "page 20"), (dict(S=0), "S=0"), (dict(S=5000), "S=5000"), (dict(W=0), "W=0"), (dict(P=0), "P=0"),
+    (dict(table=0), "NULL"), (dict(table_ss=3), "row stride"), (dict(elem_size=1), "elem_size"), (dict(D=12), "D=12"),
+    (dict(L=0), "L=0"), (dict(k=8), "aligned"), (dict(k_st=4), "strides"), (dict(v_sp=-64), "strides")])
+def test_kv_calls_refuse(lib, change, word):
+    a = kv_args(**change)
+    p = ctypes.c_void_p(512)
+    assert lib.fxb_kv_commit(ctypes.byref(a), p, 4, 4, p, None, p, None) == -1
+    assert word in err()
+    assert lib.fxb_kv_fork(ctypes.byref(a), p, p, None) == -1
+    assert word in err()
+
+
+def test_kv_calls_refuse_their_own_arguments(lib):
+    p, a = ctypes.c_void_p(512), kv_args()
+    assert lib.fxb_kv_commit(ctypes.byref(a), p, 4, 4, p, None, ctypes.c_void_p(256), None) == -1  # lens_out is lens
+    assert "lens_out" in err()
+    assert lib.fxb_kv_commit(ctypes.byref(a), p, 65, 65, p, None, p, None) == -1 and "T=65" in err()
+    assert lib.fxb_kv_commit(ctypes.byref(a), p, 4, 4, None, None, p, None) == -1
+    assert lib.fxb_kv_fork(ctypes.byref(a), None, p, None) == -1
+    assert lib.fxb_kv_fork(ctypes.byref(a), p, ctypes.c_void_p(8), None) == -1
+    assert lib.fxb_kv_commit(None, p, 4, 4, p, None, p, None) == -1
+    assert lib.fxb_kv_fork_workspace(0, 3) == 0
+
+
+def test_verify_refuses(lib):
+    p = ctypes.c_void_p(256)
+
+    def call(B=1, T=2, V=8, tokens=p, q=None, p_st=8, q_st=8):
+        return lib.fxb_verify_tree(tokens, p, p, p, 16, p_st, q, 16, q_st, p, p, p, p, B, T, V, None)
+
+    for kw in (dict(B=0), dict(T=65), dict(T=0), dict(V=0), dict(tokens=None), dict(p_st=-1), dict(q=p, q_st=-1)):
+        assert call(**kw) == -1 and "fxb_verify_tree" in err()
+
+
+def test_wrappers_refuse_on_the_host():
+    from fxlm import kv_commit, kv_fork, kv_reserve, tree_attention, verify_tree
+    bf = torch.bfloat16
+    q = torch.zeros(1, 2, 4, 64, dtype=bf)
+    kv = torch.zeros(1, 2, 2, 64, dtype=bf)
+    pages = torch.zeros(4, 2, 16, 64, dtype=bf)
+    i = torch.zeros(1, dtype=torch.int32)
+    rest = (i[:, None], i, i, torch.zeros(1, 2, dtype=torch.int64))
+    with pytest.raises(TypeError, match="cuda"):
+        tree_attention(q, kv, kv, pages, pages, *rest)
+    with pytest.raises(TypeError, match="share"):
+        tree_attention(q, kv.float(), kv, pages, pages, *rest)
+    with pytest.raises(TypeError, match="share"):
+        tree_attention(q.double(), kv.double(), kv.double(), pages.double(), pages.double(), *rest)
+    with pytest.raises(ValueError, match="head_dim 32"):
+        tree_attention(q[..., :32], kv[..., :32], kv[..., :32], pages[..., :32], pages[..., :32], *rest)
+    with pytest.raises(ValueError, match="shape mismatch"):
+        tree_attention(q[:, :, :3], kv, kv, pages, pages, *rest)
+    with pytest.raises(ValueError, match="T=65"):
+        z = torch.zeros(1, 65, 2, 64, dtype=bf)
+        tree_attention(z, z, z, pages, pages, *rest)
+    with pytest.raises(ValueError, match="pages"):
+        tree_attention(q, kv, kv, pages, pages[:2], *rest)
+    with pytest.raises(ValueError):
+        tree_attention(q[0], kv, kv, pages, pages, *rest)
+    p = torch.zeros(1, 2, 8)
+    with pytest.raises(TypeError, match="cuda"):
+        verify_tree(torch.zeros(1, 2, dtype=torch.int64), i, i, p, p[..., 0])
+    with pytest.raises(ValueError, match="T=65"):
+        verify_tree(torch.zeros(1, 65, dtype=torch.int64), i, i, p, p[..., 0])
+    with pytest.raises(ValueError):
+        verify_tree(torch.zeros(2, dtype=torch.int64), i, i, p, p[..., 0])
+    pool = torch.zeros(2, 4, 2, 16, 64, dtype=bf)
+    args = (i[:, None], i, i, torch.zeros(4, dtype=torch.int32))
+    with pytest.raises(TypeError, match="cuda"):
+        kv_commit(pool, pool, *args, i[:, None], i)
+    with pytest.raises(TypeError, match="cuda"):
+        kv_fork(pool, pool, *args, i)
+    with pytest.raises(TypeError, match="cuda"):
+        kv_reserve(*args, i, 16)
+
+
+def test_tree_masks():
+    from fxlm import tree_masks
+    par = torch.tensor([[-1, 0, 0, 1, 3], [-1, 0, 1, 2, 3]], dtype=torch.int32)
+    assert tree_masks(par).tolist() == [[1, 3, 5, 11, 27], [1, 3, 7, 15, 31]]
+    chain = torch.arange(-1, 63, dtype=torch.int32)[None]
+    assert tree_masks(chain)[0, -1].item() == -1 and tree_masks(chain)[0, 62].item() == 2 ** 63 - 1
+    with pytest.raises(ValueError):
+        tree_masks(torch.zeros(1, 65, dtype=torch.int32))
