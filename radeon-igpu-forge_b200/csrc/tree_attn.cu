@@ -2,120 +2,774 @@
 // No reference counterpart: its sampler keeps no cache (ml/fxlm/sample.py:63-73).
 //
 // o = softmax(scale * q k^T) v over the context slots and the visible nodes,
-// computed online: a running maximum m, sum l and output O are rescaled by
-// exp(m_old - m_new) when the maximum rises, in fp32.
+// computed in one pass over the keys: a running maximum m, sum l and output O
+// per row, rescaled by 2^(m_old - m_new) when the maximum rises. States of
+// different parts of the keys join the same way, so a sequence can be divided
+// at will.
+//
+// Work. An item is (batch row, key head, row tile): the R = T * G query rows
+// of a key head (G query heads share it; row r is node r / G, head r % G),
+// cut into tiles of rows. An item's keys are its context in blocks of 64 slots
+// and one block of nodes. All items' blocks in a row are divided evenly over
+// the thread blocks, so uneven lengths cost nothing; an item that several
+// thread blocks share is joined by the one that finishes last, from states in
+// the workspace, in the order of the keys (the result does not depend on who
+// that is).
 #include "common.cuh"
 #include "internal.h"
 
 namespace {
 
 constexpr int kMaxTree = 64;
+constexpr int kBlockKeys = 64;          // keys of a block
+constexpr int kWarps = 4;               // each takes 16 keys of a block
+constexpr int kThreads = kWarps * 32;
+constexpr int kRows = 16;               // rows of a tile
+constexpr int kTile = 16;               // keys a warp takes at once
+constexpr float kRescaleLog2 = 8.f;     // see softmax_rows
+constexpr int kMaxGrid = 1024;          // arrival counters in the workspace
 
-template <typename T>
+FXB_DEV float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 struct Params {
-  int B, T_, Hq, Hkv, G, page_shift, P, W;
+  int B, T, Hq, Hkv, G, R, RT, page_shift, P, W;
   float scale_log2;
-  const T *q, *k, *v;
-  T *o, *kp, *vp;
-  int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh, o_sb, o_st, o_sh;
+  const void* q;
+  void *o, *kp, *vp;
+  int64_t q_sb, q_st, q_sh, o_sb, o_st, o_sh;
   int64_t kp_sp, kp_sh, kp_st, vp_sp, vp_sh, vp_st;
   const int32_t* table;
   int64_t table_sb;
   const int32_t *lens, *n_nodes;
   const int64_t* mask;
   int64_t mask_sb;
+  unsigned* arrived;  // workspace: kMaxGrid counters,
+  float* parts;       // then two states for every thread block
   int* err;
 };
 
-// One warp per (row b, node t, query head): lanes hold D / 32 elements each.
-template <typename T, int D>
-__global__ void __launch_bounds__(128) tree_attn_simple(const Params<T> a) {
-  constexpr int E = D / 32;
-  pdl_trigger();
-  pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (w >= (int64_t)a.B * a.T_ * a.Hq) return;
-  const int h = (int)(w % a.Hq);
-  const int t = (int)(w / a.Hq % a.T_), b = (int)(w / a.Hq / a.T_);
-  const int hk = h / a.G, page = 1 << a.page_shift;
-  T* o = a.o + b * a.o_sb + t * a.o_st + h * a.o_sh + lane * E;
-  const int n_in = a.n_nodes[b], n = min(max(n_in, 0), a.T_);
-  if (n != n_in && lane == 0) atomicOr(a.err, FXB_DERR_PAGES);
-  float acc[E] = {}, q[E];
-  float m = -INFINITY, l = 0.f;
-  if (t < n) {
-    int64_t len = a.lens[b];
-    if (len < 0 || len > ((int64_t)a.W << a.page_shift)) {
-      if (lane == 0) atomicOr(a.err, FXB_DERR_PAGES);
-      len = len < 0 ? 0 : (int64_t)a.W << a.page_shift;
-    }
-    const int32_t* table = a.table + b * a.table_sb;
-    const T* k = a.k + b * a.k_sb + hk * a.k_sh + lane * E;
-    const T* v = a.v + b * a.v_sb + hk * a.v_sh + lane * E;
-    if (h == hk * a.G) {  // this node's key and value go into the cache
-      const int64_t at = len + t, pi = at >> a.page_shift;
-      const int pg = pi < a.W ? table[pi] : -1;
-      if (pg < 0 || pg >= a.P) {
-        if (lane == 0) atomicOr(a.err, FXB_DERR_PAGES);
-      } else {
-        T* kd = a.kp + pg * a.kp_sp + hk * a.kp_sh + (at & (page - 1)) * a.kp_st + lane * E;
-        T* vd = a.vp + pg * a.vp_sp + hk * a.vp_sh + (at & (page - 1)) * a.vp_st + lane * E;
+// ------------------------------------------------------------------ division of the work
+struct Row {  // a batch row
+  int len, n, blocks;
+};
+FXB_DEV Row row_of(const Params& a, int b) {
+  const int len_in = a.lens[b], n_in = a.n_nodes[b];
+  const int64_t most = (int64_t)a.W << a.page_shift;
+  Row r;
+  r.len = len_in < 0 ? 0 : (len_in > most ? (int)most : len_in);
+  r.n = min(max(n_in, 0), a.T);
+  if (r.len != len_in || r.n != n_in) atomicOr(a.err, FXB_DERR_PAGES);
+  if (r.n == 0) r.len = 0;  // nothing to compute: the block of nodes writes zeros
+  r.blocks = (r.len + kBlockKeys - 1) / kBlockKeys + 1;
+  return r;
+}
+
+// inclusive prefix sum over the block's threads; *total for everyone
+FXB_DEV int64_t block_scan(int64_t v, int64_t* total) {
+  __shared__ int64_t warp_total[kWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          kd[e] = k[t * a.k_st + e];
-          vd[e] = v[t * a.v_st + e];
-        }
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-      q[e] = to_f<T>(a.q[b * a.q_sb + t * a.q_st + h * a.q_sh + lane * E + e]) * a.scale_log2;
-    const uint64_t see = (uint64_t)a.mask[b * a.mask_sb + t];
-    for (int64_t j = 0; j < len + n; ++j) {
-      const T *kj, *vj;
-      if (j < len) {
-        const int pg = table[j >> a.page_shift];
-        if (pg < 0 || pg >= a.P) {
-          if (lane == 0) atomicOr(a.err, FXB_DERR_PAGES);
-          continue;
-        }
-        kj = a.kp + pg * a.kp_sp + hk * a.kp_sh + (j & (page - 1)) * a.kp_st + lane * E;
-        vj = a.vp + pg * a.vp_sp + hk * a.vp_sh + (j & (page - 1)) * a.vp_st + lane * E;
-      } else {
-        const int i = (int)(j - len);
-        if (!((see >> i) & 1)) continue;
-        kj = k + i * a.k_st;
-        vj = v + i * a.v_st;
-      }
-      float s = 0.f;
-#pragma unroll
-      for (int e = 0; e < E; ++e) s = fmaf(q[e], to_f<T>(kj[e]), s);
-      s = warp_sum(s);
-      if (s == -INFINITY) continue;  // weight 0
-      const float mn = fmaxf(m, s);
-      const float r = m == mn ? 1.f : exp2f(m - mn), p = exp2f(s - mn);
-      m = mn;
-      l = fmaf(l, r, p);
-#pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] = fmaf(acc[e], r, p * to_f<T>(vj[e]));
-    }
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += y;
   }
-  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // no visible key: zeros; NaN stays
+  __syncthreads();
+  if (lane == 31) warp_total[warp] = v;
+  __syncthreads();
+  int64_t all = 0;
 #pragma unroll
-  for (int e = 0; e < E; ++e) o[e] = from_f<T>(acc[e] * inv);
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) v += warp_total[w];
+    all += warp_total[w];
+  }
+  *total = all;
+  return v;
+}
+
+// position in the sequence of all blocks: block j of item (b, hr), hr = key head * RT + row tile
+struct Cursor {
+  int64_t u;
+  int b, hr, j;
+  Row row;
+};
+FXB_DEV void next(const Params& a, Cursor& c, int64_t end) {
+  ++c.u;
+  if (++c.j < c.row.blocks) return;
+  c.j = 0;
+  if (++c.hr < a.Hkv * a.RT) return;
+  c.hr = 0;
+  ++c.b;
+  if (c.u < end) c.row = row_of(a, c.b);
+}
+
+// This thread block's share [c.u, *end) of all *total blocks, c set to its
+// first one. No share is empty, but for thread blocks beyond the number of blocks.
+FXB_DEV int64_t sharers(int64_t total) { return total < (int64_t)gridDim.x ? total : (int64_t)gridDim.x; }
+FXB_DEV int64_t share_begin(int64_t cta, int64_t total) {
+  const int64_t g = sharers(total);
+  return cta < g ? total * cta / g : total;
+}
+FXB_DEV Cursor share(const Params& a, int64_t* end, int64_t* total) {
+  __shared__ int s_b;
+  __shared__ int64_t s_rest;
+  const int per = a.Hkv * a.RT, tid = threadIdx.x;
+  int64_t n = 0, mine = 0, incl = 0;
+  for (int b0 = 0; b0 < a.B; b0 += kThreads) {
+    const int b = b0 + tid;
+    mine = b < a.B ? (int64_t)row_of(a, b).blocks * per : 0;
+    int64_t all;
+    incl = block_scan(mine, &all) + n;
+    n += all;
+  }
+  Cursor c;
+  c.u = share_begin(blockIdx.x, n);
+  *end = share_begin(blockIdx.x + 1, n);
+  *total = n;
+  if (c.u >= *end) return c;
+  if (a.B > kThreads) n = 0;
+  for (int b0 = 0; b0 < a.B; b0 += kThreads) {
+    const int b = b0 + tid;
+    if (a.B > kThreads) {
+      mine = b < a.B ? (int64_t)row_of(a, b).blocks * per : 0;
+      int64_t all;
+      incl = block_scan(mine, &all) + n;
+      n += all;
+    }
+    if (c.u < incl && c.u >= incl - mine) {
+      s_b = b;
+      s_rest = c.u - (incl - mine);
+    }
+    if (a.B > kThreads && n > c.u) break;
+  }
+  __syncthreads();
+  c.b = s_b;
+  c.row = row_of(a, c.b);
+  c.hr = (int)(s_rest / c.row.blocks);
+  c.j = (int)(s_rest - (int64_t)c.hr * c.row.blocks);
+  return c;
+}
+// the thread block that owns block u
+FXB_DEV int owner(int64_t u, int64_t total) { return (int)(((u + 1) * sharers(total) - 1) / total); }
+
+// ------------------------------------------------------------------ joining states
+// State of an item's part in the workspace: m and l of each row, then O.
+// A thread block has two places: 1 for an item that it begins, 0 for one that
+// it continues. The counter of an item is that of the block that begins it.
+template <int ROWS, int D>
+FXB_DEV float* part_of(const Params& a, int cta, int place) {
+  return a.parts + ((int64_t)cta * 2 + place) * ROWS * (D + 2);
 }
 
 template <typename T, int D>
-int launch(const fxb_tree_attn_args* a, int shift, int* err, void* stream) {
-  Params<T> p = {a->B, a->T, a->Hq, a->Hkv, a->Hq / a->Hkv, shift, a->P, a->W, a->scale * 1.4426950408889634f,
-                 static_cast<const T*>(a->q), static_cast<const T*>(a->k), static_cast<const T*>(a->v),
-                 static_cast<T*>(a->o), static_cast<T*>(a->k_pages), static_cast<T*>(a->v_pages),
-                 a->q_sb, a->q_st, a->q_sh, a->k_sb, a->k_st, a->k_sh, a->v_sb, a->v_st, a->v_sh,
-                 a->o_sb, a->o_st, a->o_sh, a->kp_sp, a->kp_sh, a->kp_st, a->vp_sp, a->vp_sh, a->vp_st,
-                 a->table, a->table_sb, a->lens, a->n_nodes, a->mask, a->mask_sb, err};
-  const int64_t warps = (int64_t)a->B * a->T * a->Hq;
-  fxb::pdl_launch(tree_attn_simple<T, D>, dim3((unsigned)((warps + 3) / 4)), dim3(128), 0, fxb::as_stream(stream), p);
+FXB_DEV void write_out(const Params& a, int b, int hk, int r, int d, float4 o, float l) {
+  if (r >= a.R) return;
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // no visible key: zeros; NaN stays
+  const int t = r / a.G, h = hk * a.G + (r - t * a.G);
+  T* p = static_cast<T*>(a.o) + b * a.o_sb + t * a.o_st + h * a.o_sh + d;
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(p) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+  } else {
+    *reinterpret_cast<uint2*>(p) = make_uint2(pack2<T>(o.x * inv, o.y * inv), pack2<T>(o.z * inv, o.w * inv));
+  }
+}
+FXB_DEV void axpy4(float4& o, float w, const float4& x) {
+  o.x = fmaf(w, x.x, o.x);
+  o.y = fmaf(w, x.y, o.y);
+  o.z = fmaf(w, x.z, o.z);
+  o.w = fmaf(w, x.w, o.w);
+}
+// weight of a state with maximum m in a join with maximum mx
+FXB_DEV float weight(float m, float mx) { return m == -INFINITY ? 0.f : ex2(m - mx); }
+
+// Called by all threads after this thread block's part is written: the last
+// one to arrive joins the parts and writes the item's rows.
+template <typename T, int ROWS, int D>
+FXB_DEV void join_parts(const Params& a, int b, int hk, int row0, int64_t u_first, int64_t u_last, int64_t total) {
+  __shared__ int last;
+  const int lo = owner(u_first, total), hi = owner(u_last, total);
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const unsigned before = atomicAdd(&a.arrived[lo], 1u);
+    last = before == (unsigned)(hi - lo);
+    if (last) a.arrived[lo] = 0;  // for the next call
+  }
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  for (int i = threadIdx.x; i < ROWS * (D / 4); i += kThreads) {
+    const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
+    if (row0 + r >= a.R) break;
+    float m = -INFINITY, l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int c = lo; c <= hi; ++c) {
+      const float* p = part_of<ROWS, D>(a, c, c == lo);
+      const float mc = __ldcg(p + r), lc = __ldcg(p + ROWS + r);
+      const float4 oc = __ldcg(reinterpret_cast<const float4*>(p + 2 * ROWS + r * D + d));
+      const float mx = fmaxf(m, mc);
+      const float w0 = weight(m, mx), w1 = weight(mc, mx);
+      o = make_float4(o.x * w0, o.y * w0, o.z * w0, o.w * w0);
+      axpy4(o, w1, oc);
+      l = fmaf(l, w0, lc * w1);
+      m = mx;
+    }
+    write_out<T, D>(a, b, hk, row0 + r, d, o, l);
+  }
+}
+
+// ------------------------------------------------------------------ few rows: a warp takes 16 keys at once
+template <typename T, int D> struct Shape {
+  static constexpr int kBoxCols = 128 / sizeof(T);           // columns of a 128-byte swizzled row
+  static constexpr int kBoxes = D / kBoxCols;
+  static constexpr int kOperand = kTile * D * sizeof(T);      // one warp's keys (or values)
+  static constexpr int kSlot = 2 * kOperand;                  // of one stage; >= 16 rows of O in fp32
+  static constexpr int kStages = sizeof(T) == 4 ? 3 : (D == 128 ? 3 : 6);
+  static constexpr int kQPitch = D + 4;                       // fp32: rows of Q in shared memory
+  static constexpr int kQBytes = sizeof(T) == 4 ? kRows * kQPitch * 4 : 0;
+  static constexpr int kPBytes = sizeof(T) == 4 ? kWarps * (kTile * kRows + kRows) * 4 : 0;
+  static constexpr int kSmem = 1024 + kWarps * kStages * kSlot + kQBytes + kPBytes;
+  static constexpr int kCtas = kSmem <= 112 * 1024 ? 2 : 1;   // thread blocks of an SM
+};
+// offset of element d of row r of O in a slot: 32-byte pieces exchanged by row, so that the
+// eight rows that a warp's accumulators hold at once fall into different banks
+template <int D> FXB_DEV int o_at(int r, int d) { return r * D + ((((d >> 3) ^ (r & 7)) << 3) | (d & 7)); }
+
+FXB_DEV void ldmatrix4(uint32_t addr, uint32_t* r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+FXB_DEV void ldmatrix4t(uint32_t addr, uint32_t* r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+template <typename T> FXB_DEV void mma16816(float* c, const uint32_t* a, uint32_t b0, uint32_t b1);
+template <> FXB_DEV void mma16816<__nv_bfloat16>(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <> FXB_DEV void mma16816<__half>(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// byte offset of 16-byte piece c of row r of an operand in shared memory (128-byte swizzle)
+FXB_DEV uint32_t sw(int r, int c) { return (c >> 3) * (kTile * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4); }
+
+// 16-bit types: m16n8k16 products. A lane holds, of rows lane / 4 and lane / 4
+// + 8, two columns of every eight.
+template <typename T, int D>
+struct Rows16 {
+  uint32_t q[D / 16][4];
+  float o[D / 8][4];
+  float m[2], l[2];
+  uint64_t see[2];
+  bool live[2];  // rows of nodes that exist; the others see nothing
+
+  FXB_DEV void begin(const Params& a, int b, int hk, int row0, int n, float*) {
+    const int lane = threadIdx.x & 31;
+    const T* base = static_cast<const T*>(a.q) + b * a.q_sb + 2 * (lane & 3);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = row0 + (lane >> 2) + 8 * i, t = r / a.G;
+      live[i] = r < a.R && t < n;
+      see[i] = live[i] ? (uint64_t)a.mask[b * a.mask_sb + t] : 0;
+      const T* p = base + t * a.q_st + (hk * a.G + (r - t * a.G)) * a.q_sh;
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        q[k][i] = live[i] ? *reinterpret_cast<const uint32_t*>(p + k * 16) : 0u;
+        q[k][i + 2] = live[i] ? *reinterpret_cast<const uint32_t*>(p + k * 16 + 8) : 0u;
+      }
+      m[i] = -INFINITY;
+      l[i] = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  }
+
+  // context tile: keys [0, valid) count. Tree tile (tree): the nodes
+  // node0 + j, j < valid, each for the rows that see it.
+  FXB_DEV void tile(const Params& a, uint8_t* slot, int valid, bool tree, int node0, const float*, float*) {
+    const int lane = threadIdx.x & 31;
+    const uint32_t sk = smem_u32(slot), sv = sk + Shape<T, D>::kOperand;
+    // scores of 16 rows x 16 keys; even and odd slices of D apart, for two shorter chains of products
+    float s[2][4] = {}, s1[2][4] = {};
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k) {
+      uint32_t f[4];
+      ldmatrix4(sk + sw((lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)), f);
+      mma16816<T>(k & 1 ? s1[0] : s[0], q[k], f[0], f[1]);
+      mma16816<T>(k & 1 ? s1[1] : s[1], q[k], f[2], f[3]);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int j = i * 8 + 2 * (lane & 3) + (e & 1);
+        const bool in = j < valid && (tree ? (see[e >> 1] >> (node0 + j)) & 1 : live[e >> 1]);
+        s[i][e] = in ? (s[i][e] + s1[i][e]) * a.scale_log2 : -INFINITY;
+      }
+    // The reference maximum m of a row moves only when a tile exceeds it by
+    // more than 2^8: probabilities then stay below 2^8, which fp32 sums and
+    // 16-bit probabilities hold as well as [0, 1], and O is rarely rescaled.
+    float mx[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float x = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1]));
+      x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+      mx[h] = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+    }
+    const bool up0 = mx[0] > m[0] + kRescaleLog2, up1 = mx[1] > m[1] + kRescaleLog2;
+    if (__any_sync(0xffffffffu, up0 || up1)) {
+      const float m0 = up0 ? mx[0] : m[0], m1 = up1 ? mx[1] : m[1];
+      const float r0 = up0 ? ex2(m[0] - m0) : 1.f, r1 = up1 ? ex2(m[1] - m1) : 1.f;
+      m[0] = m0;
+      m[1] = m1;
+      l[0] *= r0;
+      l[1] *= r1;
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        o[i][0] *= r0;
+        o[i][1] *= r0;
+        o[i][2] *= r1;
+        o[i][3] *= r1;
+      }
+    }
+    const float z0 = m[0] == -INFINITY ? 0.f : m[0], z1 = m[1] == -INFINITY ? 0.f : m[1];
+    uint32_t p[4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float p0 = ex2(s[i][0] - z0), p1 = ex2(s[i][1] - z0), p2 = ex2(s[i][2] - z1), p3 = ex2(s[i][3] - z1);
+      l[0] += p0 + p1;
+      l[1] += p2 + p3;
+      // the probabilities enter the second product in the inputs' type, as its operands must
+      p[2 * i] = pack2<T>(p0, p1);
+      p[2 * i + 1] = pack2<T>(p2, p3);
+    }
+    if (valid < kTile || tree) {
+      // values that no row may count are zeroed (0 * NaN is NaN): those behind
+      // the sequence, and infinities and NaN in nodes, which are then added
+      // to the rows that see them
+      uint8_t* vs = slot + Shape<T, D>::kOperand;
+      bool odd = false;
+      for (int i = lane; i < kTile * (D / 8); i += 32) {
+        const int r = i / (D / 8), c = i - r * (D / 8);
+        uint4* x = reinterpret_cast<uint4*>(vs + sw(r, c));
+        if (r >= valid) {
+          *x = make_uint4(0, 0, 0, 0);
+        } else if (tree) {
+          float f[8];
+          unpack8<T>(*x, f);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) odd |= !(fabsf(f[e]) < INFINITY);
+        }
+      }
+      __syncwarp();
+      if (__any_sync(0xffffffffu, odd)) {
+        for (int j = 0; j < valid; ++j)
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i) {
+            const float2 f = unpack2<T>(*reinterpret_cast<const uint32_t*>(vs + sw(j, i) + 4 * (lane & 3)));
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              if ((see[h] >> (node0 + j)) & 1) {
+                if (!(fabsf(f.x) < INFINITY)) o[i][2 * h] += f.x;
+                if (!(fabsf(f.y) < INFINITY)) o[i][2 * h + 1] += f.y;
+              }
+          }
+        __syncwarp();
+        for (int i = lane; i < valid * D; i += 32) {
+          T* x = reinterpret_cast<T*>(vs + sw(i / D, (i % D) / 8)) + i % 8;
+          if (!(fabsf(to_f<T>(*x)) < INFINITY)) *x = from_f<T>(0.f);
+        }
+      }
+      fence_proxy_async_smem();  // these writes come before the next copy into the stage
+      __syncwarp();
+    }
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) {
+      uint32_t f[4];
+      ldmatrix4t(sv + sw((lane & 7) + (((lane >> 3) & 1) << 3), 2 * c + (lane >> 4)), f);
+      mma16816<T>(o[2 * c], p, f[0], f[1]);
+      mma16816<T>(o[2 * c + 1], p, f[2], f[3]);
+    }
+  }
+
+  FXB_DEV void end(float* slot, float* sm, float* sl) {
+    const int lane = threadIdx.x & 31, r = lane >> 2;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float x = l[h] + __shfl_xor_sync(0xffffffffu, l[h], 1);
+      x += __shfl_xor_sync(0xffffffffu, x, 2);
+      if ((lane & 3) == 0) {
+        sm[r + 8 * h] = m[h];
+        sl[r + 8 * h] = x;
+      }
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i)
+        *reinterpret_cast<float2*>(slot + o_at<D>(r + 8 * h, i * 8 + 2 * (lane & 3))) =
+            make_float2(o[i][2 * h], o[i][2 * h + 1]);
+    }
+  }
+};
+
+// fp32: FMA. For the scores a lane holds rows 4 (lane / 8) .. + 3 and keys
+// lane % 8 and + 8; for O all 16 rows and D / 32 columns.
+template <int D>
+struct Rows32 {
+  static constexpr int C = D / 32;
+  float o[kRows][C];
+  float m[4], l[4];
+  uint64_t see[4];
+  bool live[4];
+
+  FXB_DEV void begin(const Params& a, int b, int hk, int row0, int n, float* sq) {
+    const int lane = threadIdx.x & 31;
+    __syncthreads();  // the previous item's Q has been read
+    for (int i = threadIdx.x; i < kRows * (D / 4); i += kThreads) {
+      const int rr = i / (D / 4), d = (i - rr * (D / 4)) * 4, r = row0 + rr, t = r / a.G;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (r < a.R && t < n)
+        x = *reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + b * a.q_sb + t * a.q_st +
+                                             (hk * a.G + (r - t * a.G)) * a.q_sh + d);
+      *reinterpret_cast<float4*>(sq + rr * (D + 4) + d) = x;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = row0 + (lane >> 3) * 4 + i, t = r / a.G;
+      live[i] = r < a.R && t < n;
+      see[i] = live[i] ? (uint64_t)a.mask[b * a.mask_sb + t] : 0;
+      m[i] = -INFINITY;
+      l[i] = 0.f;
+    }
+#pragma unroll
+    for (int r = 0; r < kRows; ++r)
+#pragma unroll
+      for (int c = 0; c < C; ++c) o[r][c] = 0.f;
+    __syncthreads();
+  }
+
+  FXB_DEV void tile(const Params& a, uint8_t* slot, int valid, bool tree, int node0, const float* sq, float* sp) {
+    const int lane = threadIdx.x & 31, rg = (lane >> 3) * 4, kg = lane & 7;
+    const uint8_t* vs = slot + Shape<float, D>::kOperand;
+    float s[4][2] = {};
+#pragma unroll 4
+    for (int c = 0; c < D / 4; ++c) {
+      const float4 k0 = *reinterpret_cast<const float4*>(slot + sw(kg, c));
+      const float4 k1 = *reinterpret_cast<const float4*>(slot + sw(kg + 8, c));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float4 x = *reinterpret_cast<const float4*>(sq + (rg + i) * (D + 4) + c * 4);
+        s[i][0] = fmaf(x.x, k0.x, fmaf(x.y, k0.y, fmaf(x.z, k0.z, fmaf(x.w, k0.w, s[i][0]))));
+        s[i][1] = fmaf(x.x, k1.x, fmaf(x.y, k1.y, fmaf(x.z, k1.z, fmaf(x.w, k1.w, s[i][1]))));
+      }
+    }
+    float r[4], p[4][2];
+    bool moved = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int j = kg + 8 * e;
+        const bool in = j < valid && (tree ? (see[i] >> (node0 + j)) & 1 : live[i]);
+        s[i][e] = in ? s[i][e] * a.scale_log2 : -INFINITY;
+      }
+      float x = fmaxf(s[i][0], s[i][1]);
+      x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+      x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+      x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+      const bool up = x > m[i];
+      r[i] = up ? ex2(m[i] - x) : 1.f;
+      if (up) m[i] = x;
+      moved |= up;
+      const float z = m[i] == -INFINITY ? 0.f : m[i];
+      p[i][0] = ex2(s[i][0] - z);
+      p[i][1] = ex2(s[i][1] - z);
+      l[i] = fmaf(l[i], r[i], p[i][0] + p[i][1]);
+    }
+    // probabilities by key, then the factors of the rows
+    *reinterpret_cast<float4*>(sp + kg * kRows + rg) = make_float4(p[0][0], p[1][0], p[2][0], p[3][0]);
+    *reinterpret_cast<float4*>(sp + (kg + 8) * kRows + rg) = make_float4(p[0][1], p[1][1], p[2][1], p[3][1]);
+    moved = __any_sync(0xffffffffu, moved);
+    if (moved && kg == 0) *reinterpret_cast<float4*>(sp + kTile * kRows + rg) = make_float4(r[0], r[1], r[2], r[3]);
+    __syncwarp();
+    if (moved) {
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        const float f = sp[kTile * kRows + i];
+#pragma unroll
+        for (int c = 0; c < C; ++c) o[i][c] *= f;
+      }
+    }
+    const bool some = valid < kTile || tree;  // values that count for some rows only: weight 0 is no product
+#pragma unroll 2
+    for (int j = 0; j < kTile; ++j) {
+      float v[C];
+      if constexpr (C == 4) {
+        const float4 x = *reinterpret_cast<const float4*>(vs + sw(j, lane));
+        v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+      } else {
+        const float2 x = *reinterpret_cast<const float2*>(vs + sw(j, lane >> 1) + 8 * (lane & 1));
+        v[0] = x.x; v[1] = x.y;
+      }
+#pragma unroll
+      for (int i0 = 0; i0 < kRows; i0 += 4) {
+        const float4 w = *reinterpret_cast<const float4*>(sp + j * kRows + i0);
+        const float pw[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int c = 0; c < C; ++c) {
+            const float x = fmaf(pw[i], v[c], o[i0 + i][c]);
+            o[i0 + i][c] = some && pw[i] == 0.f ? o[i0 + i][c] : x;
+          }
+      }
+    }
+    __syncwarp();
+  }
+
+  FXB_DEV void end(float* slot, float* sm, float* sl) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float x = l[i] + __shfl_xor_sync(0xffffffffu, l[i], 1);
+      x += __shfl_xor_sync(0xffffffffu, x, 2);
+      x += __shfl_xor_sync(0xffffffffu, x, 4);
+      if ((lane & 7) == 0) {
+        sm[(lane >> 3) * 4 + i] = m[i];
+        sl[(lane >> 3) * 4 + i] = x;
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < kRows; ++r)
+#pragma unroll
+      for (int c = 0; c < C; ++c) slot[o_at<D>(r, lane * C + c)] = o[r][c];
+  }
+};
+
+template <typename T, int D> struct RowsOf { using type = Rows16<T, D>; };
+template <int D> struct RowsOf<float, D> { using type = Rows32<D>; };
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads)
+tree_attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+               const __grid_constant__ CUtensorMap tmNK, const __grid_constant__ CUtensorMap tmNV, const Params a) {
+  using S = Shape<T, D>;
+  constexpr int ST = S::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t bars[kWarps][ST];
+  __shared__ float sm[kWarps][kRows], sl[kWarps][kRows];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint8_t* ring = smem + warp * ST * S::kSlot;
+  float* sq = reinterpret_cast<float*>(smem + kWarps * ST * S::kSlot);
+  float* sp = sq + S::kQBytes / 4 + warp * (kTile * kRows + kRows);
+  if (lane == 0) {
+    for (int i = 0; i < ST; ++i) mbar_init(smem_u32(&bars[warp][i]), 1);
+    fence_mbar_init();
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+    tma_prefetch_desc(&tmNK);
+    tma_prefetch_desc(&tmNV);
+  }
+  __syncwarp();
+  pdl_trigger();
+  pdl_wait();
+
+  int64_t end, total;
+  Cursor c = share(a, &end, &total);
+  if (c.u >= end) return;
+  const int64_t start = c.u;
+  Cursor f = c;          // the next block to fetch
+  int fetched = 0;       // stages filled so far, in order
+  unsigned armed = 0;    // bit s: the copy in stage s is under way, or there and not yet used
+  // page of this warp's keys of block f; read one block ahead of its use
+  auto page_of = [&]() {
+    const int slot0 = f.j * kBlockKeys + warp * kTile;
+    return f.u < end && f.j < f.row.blocks - 1 && slot0 < f.row.len
+               ? a.table[f.b * a.table_sb + (slot0 >> a.page_shift)]
+               : -1;
+  };
+  int pg = page_of();
+  auto fetch = [&]() {  // block f into stage fetched % ST; moves f on
+    if (f.u >= end) return;
+    const int s = fetched % ST;
+    const int hk = f.hr / a.RT;
+    const bool tree = f.j == f.row.blocks - 1;
+    const int at = tree ? warp * kTile : f.j * kBlockKeys + warp * kTile;
+    bool go = at < (tree ? f.row.n : f.row.len);
+    if (go && !tree && (pg < 0 || pg >= a.P)) {
+      if (lane == 0) atomicOr(a.err, FXB_DERR_PAGES);
+      go = false;
+    }
+    if (go) armed |= 1u << s;
+    if (go && lane == 0) {
+      const uint32_t bar = smem_u32(&bars[warp][s]), dst = smem_u32(ring + s * S::kSlot);
+      const int row = tree ? at : at & ((1 << a.page_shift) - 1), d3 = tree ? f.b : pg;
+      mbar_expect_tx(bar, S::kSlot);
+#pragma unroll
+      for (int x = 0; x < S::kBoxes; ++x) {
+        tma_load_4d(dst + x * kTile * 128, tree ? &tmNK : &tmK, bar, x * S::kBoxCols, row, hk, d3);
+        tma_load_4d(dst + S::kOperand + x * kTile * 128, tree ? &tmNV : &tmV, bar, x * S::kBoxCols, row, hk, d3);
+      }
+    }
+    ++fetched;
+    next(a, f, end);
+    pg = page_of();
+  };
+  for (int i = 0; i < ST; ++i) fetch();
+
+  typename RowsOf<T, D>::type rows;
+  unsigned phase = 0;    // bit s: parity of stage s
+  bool ok = true, fresh = true;
+  int64_t u_begin = 0;
+  for (int it = 0; c.u < end; ++it) {
+    const int s = it % ST, hk = c.hr / a.RT, row0 = (c.hr % a.RT) * kRows;
+    uint8_t* slot = ring + s * S::kSlot;
+    if (fresh) {
+      rows.begin(a, c.b, hk, row0, c.row.n, sq);
+      u_begin = c.u - c.j;
+      fresh = false;
+    }
+    const bool tree = c.j == c.row.blocks - 1;
+    if (ok && ((armed >> s) & 1)) {
+      ok = mbar_wait_warp(smem_u32(&bars[warp][s]), (phase >> s) & 1, a.err, FXB_DERR_ATTN_WAIT);
+      if (ok) {
+        armed &= ~(1u << s);
+        phase ^= 1u << s;
+        const int at = tree ? warp * kTile : c.j * kBlockKeys + warp * kTile;
+        const int valid = min(kTile, (tree ? c.row.n : c.row.len) - at);
+        if (tree && row0 == 0) {  // the nodes' keys and values go into the cache
+          constexpr int CH = D * (int)sizeof(T) / 16;
+          for (int i = lane; i < 2 * kTile * CH; i += 32) {
+            const int kv = i / (kTile * CH), j = (i / CH) % kTile, ch = i % CH;
+            if (j >= valid) continue;
+            const int64_t pos = (int64_t)c.row.len + at + j;
+            const int64_t pi = pos >> a.page_shift;
+            const int dst = pi < a.W ? a.table[c.b * a.table_sb + pi] : -1;
+            if (dst < 0 || dst >= a.P) {
+              atomicOr(a.err, FXB_DERR_PAGES);
+              continue;
+            }
+            const int off = (int)pos & ((1 << a.page_shift) - 1);
+            T* x = kv ? static_cast<T*>(a.vp) + dst * a.vp_sp + hk * a.vp_sh + off * a.vp_st
+                      : static_cast<T*>(a.kp) + dst * a.kp_sp + hk * a.kp_sh + off * a.kp_st;
+            reinterpret_cast<uint4*>(x)[ch] = *reinterpret_cast<const uint4*>(slot + kv * S::kOperand + sw(j, ch));
+          }
+          __syncwarp();
+        }
+        rows.tile(a, slot, valid, tree, at, sq, sp);
+      }
+    }
+    const Cursor cur = c;
+    next(a, c, end);
+    if (tree || c.u >= end) {
+      // the four warps' states join; each lies in the stage that its warp has just used up
+      __syncwarp();
+      rows.end(reinterpret_cast<float*>(slot), sm[warp], sl[warp]);
+      __syncthreads();
+      const bool begun = u_begin >= start;  // this block has the item's first keys
+      const int64_t u_last = u_begin + cur.row.blocks - 1;
+      const bool whole = begun && tree;
+      float* part = part_of<kRows, D>(a, blockIdx.x, begun);
+      for (int i = threadIdx.x; i < kRows * (D / 4); i += kThreads) {
+        const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
+        float mx = sm[0][r];
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w) mx = fmaxf(mx, sm[w][r]);
+        float l = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float wt = weight(sm[w][r], mx);
+          const float* so = reinterpret_cast<const float*>(smem + w * ST * S::kSlot + s * S::kSlot);
+          axpy4(o, wt, *reinterpret_cast<const float4*>(so + o_at<D>(r, d)));
+          l = fmaf(sl[w][r], wt, l);
+        }
+        if (whole) {
+          write_out<T, D>(a, cur.b, hk, row0 + r, d, o, l);
+        } else {
+          if (d == 0) {
+            part[r] = mx;
+            part[kRows + r] = l;
+          }
+          *reinterpret_cast<float4*>(part + 2 * kRows + r * D + d) = o;
+        }
+      }
+      if (!whole) join_parts<T, kRows, D>(a, cur.b, hk, row0, u_begin, u_last, total);
+      __syncthreads();
+      fence_proxy_async_smem();  // what was written here comes before the copies into it
+      fresh = true;
+    }
+    __syncwarp();
+    if (ok) fetch();
+  }
+  // after an expired wait copies may be under way: they land before shared memory goes
+  for (int s = 0; s < ST; ++s)
+    if ((armed >> s) & 1) mbar_wait_warp(smem_u32(&bars[warp][s]), (phase >> s) & 1, a.err, FXB_DERR_ATTN_WAIT);
+}
+
+// ------------------------------------------------------------------ host
+template <typename T> constexpr CUtensorMapDataType map_type() {
+  return sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+         : std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                          : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+}
+// (outer, heads, rows, D) view with element strides; boxes of `rows` rows of 128 bytes.
+// The stride of an axis of one entry is not used and may be anything.
+template <typename T>
+int encode(CUtensorMap* m, const void* base, int D, int rows, int64_t st, int heads, int64_t sh, int outer,
+           int64_t so, int box_rows) {
+  const uint64_t e = sizeof(T), one = D * e;
+  const uint64_t dims[4] = {(uint64_t)D, (uint64_t)rows, (uint64_t)heads, (uint64_t)outer};
+  const uint64_t strides[3] = {rows > 1 ? st * e : one, heads > 1 ? sh * e : one, outer > 1 ? so * e : one};
+  const uint32_t box[4] = {(uint32_t)(128 / e), (uint32_t)box_rows, 1, 1};
+  return fxb::encode_tiled(m, map_type<T>(), 4, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+struct Plan {
+  int grid, rows;  // thread blocks, rows of a tile
+};
+template <typename T, int D> Plan plan_rows() { return {Shape<T, D>::kCtas * fxb::num_sms(), kRows}; }
+
+Plan plan_of(int dtype, int D) {
+  if (dtype == FXB_DTYPE_F32) return D == 64 ? plan_rows<float, 64>() : plan_rows<float, 128>();
+  return D == 64 ? plan_rows<__half, 64>() : plan_rows<__half, 128>();
+}
+
+size_t workspace_bytes(const Plan& p, int D) {
+  return kMaxGrid * sizeof(unsigned) + (size_t)p.grid * 2 * p.rows * (D + 2) * sizeof(float);
+}
+
+template <typename T, int D>
+int launch(const fxb_tree_attn_args* x, const Plan& plan, Params& a, void* stream) {
+  CUtensorMap k, v, nk, nv;
+  if (int r = encode<T>(&k, x->k_pages, D, x->page, x->kp_st, x->Hkv, x->kp_sh, x->P, x->kp_sp, kTile)) return r;
+  if (int r = encode<T>(&v, x->v_pages, D, x->page, x->vp_st, x->Hkv, x->vp_sh, x->P, x->vp_sp, kTile)) return r;
+  if (int r = encode<T>(&nk, x->k, D, x->T, x->k_st, x->Hkv, x->k_sh, x->B, x->k_sb, kTile)) return r;
+  if (int r = encode<T>(&nv, x->v, D, x->T, x->v_st, x->Hkv, x->v_sh, x->B, x->v_sb, kTile)) return r;
+  a.RT = (a.R + plan.rows - 1) / plan.rows;
+  // no more thread blocks than there can be blocks of keys
+  const int64_t most = (int64_t)a.B * a.Hkv * a.RT * ((((int64_t)a.W << a.page_shift) + kBlockKeys - 1) / kBlockKeys + 1);
+  const int grid = (int)(most < plan.grid ? most : plan.grid);
+  using S = Shape<T, D>;
+  if (int r = fxb::check_cuda(
+          cudaFuncSetAttribute(tree_attn_rows<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem),
+          "fxb_tree_attn"))
+    return r;
+  fxb::pdl_launch(tree_attn_rows<T, D>, dim3(grid), dim3(kThreads), S::kSmem, fxb::as_stream(stream), k, v, nk, nv, a);
   return fxb::check_launch("fxb_tree_attn");
 }
 
@@ -123,8 +777,13 @@ int launch(const fxb_tree_attn_args* a, int shift, int* err, void* stream) {
 
 extern "C" {
 
-size_t fxb_tree_attn_workspace(int32_t, int32_t, int32_t, int32_t, int32_t, int32_t) { return 0; }
-size_t fxb_tree_attn_workspace_zeroed(int32_t, int32_t, int32_t, int32_t, int32_t, int32_t) { return 0; }
+size_t fxb_tree_attn_workspace(int32_t dtype, int32_t B, int32_t T, int32_t Hq, int32_t Hkv, int32_t D) {
+  if ((D != 64 && D != 128) || !fxb::dtype_size(dtype) || B < 1 || T < 1 || Hkv < 1 || Hq < Hkv) return 0;
+  return workspace_bytes(plan_of(dtype, D), D);
+}
+size_t fxb_tree_attn_workspace_zeroed(int32_t dtype, int32_t B, int32_t T, int32_t Hq, int32_t Hkv, int32_t D) {
+  return fxb_tree_attn_workspace(dtype, B, T, Hq, Hkv, D) ? kMaxGrid * sizeof(unsigned) : 0;
+}
 
 int fxb_tree_attn(const fxb_tree_attn_args* a, void* stream) {
   if (!a) return fxb::set_error(FXB_EINVAL, "fxb_tree_attn: args is NULL");
@@ -154,14 +813,46 @@ int fxb_tree_attn(const fxb_tree_attn_args* a, void* stream) {
       return fxb::set_error(FXB_EINVAL, "fxb_tree_attn: strides must be multiples of 16 bytes");
   if (!(a->scale > 0.f) || !(a->scale < INFINITY))
     return fxb::set_error(FXB_EINVAL, "fxb_tree_attn: scale must be positive and finite");
+  const Plan plan = plan_of(a->dtype, a->D);
+  if (!a->workspace || !fxb::aligned16(a->workspace) || a->workspace_bytes < (int64_t)workspace_bytes(plan, a->D))
+    return fxb::set_error(FXB_EINVAL, "fxb_tree_attn: workspace of fxb_tree_attn_workspace bytes, 16-byte aligned");
+  if (plan.grid > kMaxGrid) return fxb::set_error(FXB_EUNSUPPORTED, "fxb_tree_attn: device with too many SMs");
   int* err = fxb::dev_error_ptr();
   if (!err) return FXB_ECUDA;
+  Params p = {};
+  p.B = a->B;
+  p.T = a->T;
+  p.Hq = a->Hq;
+  p.Hkv = a->Hkv;
+  p.G = a->Hq / a->Hkv;
+  p.R = p.T * p.G;
+  p.page_shift = shift;
+  p.P = a->P;
+  p.W = a->W;
+  p.scale_log2 = a->scale * 1.4426950408889634f;
+  p.q = a->q;
+  p.o = a->o;
+  p.kp = a->k_pages;
+  p.vp = a->v_pages;
+  p.q_sb = a->q_sb; p.q_st = a->q_st; p.q_sh = a->q_sh;
+  p.o_sb = a->o_sb; p.o_st = a->o_st; p.o_sh = a->o_sh;
+  p.kp_sp = a->kp_sp; p.kp_sh = a->kp_sh; p.kp_st = a->kp_st;
+  p.vp_sp = a->vp_sp; p.vp_sh = a->vp_sh; p.vp_st = a->vp_st;
+  p.table = a->table;
+  p.table_sb = a->table_sb;
+  p.lens = a->lens;
+  p.n_nodes = a->n_nodes;
+  p.mask = a->mask;
+  p.mask_sb = a->mask_sb;
+  p.arrived = static_cast<unsigned*>(a->workspace);
+  p.parts = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + kMaxGrid * sizeof(unsigned));
+  p.err = err;
   if (a->dtype == FXB_DTYPE_F32)
-    return a->D == 64 ? launch<float, 64>(a, shift, err, stream) : launch<float, 128>(a, shift, err, stream);
+    return a->D == 64 ? launch<float, 64>(a, plan, p, stream) : launch<float, 128>(a, plan, p, stream);
   if (a->dtype == FXB_DTYPE_F16)
-    return a->D == 64 ? launch<__half, 64>(a, shift, err, stream) : launch<__half, 128>(a, shift, err, stream);
-  return a->D == 64 ? launch<__nv_bfloat16, 64>(a, shift, err, stream)
-                    : launch<__nv_bfloat16, 128>(a, shift, err, stream);
+    return a->D == 64 ? launch<__half, 64>(a, plan, p, stream) : launch<__half, 128>(a, plan, p, stream);
+  return a->D == 64 ? launch<__nv_bfloat16, 64>(a, plan, p, stream)
+                    : launch<__nv_bfloat16, 128>(a, plan, p, stream);
 }
 
 }  // extern "C"

@@ -37,6 +37,7 @@ def set_gemm_timing(records):
 # starts; GEMMs reset them themselves, except after an expired wait (device
 # error word bit 1), when `_reset_workspaces` zeroes them.
 _GEMM_WS = {}
+_STREAM_WS = {}      # the same for stream_workspace
 _CAPTURE_WS = None  # dict of the graph being captured, or None
 
 
@@ -49,6 +50,21 @@ def _gemm_workspace(device):
         n = int(_lib.load().fxb_gemm_workspace_size())
         ws = torch.empty(n, device=device, dtype=torch.uint8)
         ws[:4096].zero_()  # the arrival counters (inside a capture: a memset node of the graph)
+        table[key] = ws
+    return ws
+
+
+def stream_workspace(kind, device, nbytes, zeroed):
+    """Workspace of at least `nbytes` bytes for calls of one kind on the current
+    stream, kept like the GEMM's: one per (device, stream) for eager launches,
+    one of its own for a captured graph. Its first `zeroed` bytes are zero
+    before the first use; the kernels leave them so."""
+    table = _CAPTURE_WS if _CAPTURE_WS is not None else _STREAM_WS
+    key = (kind, device.index, torch.cuda.current_stream(device).cuda_stream)
+    ws = table.get(key)
+    if ws is None or ws.numel() < nbytes:
+        ws = torch.empty(nbytes, device=device, dtype=torch.uint8)
+        ws[:zeroed].zero_()
         table[key] = ws
     return ws
 

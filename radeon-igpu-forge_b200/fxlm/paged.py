@@ -23,7 +23,7 @@ import math
 
 import torch
 
-from fxb200 import _lib
+from fxb200 import _lib, ops
 
 _DTYPES = (torch.float16, torch.bfloat16, torch.float32)
 MAX_NODES = 64
@@ -112,14 +112,19 @@ def tree_attention(q, k, v, k_pages, v_pages, page_table, ctx_lens, n_nodes, tre
         raise ValueError("the last axis of every tensor must be contiguous")
     if B == 0 or T == 0:
         return out
+    lib = _lib.load()
+    code = _lib.DTYPE_CODE[dt]
+    shape = (code, B, T, Hq, Hkv, D)
+    nbytes = lib.fxb_tree_attn_workspace(*shape)
+    ws = ops.stream_workspace("tree_attn", q.device, nbytes, lib.fxb_tree_attn_workspace_zeroed(*shape))
     a = _lib.TreeAttnArgs(
-        _lib.DTYPE_CODE[dt], B, T, Hq, Hkv, D, page, P, W, scale,
+        code, B, T, Hq, Hkv, D, page, P, W, scale,
         q.data_ptr(), sq[0], sq[1], sq[2], k.data_ptr(), sk[0], sk[1], sk[2],
         v.data_ptr(), sv[0], sv[1], sv[2], out.data_ptr(), so[0], so[1], so[2],
         k_pages.data_ptr(), skp[0], skp[1], skp[2], v_pages.data_ptr(), svp[0], svp[1], svp[2],
         page_table.data_ptr(), max(page_table.stride(0), W), lens, n,
-        tree_mask.data_ptr(), max(tree_mask.stride(0), T), None, 0)
-    _lib.check(_lib.load().fxb_tree_attn(ctypes.byref(a), _lib.stream_ptr(q.device)), "fxb_tree_attn")
+        tree_mask.data_ptr(), max(tree_mask.stride(0), T), ws.data_ptr(), nbytes)
+    _lib.check(lib.fxb_tree_attn(ctypes.byref(a), _lib.stream_ptr(q.device)), "fxb_tree_attn")
     return out
 
 
