@@ -1,189 +1,23 @@
-// Attention of a tree of drafted tokens over a paged KV cache (fxb_tree_attn).
-// No reference counterpart: its sampler keeps no cache (ml/fxlm/sample.py:63-73).
-//
-// o = softmax(scale * q k^T) v over the context slots and the visible nodes,
-// computed in one pass over the keys: a running maximum m, sum l and output O
-// per row, rescaled by 2^(m_old - m_new) when the maximum rises. States of
-// different parts of the keys join the same way, so a sequence can be divided
-// at will.
-//
-// Work. An item is (batch row, key head, row tile): the R = T * G query rows
-// of a key head (G query heads share it; row r is node r / G, head r % G),
-// cut into tiles of rows. An item's keys are its context in blocks of 64 slots
-// and one block of nodes. All items' blocks in a row are divided evenly over
-// the thread blocks, so uneven lengths cost nothing; an item that several
-// thread blocks share is joined by the one that finishes last, from states in
-// the workspace, in the order of the keys (the result does not depend on who
-// that is).
-#include "common.cuh"
-#include "internal.h"
+// Attention of a tree of drafted tokens over a paged KV cache (fxb_tree_attn):
+// the kernel for few rows and the entry point. No reference counterpart: its
+// sampler keeps no cache (ml/fxlm/sample.py:63-73).
+#include "tree_attn.cuh"
 
 namespace {
 
-constexpr int kMaxTree = 64;
+using namespace fxb_tree;
+
 constexpr int kBlockKeys = 64;          // keys of a block
 constexpr int kWarps = 4;               // each takes 16 keys of a block
 constexpr int kThreads = kWarps * 32;
 constexpr int kRows = 16;               // rows of a tile
 constexpr int kTile = 16;               // keys a warp takes at once
-constexpr float kRescaleLog2 = 8.f;     // see softmax_rows
-constexpr int kMaxGrid = 1024;          // arrival counters in the workspace
 
-FXB_DEV float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-struct Params {
-  int B, T, Hq, Hkv, G, R, RT, page_shift, P, W;
-  float scale_log2;
-  const void* q;
-  void *o, *kp, *vp;
-  int64_t q_sb, q_st, q_sh, o_sb, o_st, o_sh;
-  int64_t kp_sp, kp_sh, kp_st, vp_sp, vp_sh, vp_st;
-  const int32_t* table;
-  int64_t table_sb;
-  const int32_t *lens, *n_nodes;
-  const int64_t* mask;
-  int64_t mask_sb;
-  unsigned* arrived;  // workspace: kMaxGrid counters,
-  float* parts;       // then two states for every thread block
-  int* err;
-};
-
-// ------------------------------------------------------------------ division of the work
-struct Row {  // a batch row
-  int len, n, blocks;
-};
-FXB_DEV Row row_of(const Params& a, int b) {
-  const int len_in = a.lens[b], n_in = a.n_nodes[b];
-  const int64_t most = (int64_t)a.W << a.page_shift;
-  Row r;
-  r.len = len_in < 0 ? 0 : (len_in > most ? (int)most : len_in);
-  r.n = min(max(n_in, 0), a.T);
-  if (r.len != len_in || r.n != n_in) atomicOr(a.err, FXB_DERR_PAGES);
-  if (r.n == 0) r.len = 0;  // nothing to compute: the block of nodes writes zeros
-  r.blocks = (r.len + kBlockKeys - 1) / kBlockKeys + 1;
-  return r;
-}
-
-// inclusive prefix sum over the block's threads; *total for everyone
-FXB_DEV int64_t block_scan(int64_t v, int64_t* total) {
-  __shared__ int64_t warp_total[kWarps];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t y = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += y;
-  }
-  __syncthreads();
-  if (lane == 31) warp_total[warp] = v;
-  __syncthreads();
-  int64_t all = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) v += warp_total[w];
-    all += warp_total[w];
-  }
-  *total = all;
-  return v;
-}
-
-// position in the sequence of all blocks: block j of item (b, hr), hr = key head * RT + row tile
-struct Cursor {
-  int64_t u;
-  int b, hr, j;
-  Row row;
-};
-FXB_DEV void next(const Params& a, Cursor& c, int64_t end) {
-  ++c.u;
-  if (++c.j < c.row.blocks) return;
-  c.j = 0;
-  if (++c.hr < a.Hkv * a.RT) return;
-  c.hr = 0;
-  ++c.b;
-  if (c.u < end) c.row = row_of(a, c.b);
-}
-
-// This thread block's share [c.u, *end) of all *total blocks, c set to its
-// first one. No share is empty, but for thread blocks beyond the number of blocks.
-FXB_DEV int64_t sharers(int64_t total) { return total < (int64_t)gridDim.x ? total : (int64_t)gridDim.x; }
-FXB_DEV int64_t share_begin(int64_t cta, int64_t total) {
-  const int64_t g = sharers(total);
-  return cta < g ? total * cta / g : total;
-}
-FXB_DEV Cursor share(const Params& a, int64_t* end, int64_t* total) {
-  __shared__ int s_b;
-  __shared__ int64_t s_rest;
-  const int per = a.Hkv * a.RT, tid = threadIdx.x;
-  int64_t n = 0, mine = 0, incl = 0;
-  for (int b0 = 0; b0 < a.B; b0 += kThreads) {
-    const int b = b0 + tid;
-    mine = b < a.B ? (int64_t)row_of(a, b).blocks * per : 0;
-    int64_t all;
-    incl = block_scan(mine, &all) + n;
-    n += all;
-  }
-  Cursor c;
-  c.u = share_begin(blockIdx.x, n);
-  *end = share_begin(blockIdx.x + 1, n);
-  *total = n;
-  if (c.u >= *end) return c;
-  if (a.B > kThreads) n = 0;
-  for (int b0 = 0; b0 < a.B; b0 += kThreads) {
-    const int b = b0 + tid;
-    if (a.B > kThreads) {
-      mine = b < a.B ? (int64_t)row_of(a, b).blocks * per : 0;
-      int64_t all;
-      incl = block_scan(mine, &all) + n;
-      n += all;
-    }
-    if (c.u < incl && c.u >= incl - mine) {
-      s_b = b;
-      s_rest = c.u - (incl - mine);
-    }
-    if (a.B > kThreads && n > c.u) break;
-  }
-  __syncthreads();
-  c.b = s_b;
-  c.row = row_of(a, c.b);
-  c.hr = (int)(s_rest / c.row.blocks);
-  c.j = (int)(s_rest - (int64_t)c.hr * c.row.blocks);
-  return c;
-}
-// the thread block that owns block u
-FXB_DEV int owner(int64_t u, int64_t total) { return (int)(((u + 1) * sharers(total) - 1) / total); }
-
-// ------------------------------------------------------------------ joining states
 // State of an item's part in the workspace: m and l of each row, then O.
-// A thread block has two places: 1 for an item that it begins, 0 for one that
-// it continues. The counter of an item is that of the block that begins it.
 template <int ROWS, int D>
 FXB_DEV float* part_of(const Params& a, int cta, int place) {
   return a.parts + ((int64_t)cta * 2 + place) * ROWS * (D + 2);
 }
-
-template <typename T, int D>
-FXB_DEV void write_out(const Params& a, int b, int hk, int r, int d, float4 o, float l) {
-  if (r >= a.R) return;
-  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // no visible key: zeros; NaN stays
-  const int t = r / a.G, h = hk * a.G + (r - t * a.G);
-  T* p = static_cast<T*>(a.o) + b * a.o_sb + t * a.o_st + h * a.o_sh + d;
-  if constexpr (sizeof(T) == 4) {
-    *reinterpret_cast<float4*>(p) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-  } else {
-    *reinterpret_cast<uint2*>(p) = make_uint2(pack2<T>(o.x * inv, o.y * inv), pack2<T>(o.z * inv, o.w * inv));
-  }
-}
-FXB_DEV void axpy4(float4& o, float w, const float4& x) {
-  o.x = fmaf(w, x.x, o.x);
-  o.y = fmaf(w, x.y, o.y);
-  o.z = fmaf(w, x.z, o.z);
-  o.w = fmaf(w, x.w, o.w);
-}
-// weight of a state with maximum m in a join with maximum mx
-FXB_DEV float weight(float m, float mx) { return m == -INFINITY ? 0.f : ex2(m - mx); }
 
 // Called by all threads after this thread block's part is written: the last
 // one to arrive joins the parts and writes the item's rows.
@@ -589,7 +423,7 @@ tree_attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
   pdl_wait();
 
   int64_t end, total;
-  Cursor c = share(a, &end, &total);
+  Cursor c = share<kBlockKeys, kThreads>(a, &end, &total);
   if (c.u >= end) return;
   const int64_t start = c.u;
   Cursor f = c;          // the next block to fetch
@@ -626,7 +460,7 @@ tree_attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       }
     }
     ++fetched;
-    next(a, f, end);
+    next<kBlockKeys>(a, f, end);
     pg = page_of();
   };
   for (int i = 0; i < ST; ++i) fetch();
@@ -674,7 +508,7 @@ tree_attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       }
     }
     const Cursor cur = c;
-    next(a, c, end);
+    next<kBlockKeys>(a, c, end);
     if (tree || c.u >= end) {
       // the four warps' states join; each lies in the stage that its warp has just used up
       __syncwarp();
@@ -727,43 +561,35 @@ template <typename T> constexpr CUtensorMapDataType map_type() {
          : std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                           : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
 }
-// (outer, heads, rows, D) view with element strides; boxes of `rows` rows of 128 bytes.
-// The stride of an axis of one entry is not used and may be anything.
-template <typename T>
-int encode(CUtensorMap* m, const void* base, int D, int rows, int64_t st, int heads, int64_t sh, int outer,
-           int64_t so, int box_rows) {
-  const uint64_t e = sizeof(T), one = D * e;
-  const uint64_t dims[4] = {(uint64_t)D, (uint64_t)rows, (uint64_t)heads, (uint64_t)outer};
-  const uint64_t strides[3] = {rows > 1 ? st * e : one, heads > 1 ? sh * e : one, outer > 1 ? so * e : one};
-  const uint32_t box[4] = {(uint32_t)(128 / e), (uint32_t)box_rows, 1, 1};
-  return fxb::encode_tiled(m, map_type<T>(), 4, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+// Few or many rows of a key head. The first kernel reads the cache once for
+// every 16 rows and leaves 16 x 16 products to a warp; the second takes up to
+// 128 rows with one reading, in tiles of 128 whatever the number of rows.
+bool many_rows(int dtype, int T, int G) { return dtype != FXB_DTYPE_F32 && T * G > kRows && G <= 128; }
+
+template <typename T, int D> constexpr int rows_ctas() { return Shape<T, D>::kCtas; }
+int rows_grid(int dtype, int D) {
+  const int ctas = dtype == FXB_DTYPE_F32 ? (D == 64 ? rows_ctas<float, 64>() : rows_ctas<float, 128>())
+                                          : (D == 64 ? rows_ctas<__half, 64>() : rows_ctas<__half, 128>());
+  return ctas * fxb::num_sms();
 }
 
-struct Plan {
-  int grid, rows;  // thread blocks, rows of a tile
-};
-template <typename T, int D> Plan plan_rows() { return {Shape<T, D>::kCtas * fxb::num_sms(), kRows}; }
-
-Plan plan_of(int dtype, int D) {
-  if (dtype == FXB_DTYPE_F32) return D == 64 ? plan_rows<float, 64>() : plan_rows<float, 128>();
-  return D == 64 ? plan_rows<__half, 64>() : plan_rows<__half, 128>();
-}
-
-size_t workspace_bytes(const Plan& p, int D) {
-  return kMaxGrid * sizeof(unsigned) + (size_t)p.grid * 2 * p.rows * (D + 2) * sizeof(float);
+size_t workspace_bytes(int dtype, int T, int G, int D) {
+  const size_t floats = many_rows(dtype, T, G) ? fxb::num_sms() * 2 * wide_part_floats(D)
+                                               : (size_t)rows_grid(dtype, D) * 2 * kRows * (D + 2);
+  return kMaxGrid * sizeof(unsigned) + floats * sizeof(float);
 }
 
 template <typename T, int D>
-int launch(const fxb_tree_attn_args* x, const Plan& plan, Params& a, void* stream) {
+int launch(const fxb_tree_attn_args* x, Params& a, void* stream) {
   CUtensorMap k, v, nk, nv;
-  if (int r = encode<T>(&k, x->k_pages, D, x->page, x->kp_st, x->Hkv, x->kp_sh, x->P, x->kp_sp, kTile)) return r;
-  if (int r = encode<T>(&v, x->v_pages, D, x->page, x->vp_st, x->Hkv, x->vp_sh, x->P, x->vp_sp, kTile)) return r;
-  if (int r = encode<T>(&nk, x->k, D, x->T, x->k_st, x->Hkv, x->k_sh, x->B, x->k_sb, kTile)) return r;
-  if (int r = encode<T>(&nv, x->v, D, x->T, x->v_st, x->Hkv, x->v_sh, x->B, x->v_sb, kTile)) return r;
-  a.RT = (a.R + plan.rows - 1) / plan.rows;
-  // no more thread blocks than there can be blocks of keys
-  const int64_t most = (int64_t)a.B * a.Hkv * a.RT * ((((int64_t)a.W << a.page_shift) + kBlockKeys - 1) / kBlockKeys + 1);
-  const int grid = (int)(most < plan.grid ? most : plan.grid);
+  const auto t = map_type<T>();
+  const int e = sizeof(T);
+  if (int r = encode_rows(&k, t, e, x->k_pages, D, x->page, x->kp_st, x->Hkv, x->kp_sh, x->P, x->kp_sp, kTile, 1)) return r;
+  if (int r = encode_rows(&v, t, e, x->v_pages, D, x->page, x->vp_st, x->Hkv, x->vp_sh, x->P, x->vp_sp, kTile, 1)) return r;
+  if (int r = encode_rows(&nk, t, e, x->k, D, x->T, x->k_st, x->Hkv, x->k_sh, x->B, x->k_sb, kTile, 1)) return r;
+  if (int r = encode_rows(&nv, t, e, x->v, D, x->T, x->v_st, x->Hkv, x->v_sh, x->B, x->v_sb, kTile, 1)) return r;
+  a.RT = (a.R + kRows - 1) / kRows;
+  const int grid = grid_of(x, a, kBlockKeys, rows_grid(x->dtype, D));
   using S = Shape<T, D>;
   if (int r = fxb::check_cuda(
           cudaFuncSetAttribute(tree_attn_rows<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem),
@@ -779,7 +605,7 @@ extern "C" {
 
 size_t fxb_tree_attn_workspace(int32_t dtype, int32_t B, int32_t T, int32_t Hq, int32_t Hkv, int32_t D) {
   if ((D != 64 && D != 128) || !fxb::dtype_size(dtype) || B < 1 || T < 1 || Hkv < 1 || Hq < Hkv) return 0;
-  return workspace_bytes(plan_of(dtype, D), D);
+  return workspace_bytes(dtype, T, Hq / Hkv, D);
 }
 size_t fxb_tree_attn_workspace_zeroed(int32_t dtype, int32_t B, int32_t T, int32_t Hq, int32_t Hkv, int32_t D) {
   return fxb_tree_attn_workspace(dtype, B, T, Hq, Hkv, D) ? kMaxGrid * sizeof(unsigned) : 0;
@@ -813,10 +639,12 @@ int fxb_tree_attn(const fxb_tree_attn_args* a, void* stream) {
       return fxb::set_error(FXB_EINVAL, "fxb_tree_attn: strides must be multiples of 16 bytes");
   if (!(a->scale > 0.f) || !(a->scale < INFINITY))
     return fxb::set_error(FXB_EINVAL, "fxb_tree_attn: scale must be positive and finite");
-  const Plan plan = plan_of(a->dtype, a->D);
-  if (!a->workspace || !fxb::aligned16(a->workspace) || a->workspace_bytes < (int64_t)workspace_bytes(plan, a->D))
+  const int G = a->Hq / a->Hkv;
+  if (!a->workspace || !fxb::aligned16(a->workspace) ||
+      a->workspace_bytes < (int64_t)workspace_bytes(a->dtype, a->T, G, a->D))
     return fxb::set_error(FXB_EINVAL, "fxb_tree_attn: workspace of fxb_tree_attn_workspace bytes, 16-byte aligned");
-  if (plan.grid > kMaxGrid) return fxb::set_error(FXB_EUNSUPPORTED, "fxb_tree_attn: device with too many SMs");
+  if (rows_grid(a->dtype, a->D) > kMaxGrid)
+    return fxb::set_error(FXB_EUNSUPPORTED, "fxb_tree_attn: device with too many SMs");
   int* err = fxb::dev_error_ptr();
   if (!err) return FXB_ECUDA;
   Params p = {};
@@ -824,7 +652,7 @@ int fxb_tree_attn(const fxb_tree_attn_args* a, void* stream) {
   p.T = a->T;
   p.Hq = a->Hq;
   p.Hkv = a->Hkv;
-  p.G = a->Hq / a->Hkv;
+  p.G = G;
   p.R = p.T * p.G;
   p.page_shift = shift;
   p.P = a->P;
@@ -847,12 +675,13 @@ int fxb_tree_attn(const fxb_tree_attn_args* a, void* stream) {
   p.arrived = static_cast<unsigned*>(a->workspace);
   p.parts = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + kMaxGrid * sizeof(unsigned));
   p.err = err;
+  if (many_rows(a->dtype, a->T, G)) return launch_wide(a, p, stream);
   if (a->dtype == FXB_DTYPE_F32)
-    return a->D == 64 ? launch<float, 64>(a, plan, p, stream) : launch<float, 128>(a, plan, p, stream);
+    return a->D == 64 ? launch<float, 64>(a, p, stream) : launch<float, 128>(a, p, stream);
   if (a->dtype == FXB_DTYPE_F16)
-    return a->D == 64 ? launch<__half, 64>(a, plan, p, stream) : launch<__half, 128>(a, plan, p, stream);
-  return a->D == 64 ? launch<__nv_bfloat16, 64>(a, plan, p, stream)
-                    : launch<__nv_bfloat16, 128>(a, plan, p, stream);
+    return a->D == 64 ? launch<__half, 64>(a, p, stream) : launch<__half, 128>(a, p, stream);
+  return a->D == 64 ? launch<__nv_bfloat16, 64>(a, p, stream)
+                    : launch<__nv_bfloat16, 128>(a, p, stream);
 }
 
 }  // extern "C"

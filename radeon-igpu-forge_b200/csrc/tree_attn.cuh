@@ -1,0 +1,202 @@
+// What the two kernels of fxb_tree_attn share: their parameters, the division
+// of the work over thread blocks and the joining of states.
+//
+// o = softmax(scale * q k^T) v over the context slots and the visible nodes,
+// computed in one pass over the keys: a running maximum m, sum l and output O
+// per row, rescaled by 2^(m_old - m_new) when the maximum rises. States of
+// different parts of the keys join the same way, so a sequence can be divided
+// at will.
+//
+// Work. An item is (batch row, key head, row tile): the R = T * G query rows
+// of a key head (G query heads share it; row r is node r / G, head r % G),
+// cut into tiles of rows. An item's keys are its context in blocks of
+// BLOCK_KEYS slots and one block of nodes. All items' blocks in a row are
+// divided evenly over the thread blocks, so uneven lengths cost nothing; an
+// item that several thread blocks share is joined by the one that finishes
+// last, from states in the workspace, in the order of the keys (the result
+// does not depend on who that is).
+#pragma once
+#include "common.cuh"
+#include "internal.h"
+
+namespace fxb_tree {
+
+constexpr int kMaxTree = 64;
+constexpr int kMaxGrid = 1024;        // arrival counters in the workspace
+constexpr float kRescaleLog2 = 8.f;   // how far a row's reference maximum may lag behind, in powers of two
+
+FXB_DEV float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+struct Params {
+  int B, T, Hq, Hkv, G, R, RT, NT, page_shift, P, W;  // RT row tiles of an item's rows; NT: nodes of one (many rows)
+  float scale_log2;
+  const void* q;
+  void *o, *kp, *vp;
+  int64_t q_sb, q_st, q_sh, o_sb, o_st, o_sh;
+  int64_t kp_sp, kp_sh, kp_st, vp_sp, vp_sh, vp_st;
+  const int32_t* table;
+  int64_t table_sb;
+  const int32_t *lens, *n_nodes;
+  const int64_t* mask;
+  int64_t mask_sb;
+  unsigned* arrived;  // workspace: kMaxGrid counters,
+  float* parts;       // then two states for every thread block
+  int* err;
+};
+
+// ------------------------------------------------------------------ division of the work
+struct Row {  // a batch row
+  int len, n, blocks;
+};
+template <int BLOCK_KEYS> FXB_DEV Row row_of(const Params& a, int b) {
+  const int len_in = a.lens[b], n_in = a.n_nodes[b];
+  const int64_t most = (int64_t)a.W << a.page_shift;
+  Row r;
+  r.len = len_in < 0 ? 0 : (len_in > most ? (int)most : len_in);
+  r.n = min(max(n_in, 0), a.T);
+  if (r.len != len_in || r.n != n_in) atomicOr(a.err, FXB_DERR_PAGES);
+  if (r.n == 0) r.len = 0;  // nothing to compute: the block of nodes writes zeros
+  r.blocks = (r.len + BLOCK_KEYS - 1) / BLOCK_KEYS + 1;
+  return r;
+}
+
+// inclusive prefix sum over the block's threads; *total for everyone
+template <int THREADS> FXB_DEV int64_t block_scan(int64_t v, int64_t* total) {
+  constexpr int kWarps = THREADS / 32;
+  __shared__ int64_t warp_total[kWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += y;
+  }
+  __syncthreads();
+  if (lane == 31) warp_total[warp] = v;
+  __syncthreads();
+  int64_t all = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) v += warp_total[w];
+    all += warp_total[w];
+  }
+  *total = all;
+  return v;
+}
+
+// position in the sequence of all blocks: block j of item (b, hr), hr = key head * RT + row tile
+struct Cursor {
+  int64_t u;
+  int b, hr, j;
+  Row row;
+};
+template <int BLOCK_KEYS> FXB_DEV void next(const Params& a, Cursor& c, int64_t end) {
+  ++c.u;
+  if (++c.j < c.row.blocks) return;
+  c.j = 0;
+  if (++c.hr < a.Hkv * a.RT) return;
+  c.hr = 0;
+  ++c.b;
+  if (c.u < end) c.row = row_of<BLOCK_KEYS>(a, c.b);
+}
+
+// This thread block's share [c.u, *end) of all *total blocks, c set to its
+// first one. No share is empty, but for thread blocks beyond the number of blocks.
+FXB_DEV int64_t sharers(int64_t total) { return total < (int64_t)gridDim.x ? total : (int64_t)gridDim.x; }
+FXB_DEV int64_t share_begin(int64_t cta, int64_t total) {
+  const int64_t g = sharers(total);
+  return cta < g ? total * cta / g : total;
+}
+template <int BLOCK_KEYS, int THREADS> FXB_DEV Cursor share(const Params& a, int64_t* end, int64_t* total) {
+  __shared__ int s_b;
+  __shared__ int64_t s_rest;
+  const int per = a.Hkv * a.RT, tid = threadIdx.x;
+  int64_t n = 0, mine = 0, incl = 0;
+  for (int b0 = 0; b0 < a.B; b0 += THREADS) {
+    const int b = b0 + tid;
+    mine = b < a.B ? (int64_t)row_of<BLOCK_KEYS>(a, b).blocks * per : 0;
+    int64_t all;
+    incl = block_scan<THREADS>(mine, &all) + n;
+    n += all;
+  }
+  Cursor c;
+  c.u = share_begin(blockIdx.x, n);
+  *end = share_begin(blockIdx.x + 1, n);
+  *total = n;
+  if (c.u >= *end) return c;
+  if (a.B > THREADS) n = 0;
+  for (int b0 = 0; b0 < a.B; b0 += THREADS) {
+    const int b = b0 + tid;
+    if (a.B > THREADS) {
+      mine = b < a.B ? (int64_t)row_of<BLOCK_KEYS>(a, b).blocks * per : 0;
+      int64_t all;
+      incl = block_scan<THREADS>(mine, &all) + n;
+      n += all;
+    }
+    if (c.u < incl && c.u >= incl - mine) {
+      s_b = b;
+      s_rest = c.u - (incl - mine);
+    }
+    if (a.B > THREADS && n > c.u) break;
+  }
+  __syncthreads();
+  c.b = s_b;
+  c.row = row_of<BLOCK_KEYS>(a, c.b);
+  c.hr = (int)(s_rest / c.row.blocks);
+  c.j = (int)(s_rest - (int64_t)c.hr * c.row.blocks);
+  return c;
+}
+// the thread block that owns block u
+FXB_DEV int owner(int64_t u, int64_t total) { return (int)(((u + 1) * sharers(total) - 1) / total); }
+
+// ------------------------------------------------------------------ joining states
+// Parts. A thread block has two places in the workspace: 1 for an item that it
+// begins, 0 for one that it continues. The arrival counter of an item is that
+// of the block that begins it.
+template <typename T, int D>
+FXB_DEV void write_out(const Params& a, int b, int hk, int r, int d, float4 o, float l) {
+  if (r >= a.R) return;
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // no visible key: zeros; NaN stays
+  const int t = r / a.G, h = hk * a.G + (r - t * a.G);
+  T* p = static_cast<T*>(a.o) + b * a.o_sb + t * a.o_st + h * a.o_sh + d;
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(p) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+  } else {
+    *reinterpret_cast<uint2*>(p) = make_uint2(pack2<T>(o.x * inv, o.y * inv), pack2<T>(o.z * inv, o.w * inv));
+  }
+}
+FXB_DEV void axpy4(float4& o, float w, const float4& x) {
+  o.x = fmaf(w, x.x, o.x);
+  o.y = fmaf(w, x.y, o.y);
+  o.z = fmaf(w, x.z, o.z);
+  o.w = fmaf(w, x.w, o.w);
+}
+// weight of a state with maximum m in a join with maximum mx
+FXB_DEV float weight(float m, float mx) { return m == -INFINITY ? 0.f : ex2(m - mx); }
+
+// ------------------------------------------------------------------ host
+// (outer, mid, rows, D) view with element strides, 128-byte swizzle; boxes of
+// box_rows x box_mid rows of 128 bytes. The stride of an axis of one entry is
+// not used and may be anything.
+inline int encode_rows(CUtensorMap* m, CUtensorMapDataType type, int size, const void* base, int D, int rows,
+                       int64_t s_rows, int mid, int64_t s_mid, int outer, int64_t s_outer, int box_rows, int box_mid) {
+  const uint64_t e = size, one = D * e;
+  const uint64_t dims[4] = {(uint64_t)D, (uint64_t)rows, (uint64_t)mid, (uint64_t)outer};
+  const uint64_t strides[3] = {rows > 1 ? s_rows * e : one, mid > 1 ? s_mid * e : one, outer > 1 ? s_outer * e : one};
+  const uint32_t box[4] = {(uint32_t)(128 / e), (uint32_t)box_rows, (uint32_t)box_mid, 1};
+  return fxb::encode_tiled(m, type, 4, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+// thread blocks: `most`, but no more than there can be blocks of keys
+inline int grid_of(const fxb_tree_attn_args* x, const Params& a, int block_keys, int most) {
+  const int64_t keys = (int64_t)a.W << a.page_shift;
+  const int64_t n = (int64_t)a.B * a.Hkv * a.RT * ((keys + block_keys - 1) / block_keys + 1);
+  return (int)(n < most ? n : most);
+}
+// the kernel for many rows (tree_attn_wide.cu): 16-bit types, G <= 128
+size_t wide_part_floats(int D);
+int launch_wide(const fxb_tree_attn_args* x, Params& a, void* stream);
+
+}  // namespace fxb_tree

@@ -1,0 +1,581 @@
+// Attention of a tree of drafted tokens over a paged KV cache: the kernel for
+// many rows (16-bit types), on tcgen05 tensor cores.
+//
+// A row tile is up to 128 rows (whole nodes: 128 / G of them) against tiles of
+// 128 keys; the block of nodes is one tile of 64. Persistent thread blocks, one
+// an SM, walk their share of all tiles. Roles (352 threads):
+//   warps 0-3, 4-7  two softmax groups; a thread owns one row. Tiles go to the
+//                   groups in turn, and each group keeps a state (m, l, O) of
+//                   its own, so that nothing is exchanged between them until
+//                   the item ends;
+//   warp 8          issues the products: S = Q K^T of a tile while the other
+//                   group's tile is in its softmax, O += P V;
+//   warp 9          copies Q, keys and values by TMA, a lane a page;
+//   warp 10         writes the nodes' keys and values into the cache.
+// Tensor memory (512 columns): group g's scores at 128 g (fp32; the 16-bit
+// probabilities overwrite their first half: the A operand of P V), its O at
+// 256 + 128 g.
+// Keys and values go through one ring of operands in the order of their use
+// (K0 K1 V0 K2 V1 ...), Q through two buffers.
+#include "tree_attn.cuh"
+
+namespace {
+
+using namespace fxb_tree;
+
+constexpr int kTileRows = 128;
+constexpr int kBlockKeys = 128;
+constexpr int kThreads = 352;
+constexpr int kWarpMma = 8, kWarpTma = 9, kWarpStore = 10;
+constexpr int kSoftmax = 256;  // threads of both groups
+
+template <int D> struct Wide {
+  static constexpr int kBoxes = D / 64;
+  static constexpr int kOperand = kTileRows * D * 2;  // Q, K or V of a tile: D / 64 blocks of [128 rows][128 bytes]
+  static constexpr int kSlots = D == 128 ? 4 : 10;    // ring of keys and values
+  static constexpr int kSmem = 1024 + (2 + kSlots) * kOperand;
+  static constexpr int kPart = kTileRows * (D + 2);   // floats of a state in the workspace
+};
+static_assert(Wide<128>::kSmem + 5120 <= 232448 && Wide<64>::kSmem + 5120 <= 232448, "shared memory");
+
+// byte offset of 16-byte piece c of row r of an operand (128-byte swizzle)
+FXB_DEV uint32_t sw(int r, int c) { return (c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4); }
+// steps of 16 along K of an operand whose rows are M or N (K-major) or K (MN-major)
+constexpr uint32_t kmajor_off(int kk) { return (kk >> 2) * 16384 + (kk & 3) * 32; }
+constexpr uint32_t mnmajor_off(int kk) { return kk * 2048; }
+
+struct Exchange {  // per item parity
+  float m[2][kTileRows], l[2][kTileRows];  // of each group's state
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+               const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmNK,
+               const __grid_constant__ CUtensorMap tmNV, const void* new_v, int64_t v_sb, int64_t v_st, int64_t v_sh,
+               const void* new_k, int64_t k_sb, int64_t k_st, int64_t k_sh, const Params a) {
+  using W = Wide<D>;
+  constexpr int NS = W::kSlots, NBOX = W::kBoxes;
+  constexpr int FMT = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t bars[2 * NS + 12];
+  __shared__ Exchange xch[2];
+  __shared__ int odd_value[3];  // an item's node has a value that is not finite (items in turn)
+  __shared__ uint32_t tmem_slot;
+  __shared__ int s_last;
+  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+  uint8_t* gbase = smem_raw + (base - raw);
+  const uint32_t sQ = base, sKV = base + 2 * W::kOperand;
+  const uint32_t bar0 = smem_u32(bars);
+  auto full = [&](int s) { return bar0 + 8u * s; };
+  auto empty = [&](int s) { return bar0 + 8u * (NS + s); };
+  auto q_full = [&](int i) { return bar0 + 8u * (2 * NS + i); };
+  auto q_empty = [&](int i) { return bar0 + 8u * (2 * NS + 2 + i); };
+  auto s_full = [&](int g) { return bar0 + 8u * (2 * NS + 4 + g); };
+  auto p_full = [&](int g) { return bar0 + 8u * (2 * NS + 6 + g); };
+  auto pv_done = [&](int g) { return bar0 + 8u * (2 * NS + 8 + g); };
+  const uint32_t o_free = bar0 + 8u * (2 * NS + 10), final_bar = bar0 + 8u * (2 * NS + 11);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(q_full(i), 1);
+      mbar_init(q_empty(i), 1);
+      mbar_init(s_full(i), 1);
+      mbar_init(p_full(i), 128);
+      mbar_init(pv_done(i), 1);
+    }
+    odd_value[0] = odd_value[1] = odd_value[2] = 0;
+    mbar_init(o_free, kSoftmax);
+    mbar_init(final_bar, 1);
+    fence_mbar_init();
+  }
+  if (warp == kWarpMma) {
+    tmem_alloc(smem_u32(&tmem_slot), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  pdl_trigger();
+  pdl_wait();
+
+  int64_t end, total;
+  Cursor c = share<kBlockKeys, kThreads>(a, &end, &total);
+  const int64_t start = c.u;
+  const int n_tiles = (int)(end > start ? end - start : 0);
+  // places in the ring's order of use
+  auto k_index = [&](int q) { return q == 0 ? 0 : 2 * q - 1; };
+  auto v_index = [&](int q) { return q + 1 < n_tiles ? 2 * q + 2 : 2 * q + 1; };
+  bool ok = true;
+
+  if (warp == kWarpTma) {
+    // ------------------------------------------------ copies; lane i takes page i of a tile
+    if (lane == 0) {
+      tma_prefetch_desc(&tmQ);
+      tma_prefetch_desc(&tmK);
+      tma_prefetch_desc(&tmV);
+      tma_prefetch_desc(&tmNK);
+      tma_prefetch_desc(&tmNV);
+    }
+    const int page = 1 << a.page_shift, box_rows = min(page, kBlockKeys), per_tile = kBlockKeys / box_rows;
+    int items = -1, issued = 0;
+    // this lane's page of the tile at f: -1 none; ids outside the pool read page 0 (and are reported)
+    auto page_of = [&](const Cursor& f) {
+      if (f.u >= end || f.j == f.row.blocks - 1) return -1;
+      const int slot0 = f.j * kBlockKeys + lane * box_rows;
+      if (lane >= per_tile || slot0 >= f.row.len) return -1;
+      int pg = a.table[f.b * a.table_sb + (slot0 >> a.page_shift)];
+      if (pg < 0 || pg >= a.P) {
+        atomicOr(a.err, FXB_DERR_PAGES);
+        pg = 0;
+      }
+      return pg;
+    };
+    auto load = [&](const Cursor& f, int pg, const CUtensorMap* ctx, const CUtensorMap* nodes) -> bool {
+      const int s = issued % NS;
+      if (!mbar_wait_warp(empty(s), ((issued / NS) & 1) ^ 1, a.err, FXB_DERR_ATTN_WAIT)) return false;
+      const bool tree = f.j == f.row.blocks - 1;
+      const int hk = f.hr / a.RT;
+      const int pages = tree ? 1 : (min(f.row.len - f.j * kBlockKeys, kBlockKeys) + box_rows - 1) / box_rows;
+      if (lane == 0) mbar_expect_tx(full(s), pages * (tree ? kMaxTree : box_rows) * 128 * NBOX);
+      __syncwarp();
+      if (lane < pages) {
+        const uint32_t dst = sKV + s * W::kOperand + (tree ? 0 : lane * box_rows * 128);
+        const int row = tree ? 0 : (f.j * kBlockKeys) & (page - 1);  // 0 unless a page holds several tiles
+#pragma unroll
+        for (int x = 0; x < NBOX; ++x)
+          tma_load_4d(dst + x * 16384, tree ? nodes : ctx, full(s), x * 64, row, hk, tree ? f.b : pg);
+      }
+      ++issued;
+      return true;
+    };
+    auto load_k = [&](const Cursor& f, int pg, bool begins) -> bool {
+      if (begins) {  // the item's rows of Q
+        ++items;
+        const int qb = items & 1;
+        if (!mbar_wait_warp(q_empty(qb), ((items >> 1) & 1) ^ 1, a.err, FXB_DERR_ATTN_WAIT)) return false;
+        if (lane == 0) {
+          mbar_expect_tx(q_full(qb), a.NT * a.G * 128 * NBOX);
+#pragma unroll
+          for (int x = 0; x < NBOX; ++x)
+            tma_load_4d(sQ + qb * W::kOperand + x * 16384, &tmQ, q_full(qb), x * 64, (f.hr / a.RT) * a.G,
+                        (f.hr % a.RT) * a.NT, f.b);
+        }
+      }
+      return load(f, pg, &tmK, &tmNK);
+    };
+    if (n_tiles) {
+      Cursor f = c;  // keys run one tile ahead of values, page ids one more
+      int pg = page_of(f);
+      Cursor nf = f;
+      next<kBlockKeys>(a, nf, end);
+      int npg = page_of(nf);
+      ok = load_k(f, pg, true);
+      for (int q = 0; q < n_tiles && ok; ++q) {
+        const Cursor fv = f;
+        const int pv = pg;
+        f = nf;
+        pg = npg;
+        if (q + 1 < n_tiles) {
+          next<kBlockKeys>(a, nf, end);
+          npg = page_of(nf);
+          ok = load_k(f, pg, f.j == 0);
+        }
+        if (ok) ok = load(fv, pv, &tmV, &tmNV);
+      }
+      // what is under way lands before shared memory goes
+      for (int i = max(0, issued - NS); i < issued; ++i)
+        mbar_wait_warp(full(i % NS), (i / NS) & 1, a.err, FXB_DERR_ATTN_WAIT);
+      for (int i = max(0, items - 1); i <= items; ++i)
+        mbar_wait_warp(q_full(i & 1), (i >> 1) & 1, a.err, FXB_DERR_ATTN_WAIT);
+    }
+  } else if (warp == kWarpMma) {
+    // ------------------------------------------------ products (lane 0)
+    if (lane == 0 && n_tiles) {
+      constexpr uint32_t IS = umma_idesc_f16(FMT, 0, 0, kTileRows, kBlockKeys);
+      constexpr uint32_t IST = umma_idesc_f16(FMT, 0, 0, kTileRows, kMaxTree);
+      constexpr uint32_t IPV = umma_idesc_f16(FMT, 0, 1, kTileRows, D);
+      int items_s = -1, items_p = -1;  // items begun by S products, by P V products
+      bool first[2] = {true, true};    // the group's next P V begins its O
+      Cursor cs = c, cp = c;
+      auto issue_s = [&](int q) -> bool {
+        const int i = k_index(q), s = i % NS, g = q & 1;
+        const bool tree = cs.j == cs.row.blocks - 1;
+        if (q == 0 || cs.j == 0) {
+          ++items_s;
+          if (!mbar_wait(q_full(items_s & 1), (items_s >> 1) & 1, a.err, FXB_DERR_ATTN_WAIT)) return false;
+        }
+        if (!mbar_wait(full(s), (i / NS) & 1, a.err, FXB_DERR_ATTN_WAIT)) return false;
+        // these columns still hold the probabilities of tile q - 2 until its P V is complete
+        if (q >= 2 && !mbar_wait(pv_done(g), ((q - 2) >> 1) & 1, a.err, FXB_DERR_ATTN_WAIT)) return false;
+        tc_fence_after();
+        const uint64_t qd = umma_desc_sw128(sQ + (items_s & 1) * W::kOperand, 16, 1024);
+        const uint64_t kd = umma_desc_sw128(sKV + s * W::kOperand, 16, 1024);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)
+          umma_f16(tmem + g * 128, desc_add(qd, kmajor_off(kk)), desc_add(kd, kmajor_off(kk)), tree ? IST : IS,
+                   kk > 0);
+        umma_commit(s_full(g));
+        umma_commit(empty(s));
+        if (tree || q + 1 == n_tiles) umma_commit(q_empty(items_s & 1));  // the item's last S has read Q
+        next<kBlockKeys>(a, cs, end);
+        return true;
+      };
+      auto issue_pv = [&](int q) -> bool {
+        const int i = v_index(q), s = i % NS, g = q & 1;
+        const bool tree = cp.j == cp.row.blocks - 1;
+        if (q == 0 || cp.j == 0) {
+          ++items_p;
+          first[0] = first[1] = true;
+        }
+        if (!mbar_wait(p_full(g), (q >> 1) & 1, a.err, FXB_DERR_ATTN_WAIT)) return false;
+        if (!mbar_wait(full(s), (i / NS) & 1, a.err, FXB_DERR_ATTN_WAIT)) return false;
+        // O of the previous item has been read
+        if (first[g] && items_p > 0 && !mbar_wait(o_free, (items_p - 1) & 1, a.err, FXB_DERR_ATTN_WAIT)) return false;
+        tc_fence_after();
+        const uint64_t vd = umma_desc_sw128(sKV + s * W::kOperand, 16384, 1024);
+        const int steps = tree ? kMaxTree / 16 : kBlockKeys / 16;
+#pragma unroll
+        for (int kk = 0; kk < kBlockKeys / 16; ++kk)
+          if (kk < steps)
+            umma_f16_ta(tmem + 256 + g * 128, tmem + g * 128 + kk * 8, desc_add(vd, mnmajor_off(kk)), IPV,
+                        (!first[g] || kk > 0) ? 1u : 0u);
+        umma_commit(pv_done(g));
+        umma_commit(empty(s));
+        first[g] = false;
+        next<kBlockKeys>(a, cp, end);
+        return true;
+      };
+      ok = issue_s(0);
+      for (int q = 0; q < n_tiles && ok; ++q) {
+        if (q + 1 < n_tiles) ok = issue_s(q + 1);
+        if (ok) ok = issue_pv(q);
+      }
+      umma_commit(final_bar);
+      mbar_wait(final_bar, 0, a.err, FXB_DERR_ATTN_WAIT);
+    }
+    __syncwarp();
+  } else if (warp == kWarpStore) {
+    // ------------------------------------------------ the nodes' keys and values into the cache
+    constexpr int CH = D / 8;
+    for (Cursor f = c; f.u < end; next<kBlockKeys>(a, f, end)) {
+      if (f.j != f.row.blocks - 1 || f.hr % a.RT) continue;
+      const int hk = f.hr / a.RT, n = f.row.n * CH;
+#pragma unroll 1
+      for (int i0 = lane; i0 < n; i0 += 32 * 4) {
+        uint4 xk[4], xv[4];
+        int64_t to[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int i = i0 + 32 * u, t = i / CH, ch = i % CH;
+          to[u] = -1;
+          if (i < n) {
+            const int64_t pos = (int64_t)f.row.len + t, pi = pos >> a.page_shift;
+            const int pg = pi < a.W ? a.table[f.b * a.table_sb + pi] : -1;
+            if (pg < 0 || pg >= a.P) atomicOr(a.err, FXB_DERR_PAGES);
+            else to[u] = ((int64_t)pg << a.page_shift) | (pos & ((1 << a.page_shift) - 1));
+            xk[u] = *reinterpret_cast<const uint4*>(static_cast<const T*>(new_k) + f.b * k_sb + t * k_st + hk * k_sh +
+                                                    ch * 8);
+            xv[u] = *reinterpret_cast<const uint4*>(static_cast<const T*>(new_v) + f.b * v_sb + t * v_st + hk * v_sh +
+                                                    ch * 8);
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          if (to[u] < 0) continue;
+          const int ch = (i0 + 32 * u) % CH;
+          const int64_t pg = to[u] >> a.page_shift, off = to[u] & ((1 << a.page_shift) - 1);
+          *reinterpret_cast<uint4*>(static_cast<T*>(a.kp) + pg * a.kp_sp + hk * a.kp_sh + off * a.kp_st + ch * 8) = xk[u];
+          *reinterpret_cast<uint4*>(static_cast<T*>(a.vp) + pg * a.vp_sp + hk * a.vp_sh + off * a.vp_st + ch * 8) = xv[u];
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------ softmax
+    const int g = warp >> 2, r = (warp & 3) * 32 + lane;  // group, row of the tile
+    const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t tS = tmem + lane_off + g * 128, tO = tmem + lane_off + 256;
+    int done = 0;   // tiles of this group so far
+    int item = 0;
+    auto uwait = [&](uint32_t bar, uint32_t parity) -> bool {
+      return __all_sync(0xffffffffu, mbar_wait(bar, parity, a.err, FXB_DERR_ATTN_WAIT));
+    };
+    float m = -INFINITY, l = 0.f;
+    int mine = 0;   // tiles of this group in the item
+    bool live = false, dead = true;  // this row is a node's; no row of this warp is
+    uint64_t see = 0;
+    int64_t u_first = 0;
+    for (int q = 0; q < n_tiles; ++q) {
+      const int hk = c.hr / a.RT, t0 = (c.hr % a.RT) * a.NT;
+      const bool tree = c.j == c.row.blocks - 1;
+      if (q == 0 || c.j == 0) {
+        u_first = c.u - c.j;
+        m = -INFINITY;
+        l = 0.f;
+        mine = 0;
+        const int t = t0 + r / a.G;
+        live = r < a.NT * a.G && t < c.row.n;
+        see = live ? (uint64_t)a.mask[c.b * a.mask_sb + t] : 0;
+        dead = !__any_sync(0xffffffffu, live);
+      }
+      Exchange& x = xch[item & 1];
+      if ((q & 1) == g) {
+        if (ok && !uwait(s_full(g), done & 1)) ok = false;
+        if (ok) {
+          tc_fence_after();
+          const int valid = tree ? c.row.n : min(c.row.len - c.j * kBlockKeys, kBlockKeys);
+          const int vi = v_index(q), vslot = vi % NS;
+          const int cols = tree ? kMaxTree : kBlockKeys;
+          // values that no row may count are zeroed (0 * NaN is NaN): behind the sequence, or nodes that
+          // do not exist; infinities and NaN of nodes too: who sees them adds them at the item's end
+          if (valid < cols || tree) {
+            if (!uwait(full(vslot), (vi / NS) & 1)) ok = false;
+            uint8_t* vs = gbase + (sKV - base) + vslot * W::kOperand;
+            bool odd = false;
+            for (int i = r; i < cols * (D / 8); i += 128) {
+              const int row = i / (D / 8);
+              uint4* p = reinterpret_cast<uint4*>(vs + sw(row, i % (D / 8)));
+              if (row >= valid) {
+                *p = make_uint4(0, 0, 0, 0);
+              } else if (tree) {
+                float f[8];
+                unpack8<T>(*p, f);
+                bool any = false;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                  const bool fin = fabsf(f[e]) < INFINITY;
+                  any |= !fin;
+                  f[e] = fin ? f[e] : 0.f;
+                }
+                if (any) *p = pack8<T>(f);
+                odd |= any;
+              }
+            }
+            if (odd) atomicExch(&odd_value[item % 3], 1);
+            fence_proxy_async_smem();
+          }
+          if (!dead) {
+          uint32_t v[128];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) tmem_ld32(tS + i * 32, v + 32 * i);
+          if (!tree) {
+#pragma unroll
+            for (int i = 2; i < 4; ++i) tmem_ld32(tS + i * 32, v + 32 * i);
+          }
+          tmem_wait_ld();
+          if (tree) {
+#pragma unroll
+            for (int i = 0; i < 64; ++i)
+              if (!((see >> i) & 1) || i >= valid) v[i] = __float_as_uint(-INFINITY);
+#pragma unroll
+            for (int i = 64; i < 128; ++i) v[i] = __float_as_uint(-INFINITY);
+          } else if (valid < kBlockKeys) {
+#pragma unroll
+            for (int i = 0; i < 128; ++i)
+              if (i >= valid) v[i] = __float_as_uint(-INFINITY);
+          }
+          float mv[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) mv[i] = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < 128; ++i) mv[i & 7] = fmaxf(mv[i & 7], __uint_as_float(v[i]));
+          const float mx = fmaxf(fmaxf(fmaxf(mv[0], mv[1]), fmaxf(mv[2], mv[3])),
+                                 fmaxf(fmaxf(mv[4], mv[5]), fmaxf(mv[6], mv[7]))) * a.scale_log2;
+          // the reference maximum m moves only when a tile exceeds it by more than 2^8: probabilities stay
+          // below 2^8, which 16 bits hold as well as [0, 1], and O is rarely rescaled
+          if (mine == 0) {
+            m = mx;  // the group's first P V of the item overwrites O
+          } else if (__any_sync(0xffffffffu, mx > m + kRescaleLog2)) {
+            if (!uwait(pv_done(g), (done - 1) & 1)) ok = false;
+            tc_fence_after();
+            const bool up = mx > m + kRescaleLog2;
+            const float f = up ? ex2(m - mx) : 1.f;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+              uint32_t o[16];
+              tmem_ld16(tO + g * 128 + i * 16, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tmem_st16(tO + g * 128 + i * 16, o);
+            }
+            tmem_wait_st();
+            l *= f;
+            if (up) m = mx;
+          }
+          const float z = m == -INFINITY ? 0.f : m;
+          float sum[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) sum[i] = 0.f;
+          // probabilities enter the second product in the inputs' type, as its operands must
+#pragma unroll
+          for (int i0 = 0; i0 < 128; i0 += 32) {
+            if (i0 >= 64 && tree) continue;
+            uint32_t p[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float p0 = ex2(fmaf(__uint_as_float(v[i0 + 2 * i]), a.scale_log2, -z));
+              const float p1 = ex2(fmaf(__uint_as_float(v[i0 + 2 * i + 1]), a.scale_log2, -z));
+              sum[(2 * i) & 7] += p0;
+              sum[(2 * i + 1) & 7] += p1;
+              p[i] = pack2<T>(p0, p1);
+            }
+            tmem_st16(tS + i0 / 2, p);
+          }
+          tmem_wait_st();
+          l += ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7]));
+          }
+          tc_fence_before();
+          mbar_arrive(p_full(g));
+        }
+        ++done;
+        ++mine;
+      }
+      const Cursor cur = c;
+      next<kBlockKeys>(a, c, end);
+      if (!tree && q + 1 < n_tiles) continue;
+      // ---- the item ends here: both groups' states join
+      if (ok && mine && !uwait(pv_done(g), (done - 1) & 1)) ok = false;
+      x.m[g][r] = live ? m : -INFINITY;
+      x.l[g][r] = live ? l : 0.f;
+      const int n_item = (int)(cur.u - max(u_first, start)) + 1;  // this thread block's tiles of the item
+      // the next item's flag, last read two items ago (every thread has passed the barrier since); the
+      // exchange of this item is written again two items on, likewise
+      if (threadIdx.x == 0) odd_value[(item + 1) % 3] = 0;
+      tc_fence_before();
+      named_bar_sync(1, kSoftmax);
+      const bool begun = u_first >= start, whole = begun && tree;
+      const float m0 = x.m[0][r], m1 = x.m[1][r];
+      const float mj = fmaxf(m0, m1), w0 = weight(m0, mj), w1 = weight(m1, mj);
+      const float lj = fmaf(x.l[0][r], w0, x.l[1][r] * w1);
+      // a group without a tile of this item has no O
+      const bool has0 = n_item > 1 || (q & 1) == 0, has1 = n_item > 1 || (q & 1) == 1;
+      const int rows = min(a.NT, a.T - t0) * a.G;
+      float* part = a.parts + ((int64_t)blockIdx.x * 2 + begun) * W::kPart;
+      const int d0 = g * (D / 2);
+      tc_fence_after();
+#pragma unroll
+      for (int i = 0; i < D / 2 / 16; ++i) {
+        uint32_t o0[16], o1[16];
+        tmem_ld16(tO + d0 + i * 16, o0);
+        tmem_ld16(tO + 128 + d0 + i * 16, o1);
+        tmem_wait_ld();
+        if (r < rows && ok) {
+          float o[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float y0 = has0 ? __uint_as_float(o0[e]) * w0 : 0.f, y1 = has1 ? __uint_as_float(o1[e]) * w1 : 0.f;
+            o[e] = live ? y0 + y1 : 0.f;
+          }
+          if (tree && odd_value[item % 3])
+            for (int j = 0; j < cur.row.n; ++j)
+              if ((see >> j) & 1)
+                for (int e = 0; e < 16; ++e) {
+                  const float y = to_f<T>(static_cast<const T*>(new_v)[cur.b * v_sb + j * v_st + hk * v_sh + d0 + i * 16 + e]);
+                  if (!(fabsf(y) < INFINITY)) o[e] += y;
+                }
+#pragma unroll
+          for (int e = 0; e < 16; e += 4) {
+            const float4 o4 = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            const int d = d0 + i * 16 + e;
+            if (whole) write_out<T, D>(a, cur.b, hk, t0 * a.G + r, d, o4, lj);
+            else reinterpret_cast<float4*>(part + 2 * kTileRows)[(d / 4) * kTileRows + r] = o4;
+          }
+        }
+      }
+      tc_fence_before();
+      mbar_arrive(o_free);
+      if (!whole) {
+        if (g == 0 && r < rows) {
+          part[r] = mj;
+          part[kTileRows + r] = lj;
+        }
+        const int64_t u_last = u_first + cur.row.blocks - 1;
+        const int lo = owner(u_first, total), hi = owner(u_last, total);
+        __threadfence();
+        named_bar_sync(1, kSoftmax);
+        if (threadIdx.x == 0) {
+          const unsigned before = atomicAdd(&a.arrived[lo], 1u);
+          s_last = before == (unsigned)(hi - lo);
+          if (s_last) a.arrived[lo] = 0;  // for the next call
+        }
+        named_bar_sync(1, kSoftmax);
+        if (s_last) {  // the parts in the order of the keys
+          __threadfence();
+          for (int i = threadIdx.x; i < rows * (D / 4); i += kSoftmax) {
+            const int rr = i % rows, d4 = i / rows;
+            float pm = -INFINITY, pl = 0.f;
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+            for (int k = lo; k <= hi; ++k) {
+              const float* p = a.parts + ((int64_t)k * 2 + (k == lo)) * W::kPart;
+              const float mk = __ldcg(p + rr), lk = __ldcg(p + kTileRows + rr);
+              const float4 ok4 = __ldcg(reinterpret_cast<const float4*>(p + 2 * kTileRows) + d4 * kTileRows + rr);
+              const float mn = fmaxf(pm, mk);
+              const float f0 = weight(pm, mn), f1 = weight(mk, mn);
+              o = make_float4(o.x * f0, o.y * f0, o.z * f0, o.w * f0);
+              axpy4(o, f1, ok4);
+              pl = fmaf(pl, f0, lk * f1);
+              pm = mn;
+            }
+            write_out<T, D>(a, cur.b, hk, t0 * a.G + rr, d4 * 4, o, pl);
+          }
+        }
+      }
+      ++item;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kWarpMma) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <typename T> constexpr CUtensorMapDataType map_type() {
+  return std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+}
+
+template <typename T, int D>
+int launch(const fxb_tree_attn_args* x, Params& a, int grid, void* stream) {
+  CUtensorMap q, k, v, nk, nv;
+  const auto t = map_type<T>();
+  if (int r = encode_rows(&q, t, 2, x->q, D, x->Hq, x->q_sh, x->T, x->q_st, x->B, x->q_sb, a.G, a.NT)) return r;
+  const int box = x->page < kBlockKeys ? x->page : kBlockKeys;
+  if (int r = encode_rows(&k, t, 2, x->k_pages, D, x->page, x->kp_st, x->Hkv, x->kp_sh, x->P, x->kp_sp, box, 1)) return r;
+  if (int r = encode_rows(&v, t, 2, x->v_pages, D, x->page, x->vp_st, x->Hkv, x->vp_sh, x->P, x->vp_sp, box, 1)) return r;
+  if (int r = encode_rows(&nk, t, 2, x->k, D, x->T, x->k_st, x->Hkv, x->k_sh, x->B, x->k_sb, kMaxTree, 1)) return r;
+  if (int r = encode_rows(&nv, t, 2, x->v, D, x->T, x->v_st, x->Hkv, x->v_sh, x->B, x->v_sb, kMaxTree, 1)) return r;
+  if (int r = fxb::check_cuda(
+          cudaFuncSetAttribute(tree_attn_wide<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Wide<D>::kSmem),
+          "fxb_tree_attn"))
+    return r;
+  fxb::pdl_launch(tree_attn_wide<T, D>, dim3(grid), dim3(kThreads), Wide<D>::kSmem, fxb::as_stream(stream), q, k, v,
+                  nk, nv, x->v, x->v_sb, x->v_st, x->v_sh, x->k, x->k_sb, x->k_st, x->k_sh, a);
+  return fxb::check_launch("fxb_tree_attn");
+}
+
+}  // namespace
+
+namespace fxb_tree {
+
+size_t wide_part_floats(int D) { return D == 64 ? Wide<64>::kPart : Wide<128>::kPart; }
+
+int launch_wide(const fxb_tree_attn_args* x, Params& a, void* stream) {
+  a.NT = a.T < kTileRows / a.G ? a.T : kTileRows / a.G;
+  a.RT = (a.T + a.NT - 1) / a.NT;
+  const int grid = grid_of(x, a, kBlockKeys, fxb::num_sms());
+  if (x->dtype == FXB_DTYPE_F16)
+    return x->D == 64 ? launch<__half, 64>(x, a, grid, stream) : launch<__half, 128>(x, a, grid, stream);
+  return x->D == 64 ? launch<__nv_bfloat16, 64>(x, a, grid, stream) : launch<__nv_bfloat16, 128>(x, a, grid, stream);
+}
+
+}  // namespace fxb_tree

@@ -128,12 +128,12 @@ SIGNATURES = {
     "fxb_attn_bwd": (ctypes.c_int, [ctypes.POINTER(AttnArgs), _vp]),
     "fxb_tree_attn_workspace": (ctypes.c_size_t, [_i32] * 6),
     "fxb_tree_attn_workspace_zeroed": (ctypes.c_size_t, [_i32] * 6),
-    "fxb_tree_attn": (ctypes.c_int, [ctypes.POINTER(TreeAttnArgs), _vp]),
+    "fxb_tree_attn": (ctypes.c_int, [_vp, _vp]),
     "fxb_verify_tree": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp,
                                        _vp, _vp, _i32, _i32, _i32, _vp]),
-    "fxb_kv_commit": (ctypes.c_int, [ctypes.POINTER(KvArgs), _vp, _i64, _i32, _vp, _vp, _vp, _vp]),
+    "fxb_kv_commit": (ctypes.c_int, [_vp, _vp, _i64, _i32, _vp, _vp, _vp, _vp]),
     "fxb_kv_fork_workspace": (ctypes.c_size_t, [_i32, _i32]),
-    "fxb_kv_fork": (ctypes.c_int, [ctypes.POINTER(KvArgs), _vp, _vp, _vp]),
+    "fxb_kv_fork": (ctypes.c_int, [_vp, _vp, _vp, _vp]),
     "fxb_embedding_fwd": (ctypes.c_int, [_i32, _vp, _vp, _vp, _vp, _i64, _i64, _i32, _i64, _vp]),
     "fxb_embedding_bwd": (ctypes.c_int, [_i32, _vp, _vp, _vp, _vp, _i64, _i64, _i32, _i64, _vp]),
     "fxb_axpy": (ctypes.c_int, [_i32, _vp, _i32, _vp, _vp, _i32, _i64, _vp]),
@@ -181,6 +181,12 @@ def call(name, *args):
 
 def stream_ptr(device=None):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def raw_stream(device_index):
+    """Handle of torch's current stream of a device as an integer, without the
+    Stream object that stream_ptr makes (2.4 us a call)."""
+    return torch._C._cuda_getCurrentRawStream(device_index)
 
 
 def ptr(t):

@@ -54,16 +54,16 @@ def _gemm_workspace(device):
     return ws
 
 
-def stream_workspace(kind, device, nbytes, zeroed):
-    """Workspace of at least `nbytes` bytes for calls of one kind on the current
-    stream, kept like the GEMM's: one per (device, stream) for eager launches,
-    one of its own for a captured graph. Its first `zeroed` bytes are zero
-    before the first use; the kernels leave them so."""
+def stream_workspace(kind, device_index, stream, nbytes, zeroed):
+    """Workspace of at least `nbytes` bytes for calls of one kind on a stream
+    (its handle), kept like the GEMM's: one per (device, stream) for eager
+    launches, one of its own for a captured graph. Its first `zeroed` bytes are
+    zero before the first use; the kernels leave them so."""
     table = _CAPTURE_WS if _CAPTURE_WS is not None else _STREAM_WS
-    key = (kind, device.index, torch.cuda.current_stream(device).cuda_stream)
+    key = (kind, device_index, stream)
     ws = table.get(key)
     if ws is None or ws.numel() < nbytes:
-        ws = torch.empty(nbytes, device=device, dtype=torch.uint8)
+        ws = torch.empty(nbytes, device=torch.device("cuda", device_index), dtype=torch.uint8)
         ws[:zeroed].zero_()
         table[key] = ws
     return ws

@@ -57,9 +57,10 @@ def __getattr__(name):
         from . import model as _m
         return getattr(_m, name)
     if name in ("tree_attention", "tree_masks", "kv_commit", "kv_reserve", "kv_fork"):
+        # called once a layer and token: found in the module itself from the second time on
         from . import paged as _m
-        return getattr(_m, name)
+        return globals().setdefault(name, getattr(_m, name))
     if name == "verify_tree":
-        from .speculate import verify_tree
-        return verify_tree
+        from . import speculate as _m
+        return globals().setdefault(name, _m.verify_tree)
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

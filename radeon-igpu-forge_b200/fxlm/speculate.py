@@ -5,12 +5,20 @@ from fxb200 import _lib
 from .paged import MAX_NODES, _i32
 
 
-def _probs(t, name, shape):
+def _refuse_probs(t, name, shape):
     if t.dtype != torch.float32 or not t.is_cuda:
         raise TypeError(f"{name} must be a cuda fp32 tensor, got {t.dtype} on {t.device}")
-    if tuple(t.shape) != shape or (shape[-1] > 1 and t.stride(-1) != 1):
-        raise ValueError(f"{name} must be {shape} with unit stride on the vocabulary, got {tuple(t.shape)}")
-    return t.data_ptr(), t.stride(0), t.stride(1)
+    raise ValueError(f"{name} must be {shape} with unit stride on the vocabulary, got {tuple(t.shape)}")
+
+
+def _probs(t, name, shape):
+    """(address, row stride, node stride)."""
+    if not (t.dtype == torch.float32 and t.is_cuda and t.shape == shape):
+        _refuse_probs(t, name, shape)
+    sb, st, s1 = t.stride()
+    if s1 != 1 and shape[2] > 1:
+        _refuse_probs(t, name, shape)
+    return t.data_ptr(), sb, st
 
 
 def verify_tree(tokens, parents, n_nodes, target_probs, u, draft_probs=None):
@@ -41,20 +49,18 @@ def verify_tree(tokens, parents, n_nodes, target_probs, u, draft_probs=None):
     if not tokens.is_contiguous():
         raise ValueError("tokens must be contiguous")
     V = target_probs.shape[-1]
-    pp, p_sb, p_st = _probs(target_probs, "target_probs", (B, T, V))
-    qp, q_sb, q_st = (None, 0, 0) if draft_probs is None else _probs(draft_probs, "draft_probs", (B, T, V))
+    p, p_sb, p_st = _probs(target_probs, "target_probs", (B, T, V))
+    q, q_sb, q_st = (None, 0, 0) if draft_probs is None else _probs(draft_probs, "draft_probs", (B, T, V))
     par, nn = _i32(parents, "parents", (B, T)), _i32(n_nodes, "n_nodes", (B,))
     if u.dtype != torch.float32 or not u.is_cuda:
         raise TypeError("u must be a cuda fp32 tensor")
-    if tuple(u.shape) != (B, T) or not u.is_contiguous():
+    if u.shape != (B, T) or not u.is_contiguous():
         raise ValueError(f"u must be contiguous ({B},{T}), got {tuple(u.shape)}")
-    dev = tokens.device
-    path = torch.empty((B, T), device=dev, dtype=torch.int32)
-    n_path = torch.empty((B,), device=dev, dtype=torch.int32)
-    nxt = torch.empty((B,), device=dev, dtype=torch.int64)
-    if B == 0:
-        return path, n_path, nxt
-    _lib.check(_lib.load().fxb_verify_tree(
-        tokens.data_ptr(), par, nn, pp, p_sb, p_st, qp, q_sb, q_st, u.data_ptr(), path.data_ptr(),
-        n_path.data_ptr(), nxt.data_ptr(), B, T, V, _lib.stream_ptr(dev)), "fxb_verify_tree")
+    path, n_path, nxt = torch.empty_like(parents), torch.empty_like(n_nodes), tokens.new_empty(B)
+    if B:
+        rc = _lib.load().fxb_verify_tree(
+            tokens.data_ptr(), par, nn, p, p_sb, p_st, q, q_sb, q_st, u.data_ptr(), path.data_ptr(),
+            n_path.data_ptr(), nxt.data_ptr(), B, T, V, _lib.raw_stream(tokens.get_device()))
+        if rc:
+            _lib.check(rc, "fxb_verify_tree")
     return path, n_path, nxt

@@ -39,6 +39,11 @@ def test_struct_layouts_match(lib):
     from fxb200 import _lib
     assert lib.fxb_abi_struct_size(2) == ctypes.sizeof(_lib.TreeAttnArgs)
     assert lib.fxb_abi_struct_size(3) == ctypes.sizeof(_lib.KvArgs)
+    from fxlm import paged
+    for packed, mirror in ((paged._TREE_ARGS, _lib.TreeAttnArgs), (paged._KV_ARGS, _lib.KvArgs)):
+        assert packed.size == ctypes.sizeof(mirror)
+        m = mirror.from_buffer_copy(packed.pack(*range(1, len(mirror._fields_) + 1)))
+        assert [getattr(m, f[0]) for f in mirror._fields_] == list(range(1, len(mirror._fields_) + 1))
 
 
 @pytest.mark.parametrize("change,word", [
