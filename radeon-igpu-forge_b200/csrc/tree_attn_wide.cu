@@ -44,6 +44,18 @@ FXB_DEV uint32_t sw(int r, int c) { return (c >> 3) * 16384 + r * 128 + (((c & 7
 constexpr uint32_t kmajor_off(int kk) { return (kk >> 2) * 16384 + (kk & 3) * 32; }
 constexpr uint32_t mnmajor_off(int kk) { return kk * 2048; }
 
+// completes loads from tensor memory; the registers pass through it, so that nothing that uses them moves before it
+FXB_DEV void tmem_wait_ld32(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                 "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                 "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+
 struct Exchange {  // per item parity
   float m[2][kTileRows], l[2][kTileRows];  // of each group's state
 };
@@ -155,39 +167,36 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
       ++issued;
       return true;
     };
-    auto load_k = [&](const Cursor& f, int pg, bool begins) -> bool {
-      if (begins) {  // the item's rows of Q
-        ++items;
-        const int qb = items & 1;
-        if (!mbar_wait_warp(q_empty(qb), ((items >> 1) & 1) ^ 1, a.err, FXB_DERR_ATTN_WAIT)) return false;
-        if (lane == 0) {
-          mbar_expect_tx(q_full(qb), a.NT * a.G * 128 * NBOX);
-#pragma unroll
-          for (int x = 0; x < NBOX; ++x)
-            tma_load_4d(sQ + qb * W::kOperand + x * 16384, &tmQ, q_full(qb), x * 64, (f.hr / a.RT) * a.G,
-                        (f.hr % a.RT) * a.NT, f.b);
-        }
-      }
-      return load(f, pg, &tmK, &tmNK);
-    };
+    // step q: keys of tile q, then values of tile q - 1
     if (n_tiles) {
-      Cursor f = c;  // keys run one tile ahead of values, page ids one more
-      int pg = page_of(f);
-      Cursor nf = f;
-      next<kBlockKeys>(a, nf, end);
-      int npg = page_of(nf);
-      ok = load_k(f, pg, true);
-      for (int q = 0; q < n_tiles && ok; ++q) {
-        const Cursor fv = f;
-        const int pv = pg;
-        f = nf;
-        pg = npg;
-        if (q + 1 < n_tiles) {
-          next<kBlockKeys>(a, nf, end);
-          npg = page_of(nf);
-          ok = load_k(f, pg, f.j == 0);
+      Cursor f = c, fv = c;
+      int pg = page_of(f), pv = -1;
+#pragma unroll 1
+      for (int q = 0; q <= n_tiles && ok; ++q) {
+        if (q < n_tiles && (q == 0 || f.j == 0)) {  // the item's rows of Q
+          ++items;
+          const int qb = items & 1;
+          ok = mbar_wait_warp(q_empty(qb), ((items >> 1) & 1) ^ 1, a.err, FXB_DERR_ATTN_WAIT);
+          if (!ok) break;
+          if (lane == 0) {
+            mbar_expect_tx(q_full(qb), a.NT * a.G * 128 * NBOX);
+#pragma unroll
+            for (int x = 0; x < NBOX; ++x)
+              tma_load_4d(sQ + qb * W::kOperand + x * 16384, &tmQ, q_full(qb), x * 64, (f.hr / a.RT) * a.G,
+                          (f.hr % a.RT) * a.NT, f.b);
+          }
         }
-        if (ok) ok = load(fv, pv, &tmV, &tmNV);
+        const Cursor fk = f;
+        const int pk = pg;
+        if (q < n_tiles) {
+          next<kBlockKeys>(a, f, end);
+          pg = page_of(f);  // used in the next step
+        }
+#pragma unroll 1
+        for (int kv = q < n_tiles ? 0 : 1; kv < (q ? 2 : 1) && ok; ++kv)
+          ok = load(kv ? fv : fk, kv ? pv : pk, kv ? &tmV : &tmK, kv ? &tmNV : &tmNK);
+        fv = fk;
+        pv = pk;
       }
       // what is under way lands before shared memory goes
       for (int i = max(0, issued - NS); i < issued; ++i)
@@ -196,69 +205,77 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
         mbar_wait_warp(q_full(i & 1), (i >> 1) & 1, a.err, FXB_DERR_ATTN_WAIT);
     }
   } else if (warp == kWarpMma) {
-    // ------------------------------------------------ products (lane 0)
-    if (lane == 0 && n_tiles) {
+    // ------------------------------------------------ products: the warp stays together, one lane issues
+    if (n_tiles) {
       constexpr uint32_t IS = umma_idesc_f16(FMT, 0, 0, kTileRows, kBlockKeys);
       constexpr uint32_t IST = umma_idesc_f16(FMT, 0, 0, kTileRows, kMaxTree);
       constexpr uint32_t IPV = umma_idesc_f16(FMT, 0, 1, kTileRows, D);
       int items_s = -1, items_p = -1;  // items begun by S products, by P V products
-      bool first[2] = {true, true};    // the group's next P V begins its O
+      unsigned first = 3;              // bit g: the group's next P V begins its O
       Cursor cs = c, cp = c;
-      auto issue_s = [&](int q) -> bool {
-        const int i = k_index(q), s = i % NS, g = q & 1;
-        const bool tree = cs.j == cs.row.blocks - 1;
-        if (q == 0 || cs.j == 0) {
-          ++items_s;
-          if (!mbar_wait(q_full(items_s & 1), (items_s >> 1) & 1, a.err, FXB_DERR_ATTN_WAIT)) return false;
-        }
-        if (!mbar_wait(full(s), (i / NS) & 1, a.err, FXB_DERR_ATTN_WAIT)) return false;
-        // these columns still hold the probabilities of tile q - 2 until its P V is complete
-        if (q >= 2 && !mbar_wait(pv_done(g), ((q - 2) >> 1) & 1, a.err, FXB_DERR_ATTN_WAIT)) return false;
-        tc_fence_after();
-        const uint64_t qd = umma_desc_sw128(sQ + (items_s & 1) * W::kOperand, 16, 1024);
-        const uint64_t kd = umma_desc_sw128(sKV + s * W::kOperand, 16, 1024);
+      // step q: S of tile q, then P V of tile q - 1. Issued by an elected lane of the whole
+      // warp: the operands of a product are then known to be uniform
+#pragma unroll 1
+      for (int q = 0; q <= n_tiles; ++q) {
+        if (q < n_tiles) {
+          const int i = k_index(q), st = i % NS, g = q & 1;
+          const bool tree = cs.j == cs.row.blocks - 1;
+          if (q == 0 || cs.j == 0) {
+            ++items_s;
+            if (!mbar_wait_warp(q_full(items_s & 1), (items_s >> 1) & 1, a.err, FXB_DERR_ATTN_WAIT)) break;
+          }
+          if (!mbar_wait_warp(full(st), (i / NS) & 1, a.err, FXB_DERR_ATTN_WAIT)) break;
+          // these columns still hold the probabilities of tile q - 2 until its P V is complete
+          if (q >= 2 && !mbar_wait_warp(pv_done(g), ((q - 2) >> 1) & 1, a.err, FXB_DERR_ATTN_WAIT)) break;
+          tc_fence_after();
+          const uint64_t qd = umma_desc_sw128(sQ + (items_s & 1) * W::kOperand, 16, 1024);
+          const uint64_t kd = umma_desc_sw128(sKV + st * W::kOperand, 16, 1024);
+          const uint32_t is = tree ? IST : IS, d = tmem + g * 128;
+          if (elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk)
-          umma_f16(tmem + g * 128, desc_add(qd, kmajor_off(kk)), desc_add(kd, kmajor_off(kk)), tree ? IST : IS,
-                   kk > 0);
-        umma_commit(s_full(g));
-        umma_commit(empty(s));
-        if (tree || q + 1 == n_tiles) umma_commit(q_empty(items_s & 1));  // the item's last S has read Q
-        next<kBlockKeys>(a, cs, end);
-        return true;
-      };
-      auto issue_pv = [&](int q) -> bool {
-        const int i = v_index(q), s = i % NS, g = q & 1;
-        const bool tree = cp.j == cp.row.blocks - 1;
-        if (q == 0 || cp.j == 0) {
-          ++items_p;
-          first[0] = first[1] = true;
+            for (int kk = 0; kk < D / 16; ++kk)
+              umma_f16(d, desc_add(qd, kmajor_off(kk)), desc_add(kd, kmajor_off(kk)), is, kk > 0);
+            umma_commit(s_full(g));
+            umma_commit(empty(st));
+            if (tree || q + 1 == n_tiles) umma_commit(q_empty(items_s & 1));  // the item's last S has read Q
+          }
+          __syncwarp();
+          next<kBlockKeys>(a, cs, end);
         }
-        if (!mbar_wait(p_full(g), (q >> 1) & 1, a.err, FXB_DERR_ATTN_WAIT)) return false;
-        if (!mbar_wait(full(s), (i / NS) & 1, a.err, FXB_DERR_ATTN_WAIT)) return false;
-        // O of the previous item has been read
-        if (first[g] && items_p > 0 && !mbar_wait(o_free, (items_p - 1) & 1, a.err, FXB_DERR_ATTN_WAIT)) return false;
-        tc_fence_after();
-        const uint64_t vd = umma_desc_sw128(sKV + s * W::kOperand, 16384, 1024);
-        const int steps = tree ? kMaxTree / 16 : kBlockKeys / 16;
+        if (q > 0) {
+          const int p = q - 1, i = v_index(p), st = i % NS, g = p & 1;
+          const bool tree = cp.j == cp.row.blocks - 1;
+          if (p == 0 || cp.j == 0) {
+            ++items_p;
+            first = 3;
+          }
+          if (!mbar_wait_warp(p_full(g), (p >> 1) & 1, a.err, FXB_DERR_ATTN_WAIT)) break;
+          if (!mbar_wait_warp(full(st), (i / NS) & 1, a.err, FXB_DERR_ATTN_WAIT)) break;
+          // O of the previous item has been read
+          if (((first >> g) & 1) && items_p > 0 && !mbar_wait_warp(o_free, (items_p - 1) & 1, a.err, FXB_DERR_ATTN_WAIT)) break;
+          tc_fence_after();
+          const uint64_t vd = umma_desc_sw128(sKV + st * W::kOperand, 16384, 1024);
+          const uint32_t o = tmem + 256 + g * 128, pr = tmem + g * 128;
+          const uint32_t add = ((first >> g) & 1) ^ 1;
+          if (elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < kBlockKeys / 16; ++kk)
-          if (kk < steps)
-            umma_f16_ta(tmem + 256 + g * 128, tmem + g * 128 + kk * 8, desc_add(vd, mnmajor_off(kk)), IPV,
-                        (!first[g] || kk > 0) ? 1u : 0u);
-        umma_commit(pv_done(g));
-        umma_commit(empty(s));
-        first[g] = false;
-        next<kBlockKeys>(a, cp, end);
-        return true;
-      };
-      ok = issue_s(0);
-      for (int q = 0; q < n_tiles && ok; ++q) {
-        if (q + 1 < n_tiles) ok = issue_s(q + 1);
-        if (ok) ok = issue_pv(q);
+            for (int kk = 0; kk < kMaxTree / 16; ++kk)
+              umma_f16_ta(o, pr + kk * 8, desc_add(vd, mnmajor_off(kk)), IPV, kk > 0 ? 1u : add);
+            if (!tree) {
+#pragma unroll
+              for (int kk = kMaxTree / 16; kk < kBlockKeys / 16; ++kk)
+                umma_f16_ta(o, pr + kk * 8, desc_add(vd, mnmajor_off(kk)), IPV, 1u);
+            }
+            umma_commit(pv_done(g));
+            umma_commit(empty(st));
+          }
+          __syncwarp();
+          first &= ~(1u << g);
+          next<kBlockKeys>(a, cp, end);
+        }
       }
-      umma_commit(final_bar);
-      mbar_wait(final_bar, 0, a.err, FXB_DERR_ATTN_WAIT);
+      if (elect_one()) umma_commit(final_bar);
+      mbar_wait_warp(final_bar, 0, a.err, FXB_DERR_ATTN_WAIT);
     }
     __syncwarp();
   } else if (warp == kWarpStore) {
@@ -332,12 +349,13 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
           const int valid = tree ? c.row.n : min(c.row.len - c.j * kBlockKeys, kBlockKeys);
           const int vi = v_index(q), vslot = vi % NS;
           const int cols = tree ? kMaxTree : kBlockKeys;
-          // values that no row may count are zeroed (0 * NaN is NaN): behind the sequence, or nodes that
-          // do not exist; infinities and NaN of nodes too: who sees them adds them at the item's end
-          if (valid < cols || tree) {
+          if (valid < cols || tree) {  // tail of the context, or nodes
+            // values that no row may count are zeroed (0 * NaN is NaN): behind the sequence, or nodes that
+            // do not exist; infinities and NaN of nodes too: who sees them adds them at the item's end
             if (!uwait(full(vslot), (vi / NS) & 1)) ok = false;
             uint8_t* vs = gbase + (sKV - base) + vslot * W::kOperand;
             bool odd = false;
+#pragma unroll 1
             for (int i = r; i < cols * (D / 8); i += 128) {
               const int row = i / (D / 8);
               uint4* p = reinterpret_cast<uint4*>(vs + sw(row, i % (D / 8)));
@@ -359,77 +377,92 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
             }
             if (odd) atomicExch(&odd_value[item % 3], 1);
             fence_proxy_async_smem();
+            // scores that do not count
+            if (!dead) {
+#pragma unroll 1
+              for (int i0 = 0; i0 < cols; i0 += 32) {
+                const int in = min(max(valid - i0, 0), 32);
+                uint32_t w = in == 32 ? 0xffffffffu : (1u << in) - 1;
+                if (tree) w &= (uint32_t)(see >> i0);
+                uint32_t v[32];
+                tmem_ld32(tS + i0, v);
+                tmem_wait_ld32(v);
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                  if (!((w >> i) & 1)) v[i] = __float_as_uint(-INFINITY);
+                tmem_st32(tS + i0, v);
+                tmem_wait_st();
+              }
+            }
           }
           if (!dead) {
-          uint32_t v[128];
+            // Two passes over the scores, in rolled loops: with the row in 128 registers the code of a tile
+            // outgrew the instruction cache, and every warp waited for instructions (3450 cycles a tile).
+            float mv[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+            for (int i0 = 0; i0 < cols; i0 += 64) {
+              uint32_t v[32], w[32];
+              tmem_ld32(tS + i0, v);
+              tmem_ld32(tS + i0 + 32, w);
+              tmem_wait_ld32(v);
+              tmem_wait_ld32(w);
 #pragma unroll
-          for (int i = 0; i < 2; ++i) tmem_ld32(tS + i * 32, v + 32 * i);
-          if (!tree) {
+              for (int i = 0; i < 32; ++i)
+                mv[i & 3] = fmaxf(fmaxf(mv[i & 3], __uint_as_float(v[i])), __uint_as_float(w[i]));
+            }
+            const float mx = fmaxf(fmaxf(mv[0], mv[1]), fmaxf(mv[2], mv[3])) * a.scale_log2;
+            // the reference maximum m moves only when a tile exceeds it by more than 2^8: probabilities stay
+            // below 2^8, which 16 bits hold as well as [0, 1], and O is rarely rescaled
+            if (mine == 0) {
+              m = mx;  // the group's first P V of the item overwrites O
+            } else if (__any_sync(0xffffffffu, mx > m + kRescaleLog2)) {
+              if (!uwait(pv_done(g), (done - 1) & 1)) ok = false;
+              tc_fence_after();
+              const bool up = mx > m + kRescaleLog2;
+              const float f = up ? ex2(m - mx) : 1.f;
+#pragma unroll 1
+              for (int i = 0; i < D / 32; ++i) {
+                uint32_t o[32];
+                tmem_ld32(tO + g * 128 + i * 32, o);
+                tmem_wait_ld32(o);
 #pragma unroll
-            for (int i = 2; i < 4; ++i) tmem_ld32(tS + i * 32, v + 32 * i);
-          }
-          tmem_wait_ld();
-          if (tree) {
+                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                tmem_st32(tO + g * 128 + i * 32, o);
+              }
+              tmem_wait_st();
+              l *= f;
+              if (up) m = mx;
+            }
+            const float z = m == -INFINITY ? 0.f : m;
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            // probabilities of 32 keys, over scores that have been read; they enter the second product in the
+            // inputs' type, as its operands must
+            auto probabilities = [&](const uint32_t* v, int i0) {
+              uint32_t p[16];
 #pragma unroll
-            for (int i = 0; i < 64; ++i)
-              if (!((see >> i) & 1) || i >= valid) v[i] = __float_as_uint(-INFINITY);
-#pragma unroll
-            for (int i = 64; i < 128; ++i) v[i] = __float_as_uint(-INFINITY);
-          } else if (valid < kBlockKeys) {
-#pragma unroll
-            for (int i = 0; i < 128; ++i)
-              if (i >= valid) v[i] = __float_as_uint(-INFINITY);
-          }
-          float mv[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) mv[i] = -INFINITY;
-#pragma unroll
-          for (int i = 0; i < 128; ++i) mv[i & 7] = fmaxf(mv[i & 7], __uint_as_float(v[i]));
-          const float mx = fmaxf(fmaxf(fmaxf(mv[0], mv[1]), fmaxf(mv[2], mv[3])),
-                                 fmaxf(fmaxf(mv[4], mv[5]), fmaxf(mv[6], mv[7]))) * a.scale_log2;
-          // the reference maximum m moves only when a tile exceeds it by more than 2^8: probabilities stay
-          // below 2^8, which 16 bits hold as well as [0, 1], and O is rarely rescaled
-          if (mine == 0) {
-            m = mx;  // the group's first P V of the item overwrites O
-          } else if (__any_sync(0xffffffffu, mx > m + kRescaleLog2)) {
-            if (!uwait(pv_done(g), (done - 1) & 1)) ok = false;
-            tc_fence_after();
-            const bool up = mx > m + kRescaleLog2;
-            const float f = up ? ex2(m - mx) : 1.f;
-#pragma unroll
-            for (int i = 0; i < D / 16; ++i) {
-              uint32_t o[16];
-              tmem_ld16(tO + g * 128 + i * 16, o);
-              tmem_wait_ld();
-#pragma unroll
-              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-              tmem_st16(tO + g * 128 + i * 16, o);
+              for (int i = 0; i < 16; ++i) {
+                const float p0 = ex2(fmaf(__uint_as_float(v[2 * i]), a.scale_log2, -z));
+                const float p1 = ex2(fmaf(__uint_as_float(v[2 * i + 1]), a.scale_log2, -z));
+                sum[(2 * i) & 3] += p0;
+                sum[(2 * i + 1) & 3] += p1;
+                p[i] = pack2<T>(p0, p1);
+              }
+              tmem_st16(tS + i0 / 2, p);
+            };
+            uint32_t v[32], w[32];
+            tmem_ld32(tS, v);
+            tmem_wait_ld32(v);
+#pragma unroll 1
+            for (int i0 = 0; i0 < cols; i0 += 64) {
+              tmem_ld32(tS + i0 + 32, w);
+              probabilities(v, i0);
+              tmem_wait_ld32(w);
+              if (i0 + 64 < cols) tmem_ld32(tS + i0 + 64, v);
+              probabilities(w, i0 + 32);
+              tmem_wait_ld32(v);
             }
             tmem_wait_st();
-            l *= f;
-            if (up) m = mx;
-          }
-          const float z = m == -INFINITY ? 0.f : m;
-          float sum[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) sum[i] = 0.f;
-          // probabilities enter the second product in the inputs' type, as its operands must
-#pragma unroll
-          for (int i0 = 0; i0 < 128; i0 += 32) {
-            if (i0 >= 64 && tree) continue;
-            uint32_t p[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float p0 = ex2(fmaf(__uint_as_float(v[i0 + 2 * i]), a.scale_log2, -z));
-              const float p1 = ex2(fmaf(__uint_as_float(v[i0 + 2 * i + 1]), a.scale_log2, -z));
-              sum[(2 * i) & 7] += p0;
-              sum[(2 * i + 1) & 7] += p1;
-              p[i] = pack2<T>(p0, p1);
-            }
-            tmem_st16(tS + i0 / 2, p);
-          }
-          tmem_wait_st();
-          l += ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7]));
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
           }
           tc_fence_before();
           mbar_arrive(p_full(g));
@@ -460,7 +493,7 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
       float* part = a.parts + ((int64_t)blockIdx.x * 2 + begun) * W::kPart;
       const int d0 = g * (D / 2);
       tc_fence_after();
-#pragma unroll
+#pragma unroll 1
       for (int i = 0; i < D / 2 / 16; ++i) {
         uint32_t o0[16], o1[16];
         tmem_ld16(tO + d0 + i * 16, o0);
