@@ -13,49 +13,6 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kRows = 16;               // rows of a tile
 constexpr int kTile = 16;               // keys a warp takes at once
 
-// State of an item's part in the workspace: m and l of each row, then O.
-template <int ROWS, int D>
-FXB_DEV float* part_of(const Params& a, int cta, int place) {
-  return a.parts + ((int64_t)cta * 2 + place) * ROWS * (D + 2);
-}
-
-// Called by all threads after this thread block's part is written: the last
-// one to arrive joins the parts and writes the item's rows.
-template <typename T, int ROWS, int D>
-FXB_DEV void join_parts(const Params& a, int b, int hk, int row0, int64_t u_first, int64_t u_last, int64_t total) {
-  __shared__ int last;
-  const int lo = owner(u_first, total), hi = owner(u_last, total);
-  __threadfence();
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    const unsigned before = atomicAdd(&a.arrived[lo], 1u);
-    last = before == (unsigned)(hi - lo);
-    if (last) a.arrived[lo] = 0;  // for the next call
-  }
-  __syncthreads();
-  if (!last) return;
-  __threadfence();
-  for (int i = threadIdx.x; i < ROWS * (D / 4); i += kThreads) {
-    const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
-    if (row0 + r >= a.R) break;
-    float m = -INFINITY, l = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int c = lo; c <= hi; ++c) {
-      const float* p = part_of<ROWS, D>(a, c, c == lo);
-      const float mc = __ldcg(p + r), lc = __ldcg(p + ROWS + r);
-      const float4 oc = __ldcg(reinterpret_cast<const float4*>(p + 2 * ROWS + r * D + d));
-      const float mx = fmaxf(m, mc);
-      const float w0 = weight(m, mx), w1 = weight(mc, mx);
-      o = make_float4(o.x * w0, o.y * w0, o.z * w0, o.w * w0);
-      axpy4(o, w1, oc);
-      l = fmaf(l, w0, lc * w1);
-      m = mx;
-    }
-    write_out<T, D>(a, b, hk, row0 + r, d, o, l);
-  }
-}
-
 // ------------------------------------------------------------------ few rows: a warp takes 16 keys at once
 template <typename T, int D> struct Shape {
   static constexpr int kBoxCols = 128 / sizeof(T);           // columns of a 128-byte swizzled row
@@ -405,6 +362,7 @@ tree_attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t bars[kWarps][ST];
   __shared__ float sm[kWarps][kRows], sl[kWarps][kRows];
+  __shared__ int s_last;
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint8_t* ring = smem + warp * ST * S::kSlot;
@@ -519,7 +477,7 @@ tree_attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       const bool whole = begun && tree;
       float* part = part_of<kRows, D>(a, blockIdx.x, begun);
       for (int i = threadIdx.x; i < kRows * (D / 4); i += kThreads) {
-        const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
+        const int r = i % kRows, d = i / kRows * 4;
         float mx = sm[0][r];
 #pragma unroll
         for (int w = 1; w < kWarps; ++w) mx = fmaxf(mx, sm[w][r]);
@@ -539,10 +497,25 @@ tree_attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
             part[r] = mx;
             part[kRows + r] = l;
           }
-          *reinterpret_cast<float4*>(part + 2 * kRows + r * D + d) = o;
+          reinterpret_cast<float4*>(part + 2 * kRows)[(d / 4) * kRows + r] = o;
         }
       }
-      if (!whole) join_parts<T, kRows, D>(a, cur.b, hk, row0, u_begin, u_last, total);
+      if (!whole) {  // the last thread block to arrive joins the parts
+        const int lo = owner(u_begin, total), hi = owner(u_last, total);
+        __threadfence();
+        __syncthreads();
+        if (threadIdx.x == 0) {
+          const unsigned before = atomicAdd(&a.arrived[lo], 1u);
+          s_last = before == (unsigned)(hi - lo);
+          if (s_last) a.arrived[lo] = 0;  // for the next call
+        }
+        __syncthreads();
+        if (s_last) {
+          __threadfence();
+          constexpr int kStep = kThreads / kRows;
+          join_row<T, kRows, D, D / 4 / kStep>(a, cur.b, hk, row0, threadIdx.x % kRows, threadIdx.x / kRows, kStep, lo, hi);
+        }
+      }
       __syncthreads();
       fence_proxy_async_smem();  // what was written here comes before the copies into it
       fresh = true;
@@ -573,10 +546,9 @@ int rows_grid(int dtype, int D) {
   return ctas * fxb::num_sms();
 }
 
-size_t workspace_bytes(int dtype, int T, int G, int D) {
-  const size_t floats = many_rows(dtype, T, G) ? fxb::num_sms() * 2 * wide_part_floats(D)
-                                               : (size_t)rows_grid(dtype, D) * 2 * kRows * (D + 2);
-  return kMaxGrid * sizeof(unsigned) + floats * sizeof(float);
+size_t workspace_bytes(const fxb_tree_attn_args* x) {
+  if (many_rows(x->dtype, x->T, x->Hq / x->Hkv)) return wide_workspace(x);
+  return kCounters + (size_t)rows_grid(x->dtype, x->D) * 2 * kRows * (x->D + 2) * sizeof(float);
 }
 
 template <typename T, int D>
@@ -605,10 +577,17 @@ extern "C" {
 
 size_t fxb_tree_attn_workspace(int32_t dtype, int32_t B, int32_t T, int32_t Hq, int32_t Hkv, int32_t D) {
   if ((D != 64 && D != 128) || !fxb::dtype_size(dtype) || B < 1 || T < 1 || Hkv < 1 || Hq < Hkv) return 0;
-  return workspace_bytes(dtype, T, Hq / Hkv, D);
+  fxb_tree_attn_args x = {};
+  x.dtype = dtype;
+  x.B = B;
+  x.T = T;
+  x.Hq = Hq;
+  x.Hkv = Hkv;
+  x.D = D;
+  return workspace_bytes(&x);
 }
 size_t fxb_tree_attn_workspace_zeroed(int32_t dtype, int32_t B, int32_t T, int32_t Hq, int32_t Hkv, int32_t D) {
-  return fxb_tree_attn_workspace(dtype, B, T, Hq, Hkv, D) ? kMaxGrid * sizeof(unsigned) : 0;
+  return fxb_tree_attn_workspace(dtype, B, T, Hq, Hkv, D) ? kCounters : 0;
 }
 
 int fxb_tree_attn(const fxb_tree_attn_args* a, void* stream) {
@@ -641,7 +620,7 @@ int fxb_tree_attn(const fxb_tree_attn_args* a, void* stream) {
     return fxb::set_error(FXB_EINVAL, "fxb_tree_attn: scale must be positive and finite");
   const int G = a->Hq / a->Hkv;
   if (!a->workspace || !fxb::aligned16(a->workspace) ||
-      a->workspace_bytes < (int64_t)workspace_bytes(a->dtype, a->T, G, a->D))
+      a->workspace_bytes < (int64_t)workspace_bytes(a))
     return fxb::set_error(FXB_EINVAL, "fxb_tree_attn: workspace of fxb_tree_attn_workspace bytes, 16-byte aligned");
   if (rows_grid(a->dtype, a->D) > kMaxGrid)
     return fxb::set_error(FXB_EUNSUPPORTED, "fxb_tree_attn: device with too many SMs");
@@ -673,7 +652,7 @@ int fxb_tree_attn(const fxb_tree_attn_args* a, void* stream) {
   p.mask = a->mask;
   p.mask_sb = a->mask_sb;
   p.arrived = static_cast<unsigned*>(a->workspace);
-  p.parts = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + kMaxGrid * sizeof(unsigned));
+  p.parts = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + kCounters);
   p.err = err;
   if (many_rows(a->dtype, a->T, G)) return launch_wide(a, p, stream);
   if (a->dtype == FXB_DTYPE_F32)

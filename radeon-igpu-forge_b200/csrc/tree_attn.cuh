@@ -12,9 +12,9 @@
 // cut into tiles of rows. An item's keys are its context in blocks of
 // BLOCK_KEYS slots and one block of nodes. All items' blocks in a row are
 // divided evenly over the thread blocks, so uneven lengths cost nothing; an
-// item that several thread blocks share is joined by the one that finishes
-// last, from states in the workspace, in the order of the keys (the result
-// does not depend on who that is).
+// item that several thread blocks share is joined from their states in the
+// workspace, in the order of the keys: by the thread block that finishes last
+// (few rows), or by a second kernel (many rows, whose states are large).
 #pragma once
 #include "common.cuh"
 #include "internal.h"
@@ -23,6 +23,7 @@ namespace fxb_tree {
 
 constexpr int kMaxTree = 64;
 constexpr int kMaxGrid = 1024;        // arrival counters in the workspace
+constexpr size_t kCounters = kMaxGrid * sizeof(unsigned);  // the same place for both kernels: it stays zero
 constexpr float kRescaleLog2 = 8.f;   // how far a row's reference maximum may lag behind, in powers of two
 
 FXB_DEV float ex2(float x) {
@@ -43,8 +44,10 @@ struct Params {
   const int32_t *lens, *n_nodes;
   const int64_t* mask;
   int64_t mask_sb;
-  unsigned* arrived;  // workspace: kMaxGrid counters,
-  float* parts;       // then two states for every thread block
+  // workspace: kMaxGrid counters of arrivals (few rows; an item's is that of the block that begins it),
+  unsigned* arrived;
+  int2* owners;  // then the first and last thread block of each item (many rows),
+  float* parts;  // then two states for every thread block
   int* err;
 };
 
@@ -153,9 +156,6 @@ template <int BLOCK_KEYS, int THREADS> FXB_DEV Cursor share(const Params& a, int
 FXB_DEV int owner(int64_t u, int64_t total) { return (int)(((u + 1) * sharers(total) - 1) / total); }
 
 // ------------------------------------------------------------------ joining states
-// Parts. A thread block has two places in the workspace: 1 for an item that it
-// begins, 0 for one that it continues. The arrival counter of an item is that
-// of the block that begins it.
 template <typename T, int D>
 FXB_DEV void write_out(const Params& a, int b, int hk, int r, int d, float4 o, float l) {
   if (r >= a.R) return;
@@ -177,6 +177,56 @@ FXB_DEV void axpy4(float4& o, float w, const float4& x) {
 // weight of a state with maximum m in a join with maximum mx
 FXB_DEV float weight(float m, float mx) { return m == -INFINITY ? 0.f : ex2(m - mx); }
 
+// State of an item's part in the workspace: m and l of each row, then O as
+// [D / 4][ROWS] float4. A thread block has two places: 1 for an item that it
+// begins, 0 for one that it continues.
+template <int ROWS, int D> FXB_DEV float* part_of(const Params& a, int cta, int place) {
+  return a.parts + ((int64_t)cta * 2 + place) * ROWS * (D + 2);
+}
+
+// Joins the parts [lo, hi] of an item (those of thread blocks lo to hi), in
+// the order of the keys: row r of the tile at row0, its quads d4, d4 + step,
+// ... A part costs a trip to L2 whatever is read of it, so four are under way
+// at once.
+template <typename T, int ROWS, int D, int NQ>
+FXB_DEV void join_row(const Params& a, int b, int hk, int row0, int r, int d4, int step, int lo, int hi) {
+  float m = -INFINITY, l = 0.f;
+  float4 o[NQ];
+#pragma unroll
+  for (int x = 0; x < NQ; ++x) o[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+  for (int k0 = lo; k0 <= hi; k0 += 4) {
+    float mk[4], lk[4];
+    float4 ok[4][NQ];
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      const int k = min(k0 + y, hi);
+      const float* p = part_of<ROWS, D>(a, k, k == lo);
+      mk[y] = k0 + y <= hi ? __ldcg(p + r) : -INFINITY;
+      lk[y] = __ldcg(p + ROWS + r);
+#pragma unroll
+      for (int x = 0; x < NQ; ++x)
+        ok[y][x] = __ldcg(reinterpret_cast<const float4*>(p + 2 * ROWS) + (d4 + x * step) * ROWS + r);
+    }
+    const float mn = fmaxf(fmaxf(fmaxf(m, mk[0]), fmaxf(mk[1], mk[2])), mk[3]);
+    const float f = weight(m, mn);
+    l *= f;
+#pragma unroll
+    for (int x = 0; x < NQ; ++x) o[x] = make_float4(o[x].x * f, o[x].y * f, o[x].z * f, o[x].w * f);
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      if (k0 + y > hi) break;
+      const float w = weight(mk[y], mn);
+      l = fmaf(w, lk[y], l);
+#pragma unroll
+      for (int x = 0; x < NQ; ++x) axpy4(o[x], w, ok[y][x]);
+    }
+    m = mn;
+  }
+#pragma unroll
+  for (int x = 0; x < NQ; ++x) write_out<T, D>(a, b, hk, row0 + r, (d4 + x * step) * 4, o[x], l);
+}
+
 // ------------------------------------------------------------------ host
 // (outer, mid, rows, D) view with element strides, 128-byte swizzle; boxes of
 // box_rows x box_mid rows of 128 bytes. The stride of an axis of one entry is
@@ -196,7 +246,7 @@ inline int grid_of(const fxb_tree_attn_args* x, const Params& a, int block_keys,
   return (int)(n < most ? n : most);
 }
 // the kernel for many rows (tree_attn_wide.cu): 16-bit types, G <= 128
-size_t wide_part_floats(int D);
+size_t wide_workspace(const fxb_tree_attn_args* x);
 int launch_wide(const fxb_tree_attn_args* x, Params& a, void* stream);
 
 }  // namespace fxb_tree

@@ -4,19 +4,18 @@
 // A row tile is up to 128 rows (whole nodes: 128 / G of them) against tiles of
 // 128 keys; the block of nodes is one tile of 64. Persistent thread blocks, one
 // an SM, walk their share of all tiles. Roles (352 threads):
-//   warps 0-3, 4-7  two softmax groups; a thread owns one row. Tiles go to the
-//                   groups in turn, and each group keeps a state (m, l, O) of
-//                   its own, so that nothing is exchanged between them until
-//                   the item ends;
-//   warp 8          issues the products: S = Q K^T of a tile while the other
-//                   group's tile is in its softmax, O += P V;
+//   warps 0-3, 4-7  softmax: a thread owns a row and one half of a tile's keys;
+//                   the two threads of a row exchange its maximum;
+//   warp 8          issues the products: S = Q K^T of the next tile while a
+//                   tile is in its softmax, then O += P V;
 //   warp 9          copies Q, keys and values by TMA, a lane a page;
 //   warp 10         writes the nodes' keys and values into the cache.
-// Tensor memory (512 columns): group g's scores at 128 g (fp32; the 16-bit
-// probabilities overwrite their first half: the A operand of P V), its O at
-// 256 + 128 g.
+// Tensor memory (512 columns): scores of two tiles at 0 and 128 (fp32),
+// probabilities of two tiles at 256 and 320 (16 bits, the A operand of P V), O
+// at 384. Scores are free as soon as they are in registers, so that the tensor
+// cores and the softmax run side by side.
 // Keys and values go through one ring of operands in the order of their use
-// (K0 K1 V0 K2 V1 ...), Q through two buffers.
+// (K0 K1 V0 K2 V1 ...).
 #include "tree_attn.cuh"
 
 namespace {
@@ -32,8 +31,8 @@ constexpr int kSoftmax = 256;  // threads of both groups
 template <int D> struct Wide {
   static constexpr int kBoxes = D / 64;
   static constexpr int kOperand = kTileRows * D * 2;  // Q, K or V of a tile: D / 64 blocks of [128 rows][128 bytes]
-  static constexpr int kSlots = D == 128 ? 4 : 10;    // ring of keys and values
-  static constexpr int kSmem = 1024 + (2 + kSlots) * kOperand;
+  static constexpr int kSlots = D == 128 ? 5 : 11;    // ring of keys and values
+  static constexpr int kSmem = 1024 + (1 + kSlots) * kOperand;
   static constexpr int kPart = kTileRows * (D + 2);   // floats of a state in the workspace
 };
 static_assert(Wide<128>::kSmem + 5120 <= 232448 && Wide<64>::kSmem + 5120 <= 232448, "shared memory");
@@ -56,8 +55,9 @@ FXB_DEV void tmem_wait_ld32(uint32_t* r) {
                : "memory");
 }
 
-struct Exchange {  // per item parity
-  float m[2][kTileRows], l[2][kTileRows];  // of each group's state
+struct Exchange {
+  float m[2][2][kTileRows];  // [tile parity][half]: a row's maximum over half a tile
+  float l[2][2][kTileRows];  // [item parity][half]: its sum over the item
 };
 
 template <typename T, int D>
@@ -71,21 +71,20 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
   constexpr int FMT = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t bars[2 * NS + 12];
-  __shared__ Exchange xch[2];
+  __shared__ Exchange xch;
   __shared__ int odd_value[3];  // an item's node has a value that is not finite (items in turn)
   __shared__ uint32_t tmem_slot;
-  __shared__ int s_last;
   const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
   uint8_t* gbase = smem_raw + (base - raw);
-  const uint32_t sQ = base, sKV = base + 2 * W::kOperand;
+  const uint32_t sQ = base, sKV = base + W::kOperand;
   const uint32_t bar0 = smem_u32(bars);
   auto full = [&](int s) { return bar0 + 8u * s; };
   auto empty = [&](int s) { return bar0 + 8u * (NS + s); };
-  auto q_full = [&](int i) { return bar0 + 8u * (2 * NS + i); };
-  auto q_empty = [&](int i) { return bar0 + 8u * (2 * NS + 2 + i); };
-  auto s_full = [&](int g) { return bar0 + 8u * (2 * NS + 4 + g); };
-  auto p_full = [&](int g) { return bar0 + 8u * (2 * NS + 6 + g); };
-  auto pv_done = [&](int g) { return bar0 + 8u * (2 * NS + 8 + g); };
+  const uint32_t q_full = bar0 + 8u * (2 * NS), q_empty = bar0 + 8u * (2 * NS + 1);
+  auto s_full = [&](int i) { return bar0 + 8u * (2 * NS + 2 + i); };   // of tile parity i
+  auto s_empty = [&](int i) { return bar0 + 8u * (2 * NS + 4 + i); };
+  auto p_full = [&](int i) { return bar0 + 8u * (2 * NS + 6 + i); };
+  auto pv_done = [&](int i) { return bar0 + 8u * (2 * NS + 8 + i); };
   const uint32_t o_free = bar0 + 8u * (2 * NS + 10), final_bar = bar0 + 8u * (2 * NS + 11);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -95,13 +94,14 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
       mbar_init(empty(s), 1);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(q_full(i), 1);
-      mbar_init(q_empty(i), 1);
       mbar_init(s_full(i), 1);
-      mbar_init(p_full(i), 128);
+      mbar_init(s_empty(i), kSoftmax);
+      mbar_init(p_full(i), kSoftmax);
       mbar_init(pv_done(i), 1);
     }
     odd_value[0] = odd_value[1] = odd_value[2] = 0;
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
     mbar_init(o_free, kSoftmax);
     mbar_init(final_bar, 1);
     fence_mbar_init();
@@ -114,8 +114,8 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  pdl_trigger();
   pdl_wait();
+  pdl_trigger();  // after the wait: what the joining kernel reads before its own is then complete
 
   int64_t end, total;
   Cursor c = share<kBlockKeys, kThreads>(a, &end, &total);
@@ -175,14 +175,13 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
       for (int q = 0; q <= n_tiles && ok; ++q) {
         if (q < n_tiles && (q == 0 || f.j == 0)) {  // the item's rows of Q
           ++items;
-          const int qb = items & 1;
-          ok = mbar_wait_warp(q_empty(qb), ((items >> 1) & 1) ^ 1, a.err, FXB_DERR_ATTN_WAIT);
+          ok = mbar_wait_warp(q_empty, (items & 1) ^ 1, a.err, FXB_DERR_ATTN_WAIT);
           if (!ok) break;
           if (lane == 0) {
-            mbar_expect_tx(q_full(qb), a.NT * a.G * 128 * NBOX);
+            mbar_expect_tx(q_full, a.NT * a.G * 128 * NBOX);
 #pragma unroll
             for (int x = 0; x < NBOX; ++x)
-              tma_load_4d(sQ + qb * W::kOperand + x * 16384, &tmQ, q_full(qb), x * 64, (f.hr / a.RT) * a.G,
+              tma_load_4d(sQ + x * 16384, &tmQ, q_full, x * 64, (f.hr / a.RT) * a.G,
                           (f.hr % a.RT) * a.NT, f.b);
           }
         }
@@ -201,8 +200,7 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
       // what is under way lands before shared memory goes
       for (int i = max(0, issued - NS); i < issued; ++i)
         mbar_wait_warp(full(i % NS), (i / NS) & 1, a.err, FXB_DERR_ATTN_WAIT);
-      for (int i = max(0, items - 1); i <= items; ++i)
-        mbar_wait_warp(q_full(i & 1), (i >> 1) & 1, a.err, FXB_DERR_ATTN_WAIT);
+      if (items >= 0) mbar_wait_warp(q_full, items & 1, a.err, FXB_DERR_ATTN_WAIT);
     }
   } else if (warp == kWarpMma) {
     // ------------------------------------------------ products: the warp stays together, one lane issues
@@ -210,8 +208,12 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
       constexpr uint32_t IS = umma_idesc_f16(FMT, 0, 0, kTileRows, kBlockKeys);
       constexpr uint32_t IST = umma_idesc_f16(FMT, 0, 0, kTileRows, kMaxTree);
       constexpr uint32_t IPV = umma_idesc_f16(FMT, 0, 1, kTileRows, D);
+      // all lanes poll: a completed wait costs an instruction, not an exchange between lanes
+      auto uwait = [&](uint32_t bar, uint32_t parity) -> bool {
+        return __all_sync(0xffffffffu, mbar_wait(bar, parity, a.err, FXB_DERR_ATTN_WAIT));
+      };
       int items_s = -1, items_p = -1;  // items begun by S products, by P V products
-      unsigned first = 3;              // bit g: the group's next P V begins its O
+      bool first = true;               // the next P V begins O
       Cursor cs = c, cp = c;
       // step q: S of tile q, then P V of tile q - 1. Issued by an elected lane of the whole
       // warp: the operands of a product are then known to be uniform
@@ -222,13 +224,12 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
           const bool tree = cs.j == cs.row.blocks - 1;
           if (q == 0 || cs.j == 0) {
             ++items_s;
-            if (!mbar_wait_warp(q_full(items_s & 1), (items_s >> 1) & 1, a.err, FXB_DERR_ATTN_WAIT)) break;
+            if (!uwait(q_full, items_s & 1)) break;
           }
-          if (!mbar_wait_warp(full(st), (i / NS) & 1, a.err, FXB_DERR_ATTN_WAIT)) break;
-          // these columns still hold the probabilities of tile q - 2 until its P V is complete
-          if (q >= 2 && !mbar_wait_warp(pv_done(g), ((q - 2) >> 1) & 1, a.err, FXB_DERR_ATTN_WAIT)) break;
+          if (!uwait(full(st), (i / NS) & 1)) break;
+          if (!uwait(s_empty(g), ((q >> 1) & 1) ^ 1)) break;
           tc_fence_after();
-          const uint64_t qd = umma_desc_sw128(sQ + (items_s & 1) * W::kOperand, 16, 1024);
+          const uint64_t qd = umma_desc_sw128(sQ, 16, 1024);
           const uint64_t kd = umma_desc_sw128(sKV + st * W::kOperand, 16, 1024);
           const uint32_t is = tree ? IST : IS, d = tmem + g * 128;
           if (elect_one()) {
@@ -237,7 +238,7 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
               umma_f16(d, desc_add(qd, kmajor_off(kk)), desc_add(kd, kmajor_off(kk)), is, kk > 0);
             umma_commit(s_full(g));
             umma_commit(empty(st));
-            if (tree || q + 1 == n_tiles) umma_commit(q_empty(items_s & 1));  // the item's last S has read Q
+            if (tree || q + 1 == n_tiles) umma_commit(q_empty);  // the item's last S has read Q
           }
           __syncwarp();
           next<kBlockKeys>(a, cs, end);
@@ -247,16 +248,16 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
           const bool tree = cp.j == cp.row.blocks - 1;
           if (p == 0 || cp.j == 0) {
             ++items_p;
-            first = 3;
+            first = true;
           }
-          if (!mbar_wait_warp(p_full(g), (p >> 1) & 1, a.err, FXB_DERR_ATTN_WAIT)) break;
-          if (!mbar_wait_warp(full(st), (i / NS) & 1, a.err, FXB_DERR_ATTN_WAIT)) break;
+          if (!uwait(p_full(g), (p >> 1) & 1)) break;
+          if (!uwait(full(st), (i / NS) & 1)) break;
           // O of the previous item has been read
-          if (((first >> g) & 1) && items_p > 0 && !mbar_wait_warp(o_free, (items_p - 1) & 1, a.err, FXB_DERR_ATTN_WAIT)) break;
+          if (first && items_p > 0 && !uwait(o_free, (items_p - 1) & 1)) break;
           tc_fence_after();
           const uint64_t vd = umma_desc_sw128(sKV + st * W::kOperand, 16384, 1024);
-          const uint32_t o = tmem + 256 + g * 128, pr = tmem + g * 128;
-          const uint32_t add = ((first >> g) & 1) ^ 1;
+          const uint32_t o = tmem + 384, pr = tmem + 256 + g * 64;
+          const uint32_t add = first ? 0u : 1u;
           if (elect_one()) {
 #pragma unroll
             for (int kk = 0; kk < kMaxTree / 16; ++kk)
@@ -270,7 +271,7 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
             umma_commit(empty(st));
           }
           __syncwarp();
-          first &= ~(1u << g);
+          first = false;
           next<kBlockKeys>(a, cp, end);
         }
       }
@@ -315,208 +316,174 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
     }
   } else {
     // ------------------------------------------------ softmax
-    const int g = warp >> 2, r = (warp & 3) * 32 + lane;  // group, row of the tile
+    const int g = warp >> 2, r = (warp & 3) * 32 + lane;  // half of the keys, row of the tile
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t tS = tmem + lane_off + g * 128, tO = tmem + lane_off + 256;
-    int done = 0;   // tiles of this group so far
+    const uint32_t tS = tmem + lane_off, tP = tmem + lane_off + 256, tO = tmem + lane_off + 384 + g * (D / 2);
     int item = 0;
     auto uwait = [&](uint32_t bar, uint32_t parity) -> bool {
       return __all_sync(0xffffffffu, mbar_wait(bar, parity, a.err, FXB_DERR_ATTN_WAIT));
     };
     float m = -INFINITY, l = 0.f;
-    int mine = 0;   // tiles of this group in the item
     bool live = false, dead = true;  // this row is a node's; no row of this warp is
     uint64_t see = 0;
     int64_t u_first = 0;
+#pragma unroll 1
     for (int q = 0; q < n_tiles; ++q) {
-      const int hk = c.hr / a.RT, t0 = (c.hr % a.RT) * a.NT;
-      const bool tree = c.j == c.row.blocks - 1;
-      if (q == 0 || c.j == 0) {
+      const int hk = c.hr / a.RT, t0 = (c.hr % a.RT) * a.NT, par = q & 1;
+      const bool tree = c.j == c.row.blocks - 1, begins = q == 0 || c.j == 0;
+      if (begins) {
         u_first = c.u - c.j;
         m = -INFINITY;
         l = 0.f;
-        mine = 0;
         const int t = t0 + r / a.G;
         live = r < a.NT * a.G && t < c.row.n;
         see = live ? (uint64_t)a.mask[c.b * a.mask_sb + t] : 0;
         dead = !__any_sync(0xffffffffu, live);
       }
-      Exchange& x = xch[item & 1];
-      if ((q & 1) == g) {
-        if (ok && !uwait(s_full(g), done & 1)) ok = false;
-        if (ok) {
-          tc_fence_after();
-          const int valid = tree ? c.row.n : min(c.row.len - c.j * kBlockKeys, kBlockKeys);
+      if (ok && !uwait(s_full(par), (q >> 1) & 1)) ok = false;
+      if (ok) {
+        tc_fence_after();
+        const int valid = tree ? c.row.n : min(c.row.len - c.j * kBlockKeys, kBlockKeys);
+        const int cols = tree ? kMaxTree : kBlockKeys;
+        const int c0 = g * (cols / 2);  // this thread's columns: 64, or 32 of the nodes
+        const bool some = valid < cols || tree;
+        uint32_t v[64];
+        tmem_ld32(tS + par * 128 + c0, v);
+        tmem_ld32(tS + par * 128 + min(c0 + 32, 96), v + 32);
+        tmem_wait_ld32(v);
+        tmem_wait_ld32(v + 32);
+        tc_fence_before();
+        mbar_arrive(s_empty(par));
+        if (some) {  // tail of the context, or nodes
+          const int in = min(max(valid - c0, 0), 64);
+          uint64_t w = in == 64 ? ~0ull : (1ull << in) - 1;
+          if (tree) w &= (see >> c0) & 0xffffffffull;
+#pragma unroll
+          for (int i = 0; i < 64; ++i)
+            if (!((w >> i) & 1)) v[i] = __float_as_uint(-INFINITY);
+          // values that no row may count are zeroed (0 * NaN is NaN): behind the sequence, or nodes that
+          // do not exist; infinities and NaN of nodes too: who sees them adds them at the item's end
           const int vi = v_index(q), vslot = vi % NS;
-          const int cols = tree ? kMaxTree : kBlockKeys;
-          if (valid < cols || tree) {  // tail of the context, or nodes
-            // values that no row may count are zeroed (0 * NaN is NaN): behind the sequence, or nodes that
-            // do not exist; infinities and NaN of nodes too: who sees them adds them at the item's end
-            if (!uwait(full(vslot), (vi / NS) & 1)) ok = false;
-            uint8_t* vs = gbase + (sKV - base) + vslot * W::kOperand;
-            bool odd = false;
+          if (!uwait(full(vslot), (vi / NS) & 1)) ok = false;
+          uint8_t* vs = gbase + (sKV - base) + vslot * W::kOperand;
+          bool odd = false;
 #pragma unroll 1
-            for (int i = r; i < cols * (D / 8); i += 128) {
-              const int row = i / (D / 8);
-              uint4* p = reinterpret_cast<uint4*>(vs + sw(row, i % (D / 8)));
-              if (row >= valid) {
-                *p = make_uint4(0, 0, 0, 0);
-              } else if (tree) {
-                float f[8];
-                unpack8<T>(*p, f);
-                bool any = false;
+          for (int i = threadIdx.x; i < cols * (D / 8); i += kSoftmax) {
+            const int row = i / (D / 8);
+            uint4* p = reinterpret_cast<uint4*>(vs + sw(row, i % (D / 8)));
+            if (row >= valid) {
+              *p = make_uint4(0, 0, 0, 0);
+            } else if (tree) {
+              float f[8];
+              unpack8<T>(*p, f);
+              bool any = false;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                  const bool fin = fabsf(f[e]) < INFINITY;
-                  any |= !fin;
-                  f[e] = fin ? f[e] : 0.f;
-                }
-                if (any) *p = pack8<T>(f);
-                odd |= any;
+              for (int e = 0; e < 8; ++e) {
+                const bool fin = fabsf(f[e]) < INFINITY;
+                any |= !fin;
+                f[e] = fin ? f[e] : 0.f;
               }
-            }
-            if (odd) atomicExch(&odd_value[item % 3], 1);
-            fence_proxy_async_smem();
-            // scores that do not count
-            if (!dead) {
-#pragma unroll 1
-              for (int i0 = 0; i0 < cols; i0 += 32) {
-                const int in = min(max(valid - i0, 0), 32);
-                uint32_t w = in == 32 ? 0xffffffffu : (1u << in) - 1;
-                if (tree) w &= (uint32_t)(see >> i0);
-                uint32_t v[32];
-                tmem_ld32(tS + i0, v);
-                tmem_wait_ld32(v);
-#pragma unroll
-                for (int i = 0; i < 32; ++i)
-                  if (!((w >> i) & 1)) v[i] = __float_as_uint(-INFINITY);
-                tmem_st32(tS + i0, v);
-                tmem_wait_st();
-              }
+              if (any) *p = pack8<T>(f);
+              odd |= any;
             }
           }
-          if (!dead) {
-            // Two passes over the scores, in rolled loops: with the row in 128 registers the code of a tile
-            // outgrew the instruction cache, and every warp waited for instructions (3450 cycles a tile).
-            float mv[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll 1
-            for (int i0 = 0; i0 < cols; i0 += 64) {
-              uint32_t v[32], w[32];
-              tmem_ld32(tS + i0, v);
-              tmem_ld32(tS + i0 + 32, w);
-              tmem_wait_ld32(v);
-              tmem_wait_ld32(w);
+          if (odd) atomicExch(&odd_value[item % 3], 1);
+          fence_proxy_async_smem();
+        }
+        if (!dead) {
+          float mv[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-              for (int i = 0; i < 32; ++i)
-                mv[i & 3] = fmaxf(fmaxf(mv[i & 3], __uint_as_float(v[i])), __uint_as_float(w[i]));
-            }
-            const float mx = fmaxf(fmaxf(mv[0], mv[1]), fmaxf(mv[2], mv[3])) * a.scale_log2;
-            // the reference maximum m moves only when a tile exceeds it by more than 2^8: probabilities stay
-            // below 2^8, which 16 bits hold as well as [0, 1], and O is rarely rescaled
-            if (mine == 0) {
-              m = mx;  // the group's first P V of the item overwrites O
-            } else if (__any_sync(0xffffffffu, mx > m + kRescaleLog2)) {
-              if (!uwait(pv_done(g), (done - 1) & 1)) ok = false;
-              tc_fence_after();
-              const bool up = mx > m + kRescaleLog2;
-              const float f = up ? ex2(m - mx) : 1.f;
+          for (int i = 0; i < 32; ++i)
+            mv[i & 3] = fmaxf(fmaxf(mv[i & 3], __uint_as_float(v[i])), __uint_as_float(v[32 + i]));
+          float mx = fmaxf(fmaxf(mv[0], mv[1]), fmaxf(mv[2], mv[3]));
+          xch.m[par][g][r] = mx;
+          named_bar_sync(2 + (warp & 3), 64);  // the row's two threads
+          mx = fmaxf(mx, xch.m[par][g ^ 1][r]) * a.scale_log2;
+          // the reference maximum m moves only when a tile exceeds it by more than 2^8: probabilities stay
+          // below 2^8, which 16 bits hold as well as [0, 1], and O is rarely rescaled
+          if (begins) {
+            m = mx;  // the item's first P V overwrites O
+          } else if (__any_sync(0xffffffffu, mx > m + kRescaleLog2)) {
+            if (!uwait(pv_done(par ^ 1), ((q - 1) >> 1) & 1)) ok = false;
+            tc_fence_after();
+            const bool up = mx > m + kRescaleLog2;
+            const float f = up ? ex2(m - mx) : 1.f;
 #pragma unroll 1
-              for (int i = 0; i < D / 32; ++i) {
-                uint32_t o[32];
-                tmem_ld32(tO + g * 128 + i * 32, o);
-                tmem_wait_ld32(o);
+            for (int i = 0; i < D / 2 / 16; ++i) {
+              uint32_t o[16];
+              tmem_ld16(tO + i * 16, o);
+              tmem_wait_ld();
 #pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                tmem_st32(tO + g * 128 + i * 32, o);
-              }
-              tmem_wait_st();
-              l *= f;
-              if (up) m = mx;
-            }
-            const float z = m == -INFINITY ? 0.f : m;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
-            // probabilities of 32 keys, over scores that have been read; they enter the second product in the
-            // inputs' type, as its operands must
-            auto probabilities = [&](const uint32_t* v, int i0) {
-              uint32_t p[16];
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const float p0 = ex2(fmaf(__uint_as_float(v[2 * i]), a.scale_log2, -z));
-                const float p1 = ex2(fmaf(__uint_as_float(v[2 * i + 1]), a.scale_log2, -z));
-                sum[(2 * i) & 3] += p0;
-                sum[(2 * i + 1) & 3] += p1;
-                p[i] = pack2<T>(p0, p1);
-              }
-              tmem_st16(tS + i0 / 2, p);
-            };
-            uint32_t v[32], w[32];
-            tmem_ld32(tS, v);
-            tmem_wait_ld32(v);
-#pragma unroll 1
-            for (int i0 = 0; i0 < cols; i0 += 64) {
-              tmem_ld32(tS + i0 + 32, w);
-              probabilities(v, i0);
-              tmem_wait_ld32(w);
-              if (i0 + 64 < cols) tmem_ld32(tS + i0 + 64, v);
-              probabilities(w, i0 + 32);
-              tmem_wait_ld32(v);
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tmem_st16(tO + i * 16, o);
             }
             tmem_wait_st();
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            l *= f;
+            if (up) m = mx;
           }
-          tc_fence_before();
-          mbar_arrive(p_full(g));
         }
-        ++done;
-        ++mine;
+        // the place of the probabilities is free once P V of tile q - 2 is complete
+        if (q >= 2 && !uwait(pv_done(par), ((q - 2) >> 1) & 1)) ok = false;
+        if (!dead) {
+          const float z = m == -INFINITY ? 0.f : m;
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          // probabilities enter the second product in the inputs' type, as its operands must
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (h == 1 && tree) break;
+            uint32_t p[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float p0 = ex2(fmaf(__uint_as_float(v[32 * h + 2 * i]), a.scale_log2, -z));
+              const float p1 = ex2(fmaf(__uint_as_float(v[32 * h + 2 * i + 1]), a.scale_log2, -z));
+              sum[(2 * i) & 3] += p0;
+              sum[(2 * i + 1) & 3] += p1;
+              p[i] = pack2<T>(p0, p1);
+            }
+            tmem_st16(tP + par * 64 + c0 / 2 + 16 * h, p);
+          }
+          tmem_wait_st();
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        }
+        tc_fence_before();
+        mbar_arrive(p_full(par));
       }
       const Cursor cur = c;
       next<kBlockKeys>(a, c, end);
       if (!tree && q + 1 < n_tiles) continue;
-      // ---- the item ends here: both groups' states join
-      if (ok && mine && !uwait(pv_done(g), (done - 1) & 1)) ok = false;
-      x.m[g][r] = live ? m : -INFINITY;
-      x.l[g][r] = live ? l : 0.f;
-      const int n_item = (int)(cur.u - max(u_first, start)) + 1;  // this thread block's tiles of the item
+      // ---- the item ends here
+      if (ok && !uwait(pv_done(par), (q >> 1) & 1)) ok = false;
+      xch.l[item & 1][g][r] = live ? l : 0.f;
       // the next item's flag, last read two items ago (every thread has passed the barrier since); the
-      // exchange of this item is written again two items on, likewise
+      // exchange of sums is written again two items on, likewise
       if (threadIdx.x == 0) odd_value[(item + 1) % 3] = 0;
-      tc_fence_before();
       named_bar_sync(1, kSoftmax);
       const bool begun = u_first >= start, whole = begun && tree;
-      const float m0 = x.m[0][r], m1 = x.m[1][r];
-      const float mj = fmaxf(m0, m1), w0 = weight(m0, mj), w1 = weight(m1, mj);
-      const float lj = fmaf(x.l[0][r], w0, x.l[1][r] * w1);
-      // a group without a tile of this item has no O
-      const bool has0 = n_item > 1 || (q & 1) == 0, has1 = n_item > 1 || (q & 1) == 1;
+      const float mj = live ? m : -INFINITY, lj = xch.l[item & 1][0][r] + xch.l[item & 1][1][r];
       const int rows = min(a.NT, a.T - t0) * a.G;
-      float* part = a.parts + ((int64_t)blockIdx.x * 2 + begun) * W::kPart;
-      const int d0 = g * (D / 2);
+      float* part = part_of<kTileRows, D>(a, blockIdx.x, begun);
       tc_fence_after();
 #pragma unroll 1
       for (int i = 0; i < D / 2 / 16; ++i) {
-        uint32_t o0[16], o1[16];
-        tmem_ld16(tO + d0 + i * 16, o0);
-        tmem_ld16(tO + 128 + d0 + i * 16, o1);
+        uint32_t ov[16];
+        tmem_ld16(tO + i * 16, ov);
         tmem_wait_ld();
         if (r < rows && ok) {
+          const int d0 = g * (D / 2) + i * 16;
           float o[16];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float y0 = has0 ? __uint_as_float(o0[e]) * w0 : 0.f, y1 = has1 ? __uint_as_float(o1[e]) * w1 : 0.f;
-            o[e] = live ? y0 + y1 : 0.f;
-          }
+          for (int e = 0; e < 16; ++e) o[e] = live ? __uint_as_float(ov[e]) : 0.f;
           if (tree && odd_value[item % 3])
             for (int j = 0; j < cur.row.n; ++j)
               if ((see >> j) & 1)
                 for (int e = 0; e < 16; ++e) {
-                  const float y = to_f<T>(static_cast<const T*>(new_v)[cur.b * v_sb + j * v_st + hk * v_sh + d0 + i * 16 + e]);
+                  const float y = to_f<T>(static_cast<const T*>(new_v)[cur.b * v_sb + j * v_st + hk * v_sh + d0 + e]);
                   if (!(fabsf(y) < INFINITY)) o[e] += y;
                 }
 #pragma unroll
           for (int e = 0; e < 16; e += 4) {
             const float4 o4 = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-            const int d = d0 + i * 16 + e;
+            const int d = d0 + e;
             if (whole) write_out<T, D>(a, cur.b, hk, t0 * a.G + r, d, o4, lj);
             else reinterpret_cast<float4*>(part + 2 * kTileRows)[(d / 4) * kTileRows + r] = o4;
           }
@@ -524,43 +491,13 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
       }
       tc_fence_before();
       mbar_arrive(o_free);
-      if (!whole) {
-        if (g == 0 && r < rows) {
-          part[r] = mj;
-          part[kTileRows + r] = lj;
-        }
-        const int64_t u_last = u_first + cur.row.blocks - 1;
-        const int lo = owner(u_first, total), hi = owner(u_last, total);
-        __threadfence();
-        named_bar_sync(1, kSoftmax);
-        if (threadIdx.x == 0) {
-          const unsigned before = atomicAdd(&a.arrived[lo], 1u);
-          s_last = before == (unsigned)(hi - lo);
-          if (s_last) a.arrived[lo] = 0;  // for the next call
-        }
-        named_bar_sync(1, kSoftmax);
-        if (s_last) {  // the parts in the order of the keys
-          __threadfence();
-          for (int i = threadIdx.x; i < rows * (D / 4); i += kSoftmax) {
-            const int rr = i % rows, d4 = i / rows;
-            float pm = -INFINITY, pl = 0.f;
-            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-            for (int k = lo; k <= hi; ++k) {
-              const float* p = a.parts + ((int64_t)k * 2 + (k == lo)) * W::kPart;
-              const float mk = __ldcg(p + rr), lk = __ldcg(p + kTileRows + rr);
-              const float4 ok4 = __ldcg(reinterpret_cast<const float4*>(p + 2 * kTileRows) + d4 * kTileRows + rr);
-              const float mn = fmaxf(pm, mk);
-              const float f0 = weight(pm, mn), f1 = weight(mk, mn);
-              o = make_float4(o.x * f0, o.y * f0, o.z * f0, o.w * f0);
-              axpy4(o, f1, ok4);
-              pl = fmaf(pl, f0, lk * f1);
-              pm = mn;
-            }
-            write_out<T, D>(a, cur.b, hk, t0 * a.G + rr, d4 * 4, o, pl);
-          }
-        }
+      if (!whole && g == 0 && r < rows) {
+        part[r] = mj;
+        part[kTileRows + r] = lj;
       }
+      if (begun && threadIdx.x == 0)
+        a.owners[(int64_t)cur.b * a.Hkv * a.RT + cur.hr] =
+            make_int2(blockIdx.x, owner(u_first + cur.row.blocks - 1, total));
       ++item;
     }
   }
@@ -571,6 +508,23 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
+}
+
+// Joins the items that several thread blocks share: a block takes 32 rows of
+// an item, a lane a row, a warp a sixteenth of its columns.
+constexpr int kJoinThreads = 512;
+template <typename T, int D>
+__global__ void __launch_bounds__(kJoinThreads) tree_attn_join(const Params a) {
+  pdl_trigger();
+  pdl_wait();
+  const int2 own = a.owners[blockIdx.x];
+  if (own.x == own.y) return;
+  const int hr = blockIdx.x % (a.Hkv * a.RT), b = blockIdx.x / (a.Hkv * a.RT);
+  const int hk = hr / a.RT, t0 = (hr % a.RT) * a.NT;
+  const int r = blockIdx.y * 32 + (threadIdx.x & 31), warp = threadIdx.x >> 5;
+  if (r >= min(a.NT, a.T - t0) * a.G) return;
+  constexpr int kStep = kJoinThreads / 32;
+  join_row<T, kTileRows, D, D / 4 / kStep>(a, b, hk, t0 * a.G, r, warp, kStep, own.x, own.y);
 }
 
 template <typename T> constexpr CUtensorMapDataType map_type() {
@@ -593,6 +547,10 @@ int launch(const fxb_tree_attn_args* x, Params& a, int grid, void* stream) {
     return r;
   fxb::pdl_launch(tree_attn_wide<T, D>, dim3(grid), dim3(kThreads), Wide<D>::kSmem, fxb::as_stream(stream), q, k, v,
                   nk, nv, x->v, x->v_sb, x->v_st, x->v_sh, x->k, x->k_sb, x->k_st, x->k_sh, a);
+  if (int r = fxb::check_launch("fxb_tree_attn")) return r;
+  const int chunks = (a.NT * a.G + 31) / 32;
+  fxb::pdl_launch(tree_attn_join<T, D>, dim3((unsigned)(a.B * a.Hkv * a.RT), chunks), dim3(kJoinThreads), 0,
+                  fxb::as_stream(stream), a);
   return fxb::check_launch("fxb_tree_attn");
 }
 
@@ -600,11 +558,22 @@ int launch(const fxb_tree_attn_args* x, Params& a, int grid, void* stream) {
 
 namespace fxb_tree {
 
-size_t wide_part_floats(int D) { return D == 64 ? Wide<64>::kPart : Wide<128>::kPart; }
+// nodes of a row tile, row tiles
+static int nodes_of(int T, int G) { return T < kTileRows / G ? T : kTileRows / G; }
+static size_t owners_bytes(int B, int Hkv, int RT) { return ((size_t)B * Hkv * RT * sizeof(int2) + 255) / 256 * 256; }
+
+size_t wide_workspace(const fxb_tree_attn_args* x) {
+  const int NT = nodes_of(x->T, x->Hq / x->Hkv), RT = (x->T + NT - 1) / NT;
+  return kCounters + owners_bytes(x->B, x->Hkv, RT) +
+         (size_t)fxb::num_sms() * 2 * (x->D == 64 ? Wide<64>::kPart : Wide<128>::kPart) * sizeof(float);
+}
 
 int launch_wide(const fxb_tree_attn_args* x, Params& a, void* stream) {
-  a.NT = a.T < kTileRows / a.G ? a.T : kTileRows / a.G;
+  a.NT = nodes_of(a.T, a.G);
   a.RT = (a.T + a.NT - 1) / a.NT;
+  char* ws = static_cast<char*>(x->workspace) + kCounters;
+  a.owners = reinterpret_cast<int2*>(ws);
+  a.parts = reinterpret_cast<float*>(ws + owners_bytes(a.B, a.Hkv, a.RT));
   const int grid = grid_of(x, a, kBlockKeys, fxb::num_sms());
   if (x->dtype == FXB_DTYPE_F16)
     return x->D == 64 ? launch<__half, 64>(x, a, grid, stream) : launch<__half, 128>(x, a, grid, stream);
