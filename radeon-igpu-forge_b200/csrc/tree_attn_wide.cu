@@ -3,11 +3,12 @@
 //
 // A row tile is up to 128 rows (whole nodes: 128 / G of them) against tiles of
 // 128 keys; the block of nodes is one tile of 64. Persistent thread blocks, one
-// an SM, walk their share of all tiles. Roles (352 threads):
+// an SM, walk their share of all tiles. Roles (384 threads):
 //   warps 0-3, 4-7  softmax: a thread owns a row and one half of a tile's keys;
 //                   the two threads of a row exchange its maximum;
-//   warp 8          issues the products: S = Q K^T of the next tile while a
-//                   tile is in its softmax, then O += P V;
+//   warp 8          issues S = Q K^T, up to two tiles ahead of the softmax;
+//   warp 11         issues O += P V (a warp of its own: when keys are late it
+//                   still takes what the softmax has finished);
 //   warp 9          copies Q, keys and values by TMA, a lane a page;
 //   warp 10         writes the nodes' keys and values into the cache.
 // Tensor memory (512 columns): scores of two tiles at 0 and 128 (fp32),
@@ -24,8 +25,8 @@ using namespace fxb_tree;
 
 constexpr int kTileRows = 128;
 constexpr int kBlockKeys = 128;
-constexpr int kThreads = 352;
-constexpr int kWarpMma = 8, kWarpTma = 9, kWarpStore = 10;
+constexpr int kThreads = 384;
+constexpr int kWarpS = 8, kWarpTma = 9, kWarpStore = 10, kWarpPV = 11;
 constexpr int kSoftmax = 256;  // threads of both groups
 
 template <int D> struct Wide {
@@ -85,7 +86,7 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
   auto s_empty = [&](int i) { return bar0 + 8u * (2 * NS + 4 + i); };
   auto p_full = [&](int i) { return bar0 + 8u * (2 * NS + 6 + i); };
   auto pv_done = [&](int i) { return bar0 + 8u * (2 * NS + 8 + i); };
-  const uint32_t o_free = bar0 + 8u * (2 * NS + 10), final_bar = bar0 + 8u * (2 * NS + 11);
+  const uint32_t o_free = bar0 + 8u * (2 * NS + 10), final_bar = bar0 + 8u * (2 * NS + 11);  // all products are complete
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -103,10 +104,10 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
     mbar_init(q_full, 1);
     mbar_init(q_empty, 1);
     mbar_init(o_free, kSoftmax);
-    mbar_init(final_bar, 1);
+    mbar_init(final_bar, 2);
     fence_mbar_init();
   }
-  if (warp == kWarpMma) {
+  if (warp == kWarpS) {
     tmem_alloc(smem_u32(&tmem_slot), 512);
     tmem_relinquish();
   }
@@ -137,17 +138,12 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
     }
     const int page = 1 << a.page_shift, box_rows = min(page, kBlockKeys), per_tile = kBlockKeys / box_rows;
     int items = -1, issued = 0;
-    // this lane's page of the tile at f: -1 none; ids outside the pool read page 0 (and are reported)
+    // this lane's page of the tile at f, as the table has it. Nothing may depend on it here: it is read a step
+    // ahead of its use, and the warp waits at the first instruction that needs it
     auto page_of = [&](const Cursor& f) {
-      if (f.u >= end || f.j == f.row.blocks - 1) return -1;
       const int slot0 = f.j * kBlockKeys + lane * box_rows;
-      if (lane >= per_tile || slot0 >= f.row.len) return -1;
-      int pg = a.table[f.b * a.table_sb + (slot0 >> a.page_shift)];
-      if (pg < 0 || pg >= a.P) {
-        atomicOr(a.err, FXB_DERR_PAGES);
-        pg = 0;
-      }
-      return pg;
+      const bool has = f.u < end && f.j < f.row.blocks - 1 && lane < per_tile && slot0 < f.row.len;
+      return has ? a.table[f.b * a.table_sb + (slot0 >> a.page_shift)] : 0;
     };
     auto load = [&](const Cursor& f, int pg, const CUtensorMap* ctx, const CUtensorMap* nodes) -> bool {
       const int s = issued % NS;
@@ -158,6 +154,10 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
       if (lane == 0) mbar_expect_tx(full(s), pages * (tree ? kMaxTree : box_rows) * 128 * NBOX);
       __syncwarp();
       if (lane < pages) {
+        if (!tree && (pg < 0 || pg >= a.P)) {  // outside the pool: reported, page 0 is read instead
+          atomicOr(a.err, FXB_DERR_PAGES);
+          pg = 0;
+        }
         const uint32_t dst = sKV + s * W::kOperand + (tree ? 0 : lane * box_rows * 128);
         const int row = tree ? 0 : (f.j * kBlockKeys) & (page - 1);  // 0 unless a page holds several tiles
 #pragma unroll
@@ -202,83 +202,75 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
         mbar_wait_warp(full(i % NS), (i / NS) & 1, a.err, FXB_DERR_ATTN_WAIT);
       if (items >= 0) mbar_wait_warp(q_full, items & 1, a.err, FXB_DERR_ATTN_WAIT);
     }
-  } else if (warp == kWarpMma) {
-    // ------------------------------------------------ products: the warp stays together, one lane issues
-    if (n_tiles) {
+  } else if (warp == kWarpS || warp == kWarpPV) {
+    // ------------------------------------------------ products. The whole warp keeps together and polls (a
+    // completed wait costs an instruction, not an exchange between lanes); an elected lane issues, and the
+    // operands of a product are known to be uniform
+    auto uwait = [&](uint32_t bar, uint32_t parity) -> bool {
+      return __all_sync(0xffffffffu, mbar_wait(bar, parity, a.err, FXB_DERR_ATTN_WAIT));
+    };
+    int items = -1;  // items begun
+    if (warp == kWarpS) {
       constexpr uint32_t IS = umma_idesc_f16(FMT, 0, 0, kTileRows, kBlockKeys);
       constexpr uint32_t IST = umma_idesc_f16(FMT, 0, 0, kTileRows, kMaxTree);
-      constexpr uint32_t IPV = umma_idesc_f16(FMT, 0, 1, kTileRows, D);
-      // all lanes poll: a completed wait costs an instruction, not an exchange between lanes
-      auto uwait = [&](uint32_t bar, uint32_t parity) -> bool {
-        return __all_sync(0xffffffffu, mbar_wait(bar, parity, a.err, FXB_DERR_ATTN_WAIT));
-      };
-      int items_s = -1, items_p = -1;  // items begun by S products, by P V products
-      bool first = true;               // the next P V begins O
-      Cursor cs = c, cp = c;
-      // step q: S of tile q, then P V of tile q - 1. Issued by an elected lane of the whole
-      // warp: the operands of a product are then known to be uniform
+      const uint64_t qd = umma_desc_sw128(sQ, 16, 1024);
 #pragma unroll 1
-      for (int q = 0; q <= n_tiles; ++q) {
-        if (q < n_tiles) {
-          const int i = k_index(q), st = i % NS, g = q & 1;
-          const bool tree = cs.j == cs.row.blocks - 1;
-          if (q == 0 || cs.j == 0) {
-            ++items_s;
-            if (!uwait(q_full, items_s & 1)) break;
-          }
-          if (!uwait(full(st), (i / NS) & 1)) break;
-          if (!uwait(s_empty(g), ((q >> 1) & 1) ^ 1)) break;
-          tc_fence_after();
-          const uint64_t qd = umma_desc_sw128(sQ, 16, 1024);
-          const uint64_t kd = umma_desc_sw128(sKV + st * W::kOperand, 16, 1024);
-          const uint32_t is = tree ? IST : IS, d = tmem + g * 128;
-          if (elect_one()) {
-#pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk)
-              umma_f16(d, desc_add(qd, kmajor_off(kk)), desc_add(kd, kmajor_off(kk)), is, kk > 0);
-            umma_commit(s_full(g));
-            umma_commit(empty(st));
-            if (tree || q + 1 == n_tiles) umma_commit(q_empty);  // the item's last S has read Q
-          }
-          __syncwarp();
-          next<kBlockKeys>(a, cs, end);
+      for (int q = 0; q < n_tiles; ++q) {
+        const int i = k_index(q), st = i % NS, par = q & 1;
+        const bool tree = c.j == c.row.blocks - 1;
+        if (q == 0 || c.j == 0) {
+          ++items;
+          if (!uwait(q_full, items & 1)) break;
         }
-        if (q > 0) {
-          const int p = q - 1, i = v_index(p), st = i % NS, g = p & 1;
-          const bool tree = cp.j == cp.row.blocks - 1;
-          if (p == 0 || cp.j == 0) {
-            ++items_p;
-            first = true;
-          }
-          if (!uwait(p_full(g), (p >> 1) & 1)) break;
-          if (!uwait(full(st), (i / NS) & 1)) break;
-          // O of the previous item has been read
-          if (first && items_p > 0 && !uwait(o_free, (items_p - 1) & 1)) break;
-          tc_fence_after();
-          const uint64_t vd = umma_desc_sw128(sKV + st * W::kOperand, 16384, 1024);
-          const uint32_t o = tmem + 384, pr = tmem + 256 + g * 64;
-          const uint32_t add = first ? 0u : 1u;
-          if (elect_one()) {
+        if (!uwait(s_empty(par), ((q >> 1) & 1) ^ 1)) break;
+        if (!uwait(full(st), (i / NS) & 1)) break;
+        tc_fence_after();
+        const uint64_t kd = umma_desc_sw128(sKV + st * W::kOperand, 16, 1024);
+        const uint32_t is = tree ? IST : IS, d = tmem + par * 128;
+        if (elect_one()) {
 #pragma unroll
-            for (int kk = 0; kk < kMaxTree / 16; ++kk)
-              umma_f16_ta(o, pr + kk * 8, desc_add(vd, mnmajor_off(kk)), IPV, kk > 0 ? 1u : add);
-            if (!tree) {
-#pragma unroll
-              for (int kk = kMaxTree / 16; kk < kBlockKeys / 16; ++kk)
-                umma_f16_ta(o, pr + kk * 8, desc_add(vd, mnmajor_off(kk)), IPV, 1u);
-            }
-            umma_commit(pv_done(g));
-            umma_commit(empty(st));
-          }
-          __syncwarp();
-          first = false;
-          next<kBlockKeys>(a, cp, end);
+          for (int kk = 0; kk < D / 16; ++kk)
+            umma_f16(d, desc_add(qd, kmajor_off(kk)), desc_add(kd, kmajor_off(kk)), is, kk > 0);
+          umma_commit(s_full(par));
+          umma_commit(empty(st));
+          if (tree || q + 1 == n_tiles) umma_commit(q_empty);  // the item's last S has read Q
         }
+        __syncwarp();
+        next<kBlockKeys>(a, c, end);
       }
-      if (elect_one()) umma_commit(final_bar);
-      mbar_wait_warp(final_bar, 0, a.err, FXB_DERR_ATTN_WAIT);
+    } else {
+      constexpr uint32_t IPV = umma_idesc_f16(FMT, 0, 1, kTileRows, D);
+      const uint32_t o = tmem + 384;
+#pragma unroll 1
+      for (int q = 0; q < n_tiles; ++q) {
+        const int i = v_index(q), st = i % NS, par = q & 1;
+        const bool tree = c.j == c.row.blocks - 1, first = q == 0 || c.j == 0;
+        if (first) ++items;
+        if (!uwait(full(st), (i / NS) & 1)) break;
+        // the item's first product overwrites O: that of the previous item has been read
+        if (first && items > 0 && !uwait(o_free, (items - 1) & 1)) break;
+        if (!uwait(p_full(par), (q >> 1) & 1)) break;
+        tc_fence_after();
+        const uint64_t vd = umma_desc_sw128(sKV + st * W::kOperand, 16384, 1024);
+        const uint32_t pr = tmem + 256 + par * 64;
+        if (elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < kMaxTree / 16; ++kk)
+            umma_f16_ta(o, pr + kk * 8, desc_add(vd, mnmajor_off(kk)), IPV, kk > 0 || !first ? 1u : 0u);
+          if (!tree) {
+#pragma unroll
+            for (int kk = kMaxTree / 16; kk < kBlockKeys / 16; ++kk)
+              umma_f16_ta(o, pr + kk * 8, desc_add(vd, mnmajor_off(kk)), IPV, 1u);
+          }
+          umma_commit(pv_done(par));
+          umma_commit(empty(st));
+        }
+        __syncwarp();
+        next<kBlockKeys>(a, c, end);
+      }
     }
-    __syncwarp();
+    if (elect_one()) umma_commit(final_bar);
+    uwait(final_bar, 0);
   } else if (warp == kWarpStore) {
     // ------------------------------------------------ the nodes' keys and values into the cache
     constexpr int CH = D / 8;
@@ -504,7 +496,7 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
 
   tc_fence_before();
   __syncthreads();
-  if (warp == kWarpMma) {
+  if (warp == kWarpS) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
