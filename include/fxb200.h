@@ -46,7 +46,7 @@ const char* fxb_last_error(void);
 
 /* Reads (and with clear != 0 resets) the device error word that kernels set
  * when a bounded wait expires (bit 1 GEMM, 2 attention, 4 gather, 8 cross-
- * entropy), or when the page table or pool of a KV cache does not fit a call
+ * entropy, 32 verification), or when the page table or pool of a KV cache does not fit a call
  * (bit 16). Synchronises
  * the current device. No reference counterpart (the reference has no bounded
  * waits). */

@@ -25,6 +25,7 @@ enum {
   FXB_DERR_ATTN_WAIT = 2,
   FXB_DERR_GATHER_WAIT = 4,
   FXB_DERR_CE_WAIT = 8,
+  FXB_DERR_VERIFY_WAIT = 32,
   FXB_DERR_PAGES = 16,  // not a wait: page ids, counts or paths of a KV cache that do not fit
 };
 
