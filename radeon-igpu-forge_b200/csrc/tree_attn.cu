@@ -96,6 +96,7 @@ struct Rows16 {
     const int lane = threadIdx.x & 31;
     const uint32_t sk = smem_u32(slot), sv = sk + Shape<T, D>::kOperand;
     // scores of 16 rows x 16 keys; even and odd slices of D apart, for two shorter chains of products
+    const bool full = valid == kTile && !tree;
     float s[2][4] = {}, s1[2][4] = {};
 #pragma unroll
     for (int k = 0; k < D / 16; ++k) {
@@ -107,11 +108,16 @@ struct Rows16 {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int j = i * 8 + 2 * (lane & 3) + (e & 1);
-        const bool in = j < valid && (tree ? (see[e >> 1] >> (node0 + j)) & 1 : live[e >> 1]);
-        s[i][e] = in ? (s[i][e] + s1[i][e]) * a.scale_log2 : -INFINITY;
-      }
+      for (int e = 0; e < 4; ++e) s[i][e] += s1[i][e];
+    if (!full) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int j = i * 8 + 2 * (lane & 3) + (e & 1);
+          if (j >= valid || (tree && !((see[e >> 1] >> (node0 + j)) & 1))) s[i][e] = -INFINITY;
+        }
+    }
     // The reference maximum m of a row moves only when a tile exceeds it by
     // more than 2^8: probabilities then stay below 2^8, which fp32 sums and
     // 16-bit probabilities hold as well as [0, 1], and O is rarely rescaled.
@@ -120,7 +126,7 @@ struct Rows16 {
     for (int h = 0; h < 2; ++h) {
       float x = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1]));
       x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-      mx[h] = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+      mx[h] = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2)) * a.scale_log2;
     }
     const bool up0 = mx[0] > m[0] + kRescaleLog2, up1 = mx[1] > m[1] + kRescaleLog2;
     if (__any_sync(0xffffffffu, up0 || up1)) {
@@ -142,14 +148,15 @@ struct Rows16 {
     uint32_t p[4];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const float p0 = ex2(s[i][0] - z0), p1 = ex2(s[i][1] - z0), p2 = ex2(s[i][2] - z1), p3 = ex2(s[i][3] - z1);
+      const float p0 = ex2(fmaf(s[i][0], a.scale_log2, -z0)), p1 = ex2(fmaf(s[i][1], a.scale_log2, -z0));
+      const float p2 = ex2(fmaf(s[i][2], a.scale_log2, -z1)), p3 = ex2(fmaf(s[i][3], a.scale_log2, -z1));
       l[0] += p0 + p1;
       l[1] += p2 + p3;
       // the probabilities enter the second product in the inputs' type, as its operands must
       p[2 * i] = pack2<T>(p0, p1);
       p[2 * i + 1] = pack2<T>(p2, p3);
     }
-    if (valid < kTile || tree) {
+    if (!full) {
       // values that no row may count are zeroed (0 * NaN is NaN): those behind
       // the sequence, and infinities and NaN in nodes, which are then added
       // to the rows that see them
@@ -205,13 +212,13 @@ struct Rows16 {
       float x = l[h] + __shfl_xor_sync(0xffffffffu, l[h], 1);
       x += __shfl_xor_sync(0xffffffffu, x, 2);
       if ((lane & 3) == 0) {
-        sm[r + 8 * h] = m[h];
-        sl[r + 8 * h] = x;
+        sm[r + 8 * h] = live[h] ? m[h] : -INFINITY;
+        sl[r + 8 * h] = live[h] ? x : 0.f;
       }
 #pragma unroll
       for (int i = 0; i < D / 8; ++i)
         *reinterpret_cast<float2*>(slot + o_at<D>(r + 8 * h, i * 8 + 2 * (lane & 3))) =
-            make_float2(o[i][2 * h], o[i][2 * h + 1]);
+            live[h] ? make_float2(o[i][2 * h], o[i][2 * h + 1]) : make_float2(0.f, 0.f);
     }
   }
 };
@@ -380,59 +387,69 @@ tree_attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
   pdl_trigger();
   pdl_wait();
 
-  int64_t end, total;
-  Cursor c = share<kBlockKeys, kThreads>(a, &end, &total);
-  if (c.u >= end) return;
-  const int64_t start = c.u;
+  int64_t start;
+  Shares shares(1);
+  Cursor c = share<kBlockKeys, kThreads>(a, &start, &shares);
+  if (c.left == 0) return;
   Cursor f = c;          // the next block to fetch
-  int fetched = 0;       // stages filled so far, in order
+  int f_stage = 0;       // and its stage
   unsigned armed = 0;    // bit s: the copy in stage s is under way, or there and not yet used
-  // page of this warp's keys of block f; read one block ahead of its use
-  auto page_of = [&]() {
-    const int slot0 = f.j * kBlockKeys + warp * kTile;
-    return f.u < end && f.j < f.row.blocks - 1 && slot0 < f.row.len
-               ? a.table[f.b * a.table_sb + (slot0 >> a.page_shift)]
-               : -1;
+  // Page ids, read ahead: lane i has those of this warp's keys in block base + i of f's row (window), in block
+  // base + 32 + i (ahead), and in block i (front: where every key head of the row begins again)
+  const int in_block = warp * kTile;
+  auto pages_at = [&](int base) {
+    const int64_t at = ((int64_t)(base + lane) * kBlockKeys + in_block) >> a.page_shift;
+    return at < a.W ? a.table[f.b * a.table_sb + at] : -1;
   };
-  int pg = page_of();
-  auto fetch = [&]() {  // block f into stage fetched % ST; moves f on
-    if (f.u >= end) return;
-    const int s = fetched % ST;
-    const int hk = f.hr / a.RT;
+  int base = f.j, window = pages_at(base), ahead = pages_at(base + 32), front = pages_at(0);
+  auto fetch = [&]() {  // block f into its stage; moves f on
+    if (f.left == 0) return;
+    if (f.j >= base + 32) {
+      base += 32;
+      window = ahead;
+      ahead = pages_at(base + 32);
+    }
     const bool tree = f.j == f.row.blocks - 1;
-    const int at = tree ? warp * kTile : f.j * kBlockKeys + warp * kTile;
+    const int at = tree ? in_block : f.j * kBlockKeys + in_block;
+    const int pg = __shfl_sync(0xffffffffu, window, f.j - base);
     bool go = at < (tree ? f.row.n : f.row.len);
     if (go && !tree && (pg < 0 || pg >= a.P)) {
       if (lane == 0) atomicOr(a.err, FXB_DERR_PAGES);
       go = false;
     }
-    if (go) armed |= 1u << s;
+    if (go) armed |= 1u << f_stage;
     if (go && lane == 0) {
-      const uint32_t bar = smem_u32(&bars[warp][s]), dst = smem_u32(ring + s * S::kSlot);
+      const uint32_t bar = smem_u32(&bars[warp][f_stage]), dst = smem_u32(ring + f_stage * S::kSlot);
       const int row = tree ? at : at & ((1 << a.page_shift) - 1), d3 = tree ? f.b : pg;
       mbar_expect_tx(bar, S::kSlot);
 #pragma unroll
       for (int x = 0; x < S::kBoxes; ++x) {
-        tma_load_4d(dst + x * kTile * 128, tree ? &tmNK : &tmK, bar, x * S::kBoxCols, row, hk, d3);
-        tma_load_4d(dst + S::kOperand + x * kTile * 128, tree ? &tmNV : &tmV, bar, x * S::kBoxCols, row, hk, d3);
+        tma_load_4d(dst + x * kTile * 128, tree ? &tmNK : &tmK, bar, x * S::kBoxCols, row, f.hk, d3);
+        tma_load_4d(dst + S::kOperand + x * kTile * 128, tree ? &tmNV : &tmV, bar, x * S::kBoxCols, row, f.hk, d3);
       }
     }
-    ++fetched;
-    next<kBlockKeys>(a, f, end);
-    pg = page_of();
+    f_stage = f_stage + 1 == ST ? 0 : f_stage + 1;
+    const int b = f.b;
+    next<kBlockKeys>(a, f);
+    if (f.j == 0 && f.left) {
+      if (f.b != b) front = pages_at(0);
+      if (f.b != b || base) ahead = pages_at(32);
+      base = 0;
+      window = front;
+    }
   };
   for (int i = 0; i < ST; ++i) fetch();
 
   typename RowsOf<T, D>::type rows;
   unsigned phase = 0;    // bit s: parity of stage s
   bool ok = true, fresh = true;
-  int64_t u_begin = 0;
-  for (int it = 0; c.u < end; ++it) {
-    const int s = it % ST, hk = c.hr / a.RT, row0 = (c.hr % a.RT) * kRows;
+  int64_t u_begin = 0;   // the item's first block
+  for (int s = 0, done = 0; c.left; s = s + 1 == ST ? 0 : s + 1, ++done) {
+    const int hk = c.hk, row0 = c.rt * kRows;
     uint8_t* slot = ring + s * S::kSlot;
     if (fresh) {
       rows.begin(a, c.b, hk, row0, c.row.n, sq);
-      u_begin = c.u - c.j;
+      u_begin = start + done - c.j;
       fresh = false;
     }
     const bool tree = c.j == c.row.blocks - 1;
@@ -441,7 +458,7 @@ tree_attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       if (ok) {
         armed &= ~(1u << s);
         phase ^= 1u << s;
-        const int at = tree ? warp * kTile : c.j * kBlockKeys + warp * kTile;
+        const int at = tree ? in_block : c.j * kBlockKeys + in_block;
         const int valid = min(kTile, (tree ? c.row.n : c.row.len) - at);
         if (tree && row0 == 0) {  // the nodes' keys and values go into the cache
           constexpr int CH = D * (int)sizeof(T) / 16;
@@ -466,8 +483,8 @@ tree_attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       }
     }
     const Cursor cur = c;
-    next<kBlockKeys>(a, c, end);
-    if (tree || c.u >= end) {
+    next<kBlockKeys>(a, c);
+    if (tree || c.left == 0) {
       // the four warps' states join; each lies in the stage that its warp has just used up
       __syncwarp();
       rows.end(reinterpret_cast<float*>(slot), sm[warp], sl[warp]);
@@ -501,10 +518,10 @@ tree_attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         }
       }
       if (!whole) {  // the last thread block to arrive joins the parts
-        const int lo = owner(u_begin, total), hi = owner(u_last, total);
-        __threadfence();
+        const int lo = shares.owner(u_begin), hi = shares.owner(u_last);
         __syncthreads();
         if (threadIdx.x == 0) {
+          __threadfence();  // after the barrier: for the whole block's writes
           const unsigned before = atomicAdd(&a.arrived[lo], 1u);
           s_last = before == (unsigned)(hi - lo);
           if (s_last) a.arrived[lo] = 0;  // for the next call
@@ -512,8 +529,13 @@ tree_attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         __syncthreads();
         if (s_last) {
           __threadfence();
+          // 16 lanes of a row's quad: few rows leave several lanes for the parts of one
           constexpr int kStep = kThreads / kRows;
-          join_row<T, kRows, D, D / 4 / kStep>(a, cur.b, hk, row0, threadIdx.x % kRows, threadIdx.x / kRows, kStep, lo, hi);
+          const int live = min(kRows, a.R - row0);
+          const int lanes = live > 8 ? 16 : (live > 4 ? 8 : (live > 2 ? 4 : live));
+          const int x = threadIdx.x % kRows;
+          join_row<T, kRows, D, D / 4 / kStep, 128 / D * 2>(a, cur.b, hk, row0, x % lanes, threadIdx.x / kRows, kStep, lo, hi,
+                                               x / lanes, kRows / lanes, lanes);
         }
       }
       __syncthreads();

@@ -13,7 +13,7 @@
 // BLOCK_KEYS slots and one block of nodes. All items' blocks in a row are
 // divided evenly over the thread blocks, so uneven lengths cost nothing; an
 // item that several thread blocks share is joined from their states in the
-// workspace, in the order of the keys: by the thread block that finishes last
+// workspace, in a fixed order: by the thread block that finishes last
 // (few rows), or by a second kernel (many rows, whose states are large).
 #pragma once
 #include "common.cuh"
@@ -63,7 +63,7 @@ template <int BLOCK_KEYS> FXB_DEV Row row_of(const Params& a, int b) {
   r.n = min(max(n_in, 0), a.T);
   if (r.len != len_in || r.n != n_in) atomicOr(a.err, FXB_DERR_PAGES);
   if (r.n == 0) r.len = 0;  // nothing to compute: the block of nodes writes zeros
-  r.blocks = (r.len + BLOCK_KEYS - 1) / BLOCK_KEYS + 1;
+  r.blocks = r.len / BLOCK_KEYS + (r.len % BLOCK_KEYS != 0) + 1;
   return r;
 }
 
@@ -90,30 +90,46 @@ template <int THREADS> FXB_DEV int64_t block_scan(int64_t v, int64_t* total) {
   return v;
 }
 
-// position in the sequence of all blocks: block j of item (b, hr), hr = key head * RT + row tile
+// Position in the sequence of all blocks: block j of item (b, hk, rt), and how
+// many of the thread block's share are left, this one among them.
 struct Cursor {
-  int64_t u;
-  int b, hr, j;
+  int left, b, hk, rt, j;
   Row row;
 };
-template <int BLOCK_KEYS> FXB_DEV void next(const Params& a, Cursor& c, int64_t end) {
-  ++c.u;
+template <int BLOCK_KEYS> FXB_DEV void next(const Params& a, Cursor& c) {
+  --c.left;
   if (++c.j < c.row.blocks) return;
   c.j = 0;
-  if (++c.hr < a.Hkv * a.RT) return;
-  c.hr = 0;
+  if (++c.rt < a.RT) return;
+  c.rt = 0;
+  if (++c.hk < a.Hkv) return;
+  c.hk = 0;
   ++c.b;
-  if (c.u < end) c.row = row_of<BLOCK_KEYS>(a, c.b);
+  if (c.left > 0) c.row = row_of<BLOCK_KEYS>(a, c.b);
 }
 
-// This thread block's share [c.u, *end) of all *total blocks, c set to its
-// first one. No share is empty, but for thread blocks beyond the number of blocks.
-FXB_DEV int64_t sharers(int64_t total) { return total < (int64_t)gridDim.x ? total : (int64_t)gridDim.x; }
-FXB_DEV int64_t share_begin(int64_t cta, int64_t total) {
-  const int64_t g = sharers(total);
-  return cta < g ? total * cta / g : total;
-}
-template <int BLOCK_KEYS, int THREADS> FXB_DEV Cursor share(const Params& a, int64_t* end, int64_t* total) {
+// Even shares of `total` blocks: the first total % g thread blocks have one
+// more. No share is empty, but for thread blocks beyond the number of blocks.
+struct Shares {
+  int64_t total, each, more;  // blocks in all, of a share, shares with one more
+  FXB_DEV explicit Shares(int64_t n) : total(n) {
+    const int64_t g = n < (int64_t)gridDim.x ? n : (int64_t)gridDim.x;
+    // (a 64-bit division takes some hundred instructions)
+    each = n >> 32 ? n / g : (int64_t)((uint32_t)n / (uint32_t)g);
+    more = n - each * g;
+  }
+  FXB_DEV int64_t begin(int cta) const {
+    const int64_t u = each * cta + (cta < more ? cta : more);
+    return u < total ? u : total;
+  }
+  FXB_DEV int owner(int64_t u) const {  // the thread block that has block u
+    const int64_t big = more * (each + 1), v = u < big ? u : u - big, d = u < big ? each + 1 : each;
+    const int q = v >> 32 ? (int)(v / d) : (int)((uint32_t)v / (uint32_t)d);
+    return u < big ? q : (int)more + q;
+  }
+};
+// This thread block's share: begins at block *start of all.
+template <int BLOCK_KEYS, int THREADS> FXB_DEV Cursor share(const Params& a, int64_t* start, Shares* shares) {
   __shared__ int s_b;
   __shared__ int64_t s_rest;
   const int per = a.Hkv * a.RT, tid = threadIdx.x;
@@ -125,11 +141,11 @@ template <int BLOCK_KEYS, int THREADS> FXB_DEV Cursor share(const Params& a, int
     incl = block_scan<THREADS>(mine, &all) + n;
     n += all;
   }
+  *shares = Shares(n);
+  const int64_t u = *start = shares->begin(blockIdx.x);
   Cursor c;
-  c.u = share_begin(blockIdx.x, n);
-  *end = share_begin(blockIdx.x + 1, n);
-  *total = n;
-  if (c.u >= *end) return c;
+  c.left = (int)(shares->begin(blockIdx.x + 1) - u);
+  if (c.left == 0) return c;
   if (a.B > THREADS) n = 0;
   for (int b0 = 0; b0 < a.B; b0 += THREADS) {
     const int b = b0 + tid;
@@ -139,21 +155,22 @@ template <int BLOCK_KEYS, int THREADS> FXB_DEV Cursor share(const Params& a, int
       incl = block_scan<THREADS>(mine, &all) + n;
       n += all;
     }
-    if (c.u < incl && c.u >= incl - mine) {
+    if (u < incl && u >= incl - mine) {
       s_b = b;
-      s_rest = c.u - (incl - mine);
+      s_rest = u - (incl - mine);
     }
-    if (a.B > THREADS && n > c.u) break;
+    if (a.B > THREADS && n > u) break;
   }
   __syncthreads();
   c.b = s_b;
   c.row = row_of<BLOCK_KEYS>(a, c.b);
-  c.hr = (int)(s_rest / c.row.blocks);
-  c.j = (int)(s_rest - (int64_t)c.hr * c.row.blocks);
+  const int64_t rest = s_rest;
+  const int hr = rest >> 32 ? (int)(rest / c.row.blocks) : (int)((uint32_t)rest / (uint32_t)c.row.blocks);
+  c.j = (int)(rest - (int64_t)hr * c.row.blocks);
+  c.hk = hr / a.RT;
+  c.rt = hr - c.hk * a.RT;
   return c;
 }
-// the thread block that owns block u
-FXB_DEV int owner(int64_t u, int64_t total) { return (int)(((u + 1) * sharers(total) - 1) / total); }
 
 // ------------------------------------------------------------------ joining states
 template <typename T, int D>
@@ -184,38 +201,45 @@ template <int ROWS, int D> FXB_DEV float* part_of(const Params& a, int cta, int 
   return a.parts + ((int64_t)cta * 2 + place) * ROWS * (D + 2);
 }
 
-// Joins the parts [lo, hi] of an item (those of thread blocks lo to hi), in
-// the order of the keys: row r of the tile at row0, its quads d4, d4 + step,
-// ... A part costs a trip to L2 whatever is read of it, so four are under way
-// at once.
-template <typename T, int ROWS, int D, int NQ>
-FXB_DEV void join_row(const Params& a, int b, int hk, int row0, int r, int d4, int step, int lo, int hi) {
+// Joins the parts [lo, hi] of an item (those of thread blocks lo to hi), in a
+// fixed order: row r of the tile at row0, its quads d4, d4 + step,
+// ... `slices` lanes, LANES apart, take every slices-th part each and exchange
+// their states (slices a power of two, all lanes of the warp call). A part
+// costs a trip to L2 whatever is read of it, so U are under way at once.
+template <typename T, int ROWS, int D, int NQ, int U>
+FXB_DEV void join_row(const Params& a, int b, int hk, int row0, int r, int d4, int step, int lo, int hi, int slice = 0,
+                      int slices = 1, int lanes = 32) {
   float m = -INFINITY, l = 0.f;
   float4 o[NQ];
 #pragma unroll
   for (int x = 0; x < NQ; ++x) o[x] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
-  for (int k0 = lo; k0 <= hi; k0 += 4) {
-    float mk[4], lk[4];
-    float4 ok[4][NQ];
+  for (int k0 = lo + slice; k0 <= hi; k0 += U * slices) {
+    float mk[U], lk[U];
+    float4 ok[U][NQ];
 #pragma unroll
-    for (int y = 0; y < 4; ++y) {
-      const int k = min(k0 + y, hi);
-      const float* p = part_of<ROWS, D>(a, k, k == lo);
-      mk[y] = k0 + y <= hi ? __ldcg(p + r) : -INFINITY;
-      lk[y] = __ldcg(p + ROWS + r);
+    for (int y = 0; y < U; ++y) {
+      const int k = k0 + y * slices;
+      mk[y] = -INFINITY;
+      if (k <= hi) {
+        const float* p = part_of<ROWS, D>(a, k, k == lo);
+        mk[y] = __ldcg(p + r);
+        lk[y] = __ldcg(p + ROWS + r);
 #pragma unroll
-      for (int x = 0; x < NQ; ++x)
-        ok[y][x] = __ldcg(reinterpret_cast<const float4*>(p + 2 * ROWS) + (d4 + x * step) * ROWS + r);
+        for (int x = 0; x < NQ; ++x)
+          ok[y][x] = __ldcg(reinterpret_cast<const float4*>(p + 2 * ROWS) + (d4 + x * step) * ROWS + r);
+      }
     }
-    const float mn = fmaxf(fmaxf(fmaxf(m, mk[0]), fmaxf(mk[1], mk[2])), mk[3]);
+    float mn = m;
+#pragma unroll
+    for (int y = 0; y < U; ++y) mn = fmaxf(mn, mk[y]);
     const float f = weight(m, mn);
     l *= f;
 #pragma unroll
     for (int x = 0; x < NQ; ++x) o[x] = make_float4(o[x].x * f, o[x].y * f, o[x].z * f, o[x].w * f);
 #pragma unroll
-    for (int y = 0; y < 4; ++y) {
-      if (k0 + y > hi) break;
+    for (int y = 0; y < U; ++y) {
+      if (k0 + y * slices > hi) break;
       const float w = weight(mk[y], mn);
       l = fmaf(w, lk[y], l);
 #pragma unroll
@@ -223,8 +247,24 @@ FXB_DEV void join_row(const Params& a, int b, int hk, int row0, int r, int d4, i
     }
     m = mn;
   }
+  for (int s = 1; s < slices; s <<= 1) {
+    const float m1 = __shfl_xor_sync(0xffffffffu, m, s * lanes), mn = fmaxf(m, m1);
+    const float f = weight(m, mn), f1 = weight(m1, mn);
+    l = l * f + __shfl_xor_sync(0xffffffffu, l, s * lanes) * f1;
 #pragma unroll
-  for (int x = 0; x < NQ; ++x) write_out<T, D>(a, b, hk, row0 + r, (d4 + x * step) * 4, o[x], l);
+    for (int x = 0; x < NQ; ++x) {
+      float4& y = o[x];
+      y.x = y.x * f + __shfl_xor_sync(0xffffffffu, y.x, s * lanes) * f1;
+      y.y = y.y * f + __shfl_xor_sync(0xffffffffu, y.y, s * lanes) * f1;
+      y.z = y.z * f + __shfl_xor_sync(0xffffffffu, y.z, s * lanes) * f1;
+      y.w = y.w * f + __shfl_xor_sync(0xffffffffu, y.w, s * lanes) * f1;
+    }
+    m = mn;
+  }
+  if (slice == 0) {
+#pragma unroll
+    for (int x = 0; x < NQ; ++x) write_out<T, D>(a, b, hk, row0 + r, (d4 + x * step) * 4, o[x], l);
+  }
 }
 
 // ------------------------------------------------------------------ host

@@ -118,10 +118,10 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
   pdl_wait();
   pdl_trigger();  // after the wait: what the joining kernel reads before its own is then complete
 
-  int64_t end, total;
-  Cursor c = share<kBlockKeys, kThreads>(a, &end, &total);
-  const int64_t start = c.u;
-  const int n_tiles = (int)(end > start ? end - start : 0);
+  int64_t start;
+  Shares shares(1);
+  Cursor c = share<kBlockKeys, kThreads>(a, &start, &shares);
+  const int n_tiles = c.left;
   // places in the ring's order of use
   auto k_index = [&](int q) { return q == 0 ? 0 : 2 * q - 1; };
   auto v_index = [&](int q) { return q + 1 < n_tiles ? 2 * q + 2 : 2 * q + 1; };
@@ -142,14 +142,14 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
     // ahead of its use, and the warp waits at the first instruction that needs it
     auto page_of = [&](const Cursor& f) {
       const int slot0 = f.j * kBlockKeys + lane * box_rows;
-      const bool has = f.u < end && f.j < f.row.blocks - 1 && lane < per_tile && slot0 < f.row.len;
+      const bool has = f.left > 0 && f.j < f.row.blocks - 1 && lane < per_tile && slot0 < f.row.len;
       return has ? a.table[f.b * a.table_sb + (slot0 >> a.page_shift)] : 0;
     };
     auto load = [&](const Cursor& f, int pg, const CUtensorMap* ctx, const CUtensorMap* nodes) -> bool {
       const int s = issued % NS;
       if (!mbar_wait_warp(empty(s), ((issued / NS) & 1) ^ 1, a.err, FXB_DERR_ATTN_WAIT)) return false;
       const bool tree = f.j == f.row.blocks - 1;
-      const int hk = f.hr / a.RT;
+      const int hk = f.hk;
       const int pages = tree ? 1 : (min(f.row.len - f.j * kBlockKeys, kBlockKeys) + box_rows - 1) / box_rows;
       if (lane == 0) mbar_expect_tx(full(s), pages * (tree ? kMaxTree : box_rows) * 128 * NBOX);
       __syncwarp();
@@ -181,14 +181,14 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
             mbar_expect_tx(q_full, a.NT * a.G * 128 * NBOX);
 #pragma unroll
             for (int x = 0; x < NBOX; ++x)
-              tma_load_4d(sQ + x * 16384, &tmQ, q_full, x * 64, (f.hr / a.RT) * a.G,
-                          (f.hr % a.RT) * a.NT, f.b);
+              tma_load_4d(sQ + x * 16384, &tmQ, q_full, x * 64, f.hk * a.G,
+                          f.rt * a.NT, f.b);
           }
         }
         const Cursor fk = f;
         const int pk = pg;
         if (q < n_tiles) {
-          next<kBlockKeys>(a, f, end);
+          next<kBlockKeys>(a, f);
           pg = page_of(f);  // used in the next step
         }
 #pragma unroll 1
@@ -236,7 +236,7 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
           if (tree || q + 1 == n_tiles) umma_commit(q_empty);  // the item's last S has read Q
         }
         __syncwarp();
-        next<kBlockKeys>(a, c, end);
+        next<kBlockKeys>(a, c);
       }
     } else {
       constexpr uint32_t IPV = umma_idesc_f16(FMT, 0, 1, kTileRows, D);
@@ -266,7 +266,7 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
           umma_commit(empty(st));
         }
         __syncwarp();
-        next<kBlockKeys>(a, c, end);
+        next<kBlockKeys>(a, c);
       }
     }
     if (elect_one()) umma_commit(final_bar);
@@ -274,9 +274,9 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
   } else if (warp == kWarpStore) {
     // ------------------------------------------------ the nodes' keys and values into the cache
     constexpr int CH = D / 8;
-    for (Cursor f = c; f.u < end; next<kBlockKeys>(a, f, end)) {
-      if (f.j != f.row.blocks - 1 || f.hr % a.RT) continue;
-      const int hk = f.hr / a.RT, n = f.row.n * CH;
+    for (Cursor f = c; f.left > 0; next<kBlockKeys>(a, f)) {
+      if (f.j != f.row.blocks - 1 || f.rt) continue;
+      const int hk = f.hk, n = f.row.n * CH;
 #pragma unroll 1
       for (int i0 = lane; i0 < n; i0 += 32 * 4) {
         uint4 xk[4], xv[4];
@@ -321,10 +321,10 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
     int64_t u_first = 0;
 #pragma unroll 1
     for (int q = 0; q < n_tiles; ++q) {
-      const int hk = c.hr / a.RT, t0 = (c.hr % a.RT) * a.NT, par = q & 1;
+      const int hk = c.hk, t0 = c.rt * a.NT, par = q & 1;
       const bool tree = c.j == c.row.blocks - 1, begins = q == 0 || c.j == 0;
       if (begins) {
-        u_first = c.u - c.j;
+        u_first = start + q - c.j;
         m = -INFINITY;
         l = 0.f;
         const int t = t0 + r / a.G;
@@ -381,6 +381,7 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
           }
           if (odd) atomicExch(&odd_value[item % 3], 1);
           fence_proxy_async_smem();
+          __syncwarp();
         }
         if (!dead) {
           float mv[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -416,6 +417,7 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
         }
         // the place of the probabilities is free once P V of tile q - 2 is complete
         if (q >= 2 && !uwait(pv_done(par), ((q - 2) >> 1) & 1)) ok = false;
+        __syncwarp();
         if (!dead) {
           const float z = m == -INFINITY ? 0.f : m;
           float sum[4] = {0.f, 0.f, 0.f, 0.f};
@@ -441,7 +443,7 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
         mbar_arrive(p_full(par));
       }
       const Cursor cur = c;
-      next<kBlockKeys>(a, c, end);
+      next<kBlockKeys>(a, c);
       if (!tree && q + 1 < n_tiles) continue;
       // ---- the item ends here
       if (ok && !uwait(pv_done(par), (q >> 1) & 1)) ok = false;
@@ -449,48 +451,52 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
       // the next item's flag, last read two items ago (every thread has passed the barrier since); the
       // exchange of sums is written again two items on, likewise
       if (threadIdx.x == 0) odd_value[(item + 1) % 3] = 0;
+      __syncwarp();
       named_bar_sync(1, kSoftmax);
       const bool begun = u_first >= start, whole = begun && tree;
       const float mj = live ? m : -INFINITY, lj = xch.l[item & 1][0][r] + xch.l[item & 1][1][r];
       const int rows = min(a.NT, a.T - t0) * a.G;
       float* part = part_of<kTileRows, D>(a, blockIdx.x, begun);
+      // Accesses to tensor memory are collective: all of them here, where the warp is together, and none below,
+      // where lanes without a row part from the others
       tc_fence_after();
-#pragma unroll 1
-      for (int i = 0; i < D / 2 / 16; ++i) {
-        uint32_t ov[16];
-        tmem_ld16(tO + i * 16, ov);
-        tmem_wait_ld();
-        if (r < rows && ok) {
-          const int d0 = g * (D / 2) + i * 16;
-          float o[16];
+      uint32_t ov[D / 2];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) o[e] = live ? __uint_as_float(ov[e]) : 0.f;
-          if (tree && odd_value[item % 3])
-            for (int j = 0; j < cur.row.n; ++j)
-              if ((see >> j) & 1)
-                for (int e = 0; e < 16; ++e) {
-                  const float y = to_f<T>(static_cast<const T*>(new_v)[cur.b * v_sb + j * v_st + hk * v_sh + d0 + e]);
-                  if (!(fabsf(y) < INFINITY)) o[e] += y;
-                }
-#pragma unroll
-          for (int e = 0; e < 16; e += 4) {
-            const float4 o4 = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-            const int d = d0 + e;
-            if (whole) write_out<T, D>(a, cur.b, hk, t0 * a.G + r, d, o4, lj);
-            else reinterpret_cast<float4*>(part + 2 * kTileRows)[(d / 4) * kTileRows + r] = o4;
-          }
-        }
-      }
+      for (int i = 0; i < D / 2; i += 16) tmem_ld16(tO + i, ov + i);
+      tmem_wait_ld();
       tc_fence_before();
       mbar_arrive(o_free);
+      if (r < rows && ok) {
+        float o[D / 2];
+#pragma unroll
+        for (int e = 0; e < D / 2; ++e) o[e] = live ? __uint_as_float(ov[e]) : 0.f;
+        if (tree && odd_value[item % 3])
+#pragma unroll 1
+          for (int j = 0; j < cur.row.n; ++j)
+            if ((see >> j) & 1)
+#pragma unroll
+              for (int e = 0; e < D / 2; ++e) {
+                const float y =
+                    to_f<T>(static_cast<const T*>(new_v)[cur.b * v_sb + j * v_st + hk * v_sh + g * (D / 2) + e]);
+                if (!(fabsf(y) < INFINITY)) o[e] += y;
+              }
+#pragma unroll
+        for (int e = 0; e < D / 2; e += 4) {
+          const float4 o4 = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          const int d = g * (D / 2) + e;
+          if (whole) write_out<T, D>(a, cur.b, hk, t0 * a.G + r, d, o4, lj);
+          else reinterpret_cast<float4*>(part + 2 * kTileRows)[(d / 4) * kTileRows + r] = o4;
+        }
+      }
       if (!whole && g == 0 && r < rows) {
         part[r] = mj;
         part[kTileRows + r] = lj;
       }
       if (begun && threadIdx.x == 0)
-        a.owners[(int64_t)cur.b * a.Hkv * a.RT + cur.hr] =
-            make_int2(blockIdx.x, owner(u_first + cur.row.blocks - 1, total));
+        a.owners[((int64_t)cur.b * a.Hkv + cur.hk) * a.RT + cur.rt] =
+            make_int2(blockIdx.x, shares.owner(u_first + cur.row.blocks - 1));
       ++item;
+      __syncwarp();
     }
   }
 
@@ -516,7 +522,7 @@ __global__ void __launch_bounds__(kJoinThreads) tree_attn_join(const Params a) {
   const int r = blockIdx.y * 32 + (threadIdx.x & 31), warp = threadIdx.x >> 5;
   if (r >= min(a.NT, a.T - t0) * a.G) return;
   constexpr int kStep = kJoinThreads / 32;
-  join_row<T, kTileRows, D, D / 4 / kStep>(a, b, hk, t0 * a.G, r, warp, kStep, own.x, own.y);
+  join_row<T, kTileRows, D, D / 4 / kStep, 4>(a, b, hk, t0 * a.G, r, warp, kStep, own.x, own.y);
 }
 
 template <typename T> constexpr CUtensorMapDataType map_type() {
