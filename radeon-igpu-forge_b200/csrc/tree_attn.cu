@@ -390,6 +390,7 @@ tree_attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
   int64_t start;
   Shares shares(1);
   Cursor c = share<kBlockKeys, kThreads>(a, &start, &shares);
+  idle_rows<T, D, kThreads>(a);
   if (c.left == 0) return;
   Cursor f = c;          // the next block to fetch
   int f_stage = 0;       // and its stage

@@ -52,7 +52,7 @@ struct Params {
 };
 
 // ------------------------------------------------------------------ division of the work
-struct Row {  // a batch row
+struct Row {  // a batch row; one without nodes has no blocks (its zeros are written apart)
   int len, n, blocks;
 };
 template <int BLOCK_KEYS> FXB_DEV Row row_of(const Params& a, int b) {
@@ -62,8 +62,7 @@ template <int BLOCK_KEYS> FXB_DEV Row row_of(const Params& a, int b) {
   r.len = len_in < 0 ? 0 : (len_in > most ? (int)most : len_in);
   r.n = min(max(n_in, 0), a.T);
   if (r.len != len_in || r.n != n_in) atomicOr(a.err, FXB_DERR_PAGES);
-  if (r.n == 0) r.len = 0;  // nothing to compute: the block of nodes writes zeros
-  r.blocks = r.len / BLOCK_KEYS + (r.len % BLOCK_KEYS != 0) + 1;
+  r.blocks = r.n ? r.len / BLOCK_KEYS + (r.len % BLOCK_KEYS != 0) + 1 : 0;
   return r;
 }
 
@@ -104,8 +103,9 @@ template <int BLOCK_KEYS> FXB_DEV void next(const Params& a, Cursor& c) {
   c.rt = 0;
   if (++c.hk < a.Hkv) return;
   c.hk = 0;
-  ++c.b;
-  if (c.left > 0) c.row = row_of<BLOCK_KEYS>(a, c.b);
+  if (c.left > 0) do
+      c.row = row_of<BLOCK_KEYS>(a, ++c.b);
+    while (c.row.blocks == 0);
 }
 
 // Even shares of `total` blocks: the first total % g thread blocks have one
@@ -113,7 +113,7 @@ template <int BLOCK_KEYS> FXB_DEV void next(const Params& a, Cursor& c) {
 struct Shares {
   int64_t total, each, more;  // blocks in all, of a share, shares with one more
   FXB_DEV explicit Shares(int64_t n) : total(n) {
-    const int64_t g = n < (int64_t)gridDim.x ? n : (int64_t)gridDim.x;
+    const int64_t g = n < 1 ? 1 : (n < (int64_t)gridDim.x ? n : (int64_t)gridDim.x);
     // (a 64-bit division takes some hundred instructions)
     each = n >> 32 ? n / g : (int64_t)((uint32_t)n / (uint32_t)g);
     more = n - each * g;
@@ -170,6 +170,20 @@ template <int BLOCK_KEYS, int THREADS> FXB_DEV Cursor share(const Params& a, int
   c.hk = hr / a.RT;
   c.rt = hr - c.hk * a.RT;
   return c;
+}
+
+// Zeros for the batch rows without nodes, dealt out to the thread blocks.
+template <typename T, int D, int THREADS> FXB_DEV void idle_rows(const Params& a) {
+  constexpr int kPer = 16 / sizeof(T);
+  for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
+    if (a.n_nodes[b] > 0) continue;
+    const int n = a.T * a.Hq * (D / kPer);
+    for (int i = threadIdx.x; i < n; i += THREADS) {
+      const int d = i % (D / kPer), x = i / (D / kPer), t = x / a.Hq, h = x - t * a.Hq;
+      *reinterpret_cast<uint4*>(static_cast<T*>(a.o) + b * a.o_sb + t * a.o_st + h * a.o_sh + d * kPer) =
+          make_uint4(0, 0, 0, 0);
+    }
+  }
 }
 
 // ------------------------------------------------------------------ joining states

@@ -121,6 +121,7 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
   int64_t start;
   Shares shares(1);
   Cursor c = share<kBlockKeys, kThreads>(a, &start, &shares);
+  idle_rows<T, D, kThreads>(a);
   const int n_tiles = c.left;
   // places in the ring's order of use
   auto k_index = [&](int q) { return q == 0 ? 0 : 2 * q - 1; };
@@ -515,9 +516,9 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads) tree_attn_join(const Params a) {
   pdl_trigger();
   pdl_wait();
-  const int2 own = a.owners[blockIdx.x];
-  if (own.x == own.y) return;
   const int hr = blockIdx.x % (a.Hkv * a.RT), b = blockIdx.x / (a.Hkv * a.RT);
+  const int2 own = a.owners[blockIdx.x];
+  if (a.n_nodes[b] <= 0 || own.x == own.y) return;  // (no nodes: no owners either)
   const int hk = hr / a.RT, t0 = (hr % a.RT) * a.NT;
   const int r = blockIdx.y * 32 + (threadIdx.x & 31), warp = threadIdx.x >> 5;
   if (r >= min(a.NT, a.T - t0) * a.G) return;

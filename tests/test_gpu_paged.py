@@ -710,3 +710,20 @@ def test_page_calls_in_a_graph(dev):
         from fxlm import kv_reserve
         kv_reserve(c["table"], c["n_pages"], c["lens"], c["ref"], room, 16)
         want.commit(None, None, room.tolist())
+
+
+@pytest.mark.parametrize("T,Hq,Hkv", [(2, 4, 2), (20, 2, 2)])
+def test_attention_many_batch_rows(dev, T, Hq, Hkv):
+    # more batch rows than a thread block has threads, most of them short, a third without nodes,
+    # runs of idle rows at both ends; then no row with a node at all
+    rng = np.random.RandomState(T)
+    B = 450
+    n = [0 if b < 9 or b > B - 12 or rng.rand() < 0.3 else int(rng.randint(1, T + 1)) for b in range(B)]
+    lens = [int(rng.choice([0, 1, 20, 130, 300])) for _ in range(B)]
+    a = make(dev, BF16, B, T, Hq, Hkv, 64, lens, 32, seed=T, n_nodes=n)
+    o = check(a)
+    for b in range(B):
+        assert not o[b, n[b]:].any()
+    from fxlm import tree_attention
+    a["n_nodes"].zero_()
+    assert not tree_attention(**a).any()
