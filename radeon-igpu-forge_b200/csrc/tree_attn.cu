@@ -388,9 +388,10 @@ tree_attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
   pdl_wait();
 
   int64_t start;
-  Shares shares(1);
-  Cursor c = share<kBlockKeys, kThreads>(a, &start, &shares);
-  idle_rows<T, D, kThreads>(a);
+  Shares shares;
+  const int nodes = (int)blockIdx.x < a.B ? a.n_nodes[blockIdx.x] : 1;
+  Cursor c = share<kBlockKeys, kThreads, true>(a, &start, &shares);
+  idle_rows<T, D, kThreads>(a, nodes);
   if (c.left == 0) return;
   Cursor f = c;          // the next block to fetch
   int f_stage = 0;       // and its stage
@@ -491,7 +492,6 @@ tree_attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       rows.end(reinterpret_cast<float*>(slot), sm[warp], sl[warp]);
       __syncthreads();
       const bool begun = u_begin >= start;  // this block has the item's first keys
-      const int64_t u_last = u_begin + cur.row.blocks - 1;
       const bool whole = begun && tree;
       float* part = part_of<kRows, D>(a, blockIdx.x, begun);
       for (int i = threadIdx.x; i < kRows * (D / 4); i += kThreads) {
@@ -519,7 +519,8 @@ tree_attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         }
       }
       if (!whole) {  // the last thread block to arrive joins the parts
-        const int lo = shares.owner(u_begin), hi = shares.owner(u_last);
+        const int2 own = shares.owners(u_begin, cur.row.blocks);
+        const int lo = own.x, hi = own.y;
         __syncthreads();
         if (threadIdx.x == 0) {
           __threadfence();  // after the barrier: for the whole block's writes

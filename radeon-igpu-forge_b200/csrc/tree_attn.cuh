@@ -10,8 +10,8 @@
 // Work. An item is (batch row, key head, row tile): the R = T * G query rows
 // of a key head (G query heads share it; row r is node r / G, head r % G),
 // cut into tiles of rows. An item's keys are its context in blocks of
-// BLOCK_KEYS slots and one block of nodes. All items' blocks in a row are
-// divided evenly over the thread blocks, so uneven lengths cost nothing; an
+// BLOCK_KEYS slots and one block of nodes. The blocks are shared out evenly
+// over the thread blocks, whatever the sequences' lengths (see Shares); an
 // item that several thread blocks share is joined from their states in the
 // workspace, in a fixed order: by the thread block that finishes last
 // (few rows), or by a second kernel (many rows, whose states are large).
@@ -108,15 +108,24 @@ template <int BLOCK_KEYS> FXB_DEV void next(const Params& a, Cursor& c) {
     while (c.row.blocks == 0);
 }
 
-// Even shares of `total` blocks: the first total % g thread blocks have one
-// more. No share is empty, but for thread blocks beyond the number of blocks.
+// How the blocks are shared out. Even: the sequence of all blocks is cut into
+// equal shares, the first `more` of them one block longer; a share may end one
+// item and begin the next. Whole: every item is cut into `pieces` equal parts
+// by itself, a thread block each, so that no thread block has two parts to hand
+// over (about 2.5 us each); taken where items are few, shares longer than two
+// blocks, and the longest part not much longer than an even share (8 rows of
+// 16 nodes at 1008 slots: 18.2 -> 15.5 us). WHOLE: the kernel for few rows; the
+// other joins its states in a kernel of its own and gains nothing.
 struct Shares {
-  int64_t total, each, more;  // blocks in all, of a share, shares with one more
-  FXB_DEV explicit Shares(int64_t n) : total(n) {
+  int64_t total, each, more;  // even: blocks in all, of a share, shares with one more
+  int first, pieces;          // whole: the item's thread blocks (pieces > 0)
+  FXB_DEV void even(int64_t n) {
+    total = n;
     const int64_t g = n < 1 ? 1 : (n < (int64_t)gridDim.x ? n : (int64_t)gridDim.x);
     // (a 64-bit division takes some hundred instructions)
     each = n >> 32 ? n / g : (int64_t)((uint32_t)n / (uint32_t)g);
     more = n - each * g;
+    pieces = 0;
   }
   FXB_DEV int64_t begin(int cta) const {
     const int64_t u = each * cta + (cta < more ? cta : more);
@@ -127,24 +136,47 @@ struct Shares {
     const int q = v >> 32 ? (int)(v / d) : (int)((uint32_t)v / (uint32_t)d);
     return u < big ? q : (int)more + q;
   }
+  // the thread blocks of the item whose first block is u and that has n blocks
+  FXB_DEV int2 owners(int64_t u, int n) const {
+    return pieces ? make_int2(first, first + pieces - 1) : make_int2(owner(u), owner(u + n - 1));
+  }
 };
-// This thread block's share: begins at block *start of all.
-template <int BLOCK_KEYS, int THREADS> FXB_DEV Cursor share(const Params& a, int64_t* start, Shares* shares) {
+// This thread block's share. Its first block has number *start: in all (even),
+// or in its item (whole).
+template <int BLOCK_KEYS, int THREADS, bool WHOLE> FXB_DEV Cursor share(const Params& a, int64_t* start, Shares* shares) {
   __shared__ int s_b;
   __shared__ int64_t s_rest;
-  const int per = a.Hkv * a.RT, tid = threadIdx.x;
+  const int per = a.Hkv * a.RT, tid = threadIdx.x, G = gridDim.x;
   int64_t n = 0, mine = 0, incl = 0;
+  int blocks = 0;
   for (int b0 = 0; b0 < a.B; b0 += THREADS) {
     const int b = b0 + tid;
-    mine = b < a.B ? (int64_t)row_of<BLOCK_KEYS>(a, b).blocks * per : 0;
+    blocks = b < a.B ? row_of<BLOCK_KEYS>(a, b).blocks : 0;
+    mine = (int64_t)blocks * per;
     int64_t all;
     incl = block_scan<THREADS>(mine, &all) + n;
     n += all;
   }
-  *shares = Shares(n);
-  const int64_t u = *start = shares->begin(blockIdx.x);
+  shares->even(n);
+  int64_t u = *start = shares->begin(blockIdx.x);
   Cursor c;
   c.left = (int)(shares->begin(blockIdx.x + 1) - u);
+  int part = 0;  // whole: the longest part that is allowed
+  const int least = (int)shares->each + (shares->more != 0);
+  if (WHOLE && a.B <= THREADS && (int64_t)a.B * per <= G / 2 && least > 2) {
+    for (int more = 0; more <= 4 && !part; more = more ? 2 * more : 1) {
+      const int q = least + more, cuts = (blocks + q - 1) / q;
+      int64_t all;
+      const int64_t x = block_scan<THREADS>((int64_t)cuts * per, &all);
+      if (all <= G) {
+        part = q;
+        mine = (int64_t)cuts * per;
+        incl = x;
+        u = blockIdx.x;
+        c.left = u < all;
+      }
+    }
+  }
   if (c.left == 0) return c;
   if (a.B > THREADS) n = 0;
   for (int b0 = 0; b0 < a.B; b0 += THREADS) {
@@ -165,18 +197,28 @@ template <int BLOCK_KEYS, int THREADS> FXB_DEV Cursor share(const Params& a, int
   c.b = s_b;
   c.row = row_of<BLOCK_KEYS>(a, c.b);
   const int64_t rest = s_rest;
-  const int hr = rest >> 32 ? (int)(rest / c.row.blocks) : (int)((uint32_t)rest / (uint32_t)c.row.blocks);
-  c.j = (int)(rest - (int64_t)hr * c.row.blocks);
+  const int unit = part ? (c.row.blocks + part - 1) / part : c.row.blocks;  // of an item, in what u counts
+  const int hr = rest >> 32 ? (int)(rest / unit) : (int)((uint32_t)rest / (uint32_t)unit);
+  c.j = (int)(rest - (int64_t)hr * unit);
+  if (part) {
+    const int k = c.j;
+    shares->first = blockIdx.x - k;
+    shares->pieces = unit;
+    c.j = (int)((int64_t)c.row.blocks * k / unit);
+    c.left = (int)((int64_t)c.row.blocks * (k + 1) / unit) - c.j;
+    *start = c.j;
+  }
   c.hk = hr / a.RT;
   c.rt = hr - c.hk * a.RT;
   return c;
 }
 
 // Zeros for the batch rows without nodes, dealt out to the thread blocks.
-template <typename T, int D, int THREADS> FXB_DEV void idle_rows(const Params& a) {
+// `nodes`: those of the first such row, read ahead.
+template <typename T, int D, int THREADS> FXB_DEV void idle_rows(const Params& a, int nodes) {
   constexpr int kPer = 16 / sizeof(T);
   for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
-    if (a.n_nodes[b] > 0) continue;
+    if ((b == (int)blockIdx.x ? nodes : a.n_nodes[b]) > 0) continue;
     const int n = a.T * a.Hq * (D / kPer);
     for (int i = threadIdx.x; i < n; i += THREADS) {
       const int d = i % (D / kPer), x = i / (D / kPer), t = x / a.Hq, h = x - t * a.Hq;

@@ -119,9 +119,10 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
   pdl_trigger();  // after the wait: what the joining kernel reads before its own is then complete
 
   int64_t start;
-  Shares shares(1);
-  Cursor c = share<kBlockKeys, kThreads>(a, &start, &shares);
-  idle_rows<T, D, kThreads>(a);
+  Shares shares;
+  const int nodes = (int)blockIdx.x < a.B ? a.n_nodes[blockIdx.x] : 1;
+  Cursor c = share<kBlockKeys, kThreads, false>(a, &start, &shares);
+  idle_rows<T, D, kThreads>(a, nodes);
   const int n_tiles = c.left;
   // places in the ring's order of use
   auto k_index = [&](int q) { return q == 0 ? 0 : 2 * q - 1; };
@@ -495,7 +496,7 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
       }
       if (begun && threadIdx.x == 0)
         a.owners[((int64_t)cur.b * a.Hkv + cur.hk) * a.RT + cur.rt] =
-            make_int2(blockIdx.x, shares.owner(u_first + cur.row.blocks - 1));
+            shares.owners(u_first, cur.row.blocks);
       ++item;
       __syncwarp();
     }
