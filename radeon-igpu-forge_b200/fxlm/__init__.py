@@ -28,6 +28,10 @@ __all__ = [
     "kv_reserve",
     "kv_fork",
     "verify_tree",
+    "PagedKVCache",
+    "DecodeStep",
+    "tree_logits",
+    "generate_cached",
 ]
 
 
@@ -63,4 +67,7 @@ def __getattr__(name):
     if name == "verify_tree":
         from . import speculate as _m
         return globals().setdefault(name, _m.verify_tree)
+    if name in ("PagedKVCache", "DecodeStep", "tree_logits", "generate_cached"):
+        from . import decode as _m
+        return getattr(_m, name)
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

@@ -68,13 +68,14 @@ def tree_masks(parents):
     B, T = parents.shape
     if T > MAX_NODES:
         raise ValueError(f"T={T}: at most {MAX_NODES} nodes")
-    par = parents.long()
-    mask = torch.zeros(B, T, dtype=torch.int64, device=parents.device)
-    for c in range(T):
-        up = mask.gather(1, par[:, c:c + 1].clamp(min=0))[:, 0] if c else 0
-        own = 1 << c if c < 63 else -(1 << 63)
-        mask[:, c] = torch.where(par[:, c] >= 0, up, 0) | own
-    return mask
+    up = parents.long()
+    mask = torch.ones((), dtype=torch.int64, device=parents.device) << torch.arange(T, device=parents.device)
+    mask = mask.expand(B, T)
+    for _ in range(max(T - 1, 0).bit_length()):  # doubling: after k steps the 2^k nearest ancestors are in
+        has = up >= 0
+        at = up.clamp(min=0)
+        mask, up = mask | torch.where(has, mask.gather(1, at), 0), torch.where(has, up.gather(1, at), -1)
+    return mask.contiguous()
 
 
 @functools.lru_cache(maxsize=1024)

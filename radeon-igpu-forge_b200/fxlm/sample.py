@@ -10,7 +10,9 @@ checkpoints (`meta.tokenizer == "bytes"`) encode the prompt as UTF-8 bytes
 (an empty prompt starts from "\\n") and decode the output with replacement.
 Additions: `--dtype` (default: the dtype the checkpoint was trained in, fp16
 when it does not say, as the reference's `model.half()`), `--seed`, and for
-other tokenizers `--prompt-ids` / token ids printed on stdout.
+other tokenizers `--prompt-ids` / token ids printed on stdout; `--draft N`
+generates with a KV cache, N drafted tokens a step (0: none; the same
+distribution, fxlm.decode), and `--num-samples K` prints K continuations.
 
     python -m fxlm.sample --ckpt runs/demo/ckpt_last.pt --prompt "def " \\
         --max-new 200 --temperature 0.8 --top-k 50
@@ -74,6 +76,9 @@ def main(argv=None):
     ap.add_argument("--top-k", type=int, default=50)
     ap.add_argument("--dtype", choices=sorted(_DTYPES), default=None)
     ap.add_argument("--seed", type=int, default=None)
+    ap.add_argument("--draft", type=int, default=None,
+                    help="generate with a KV cache and up to this many drafted tokens a step")
+    ap.add_argument("--num-samples", type=int, default=1)
     args = ap.parse_args(argv)
 
     from fxlm.env import setup_lm_env
@@ -103,8 +108,14 @@ def main(argv=None):
     else:
         raise SystemExit(f"tokenizer '{tok}' has no text encoding: give --prompt-ids")
     ids = torch.tensor(raw, dtype=torch.long, device=device)
-    out = generate(model, ids, args.max_new, args.temperature, args.top_k, gen)[0, ids.numel():]
-    text = decode(out)
+    if args.draft is not None:
+        from fxlm.decode import generate_cached
+        outs = generate_cached(model, ids, args.max_new, args.temperature, args.top_k, gen, draft=args.draft,
+                               samples=args.num_samples)
+    else:
+        outs = [generate(model, ids, args.max_new, args.temperature, args.top_k, gen)[0]
+                for _ in range(args.num_samples)]
+    text = "\n".join(decode(out[ids.numel():]) for out in outs)
     sys.stdout.write(text + "\n")
     sys.stdout.flush()
     return text

@@ -161,3 +161,42 @@ def test_tree_masks():
     assert tree_masks(chain)[0, -1].item() == -1 and tree_masks(chain)[0, 62].item() == 2 ** 63 - 1
     with pytest.raises(ValueError):
         tree_masks(torch.zeros(1, 65, dtype=torch.int32))
+
+
+def test_tree_batch_and_masks_agree():
+    from fxlm import tree_masks
+    from fxlm.decode import tree_batch
+    trees = [([5, 6, 7, 8], [-1, 0, 0, 2]), ([], []), (list(range(64)), list(range(-1, 63)))]
+    tok, par, n, mask, depth = tree_batch(trees, "cpu")
+    assert n.tolist() == [4, 0, 64] and tok[0].tolist()[:5] == [5, 6, 7, 8, 0]
+    want = tree_masks(par)
+    assert mask[0, :4].tolist() == want[0, :4].tolist() and mask[2].tolist() == want[2].tolist()
+    assert depth[0, :4].tolist() == [0, 1, 1, 2] and depth[2].tolist() == list(range(64))
+
+
+def test_draft_from_text():
+    from fxlm.decode import draft_from_text
+    # the last three tokens occurred twice: both continuations, common beginning merged
+    seq = [1, 2, 3, 9, 8, 7, 1, 2, 3, 9, 5, 1, 2, 3]
+    tok, par = draft_from_text(seq, 7)
+    assert tok[0] == 3 and tok.count(9) == 1 and par[0] == -1 and all(0 <= p < c for c, p in enumerate(par) if c)
+    paths = set()
+    for c in range(len(tok)):
+        p, x = [], c
+        while x > 0:
+            p.insert(0, tok[x])
+            x = par[x]
+        paths.add(tuple(p))
+    assert (9, 5, 1) in paths and (9, 8, 7) in paths
+    assert draft_from_text([4], 5) == ([4], [-1])
+    assert draft_from_text([4, 5, 6], 5) == ([6], [-1])          # nothing to repeat
+    assert draft_from_text(seq, 1) == ([3], [-1])
+    assert len(draft_from_text([7] * 200, 64)[0]) <= 64
+
+
+def test_next_probs():
+    from fxlm.decode import next_probs
+    x = torch.tensor([[1.0, 3.0, 3.0, 2.0, -1.0]])
+    p = next_probs(x, 0.5, 2)
+    assert p[0, 1] == p[0, 2] == 0.5 and p[0, 0] == p[0, 3] == p[0, 4] == 0
+    assert torch.allclose(next_probs(x, 1.0, 0), torch.softmax(x, -1))
