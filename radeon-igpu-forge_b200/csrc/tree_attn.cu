@@ -357,6 +357,31 @@ struct Rows32 {
   }
 };
 
+// The nodes' keys and values into the cache. Up to 16 nodes leave the first
+// warp to the products: the other three copy.
+template <typename T, int D>
+FXB_DEV void store_nodes(const Params& a, int b, int hk, const Row& row) {
+  constexpr int kPer = 16 / sizeof(T), CH = D / kPer;  // 16-byte pieces of a row
+  const int skip = row.n <= kTile ? 32 : 0, tid = (int)threadIdx.x - skip;
+  if (tid < 0) return;
+  const T* k = static_cast<const T*>(a.k) + b * a.k_sb + hk * a.k_sh;
+  const T* v = static_cast<const T*>(a.v) + b * a.v_sb + hk * a.v_sh;
+  for (int i = tid; i < row.n * CH; i += kThreads - skip) {
+    const int t = i / CH, d = (i % CH) * kPer;
+    const uint4 xk = *reinterpret_cast<const uint4*>(k + t * a.k_st + d);
+    const uint4 xv = *reinterpret_cast<const uint4*>(v + t * a.v_st + d);
+    const int64_t pos = (int64_t)row.len + t, pi = pos >> a.page_shift;
+    const int pg = pi < a.W ? a.table[b * a.table_sb + pi] : -1;
+    if (pg < 0 || pg >= a.P) {
+      atomicOr(a.err, FXB_DERR_PAGES);
+      continue;
+    }
+    const int64_t off = pos & ((1 << a.page_shift) - 1);
+    *reinterpret_cast<uint4*>(static_cast<T*>(a.kp) + pg * a.kp_sp + hk * a.kp_sh + off * a.kp_st + d) = xk;
+    *reinterpret_cast<uint4*>(static_cast<T*>(a.vp) + pg * a.vp_sp + hk * a.vp_sh + off * a.vp_st + d) = xv;
+  }
+}
+
 template <typename T, int D> struct RowsOf { using type = Rows16<T, D>; };
 template <int D> struct RowsOf<float, D> { using type = Rows32<D>; };
 
@@ -440,12 +465,13 @@ tree_attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       window = front;
     }
   };
+  typename RowsOf<T, D>::type rows;
+  rows.begin(a, c.b, c.hk, c.rt * kRows, c.row.n, sq);  // the loads of Q are under way while the ring fills
   for (int i = 0; i < ST; ++i) fetch();
 
-  typename RowsOf<T, D>::type rows;
   unsigned phase = 0;    // bit s: parity of stage s
-  bool ok = true, fresh = true;
-  int64_t u_begin = 0;   // the item's first block
+  bool ok = true, fresh = false;
+  int64_t u_begin = start - c.j;   // the item's first block
   for (int s = 0, done = 0; c.left; s = s + 1 == ST ? 0 : s + 1, ++done) {
     const int hk = c.hk, row0 = c.rt * kRows;
     uint8_t* slot = ring + s * S::kSlot;
@@ -455,6 +481,7 @@ tree_attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       fresh = false;
     }
     const bool tree = c.j == c.row.blocks - 1;
+    if (tree && row0 == 0) store_nodes<T, D>(a, c.b, hk, c.row);
     if (ok && ((armed >> s) & 1)) {
       ok = mbar_wait_warp(smem_u32(&bars[warp][s]), (phase >> s) & 1, a.err, FXB_DERR_ATTN_WAIT);
       if (ok) {
@@ -462,25 +489,6 @@ tree_attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         phase ^= 1u << s;
         const int at = tree ? in_block : c.j * kBlockKeys + in_block;
         const int valid = min(kTile, (tree ? c.row.n : c.row.len) - at);
-        if (tree && row0 == 0) {  // the nodes' keys and values go into the cache
-          constexpr int CH = D * (int)sizeof(T) / 16;
-          for (int i = lane; i < 2 * kTile * CH; i += 32) {
-            const int kv = i / (kTile * CH), j = (i / CH) % kTile, ch = i % CH;
-            if (j >= valid) continue;
-            const int64_t pos = (int64_t)c.row.len + at + j;
-            const int64_t pi = pos >> a.page_shift;
-            const int dst = pi < a.W ? a.table[c.b * a.table_sb + pi] : -1;
-            if (dst < 0 || dst >= a.P) {
-              atomicOr(a.err, FXB_DERR_PAGES);
-              continue;
-            }
-            const int off = (int)pos & ((1 << a.page_shift) - 1);
-            T* x = kv ? static_cast<T*>(a.vp) + dst * a.vp_sp + hk * a.vp_sh + off * a.vp_st
-                      : static_cast<T*>(a.kp) + dst * a.kp_sp + hk * a.kp_sh + off * a.kp_st;
-            reinterpret_cast<uint4*>(x)[ch] = *reinterpret_cast<const uint4*>(slot + kv * S::kOperand + sw(j, ch));
-          }
-          __syncwarp();
-        }
         rows.tile(a, slot, valid, tree, at, sq, sp);
       }
     }
@@ -662,11 +670,15 @@ int fxb_tree_attn(const fxb_tree_attn_args* a, void* stream) {
   p.W = a->W;
   p.scale_log2 = a->scale * 1.4426950408889634f;
   p.q = a->q;
+  p.k = a->k;
+  p.v = a->v;
   p.o = a->o;
   p.kp = a->k_pages;
   p.vp = a->v_pages;
   p.q_sb = a->q_sb; p.q_st = a->q_st; p.q_sh = a->q_sh;
   p.o_sb = a->o_sb; p.o_st = a->o_st; p.o_sh = a->o_sh;
+  p.k_sb = a->k_sb; p.k_st = a->k_st; p.k_sh = a->k_sh;
+  p.v_sb = a->v_sb; p.v_st = a->v_st; p.v_sh = a->v_sh;
   p.kp_sp = a->kp_sp; p.kp_sh = a->kp_sh; p.kp_st = a->kp_st;
   p.vp_sp = a->vp_sp; p.vp_sh = a->vp_sh; p.vp_st = a->vp_st;
   p.table = a->table;

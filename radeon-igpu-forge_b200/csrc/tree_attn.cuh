@@ -35,9 +35,10 @@ FXB_DEV float ex2(float x) {
 struct Params {
   int B, T, Hq, Hkv, G, R, RT, NT, page_shift, P, W;  // RT row tiles of an item's rows; NT: nodes of one (many rows)
   float scale_log2;
-  const void* q;
+  const void *q, *k, *v;  // k, v: of the nodes
   void *o, *kp, *vp;
   int64_t q_sb, q_st, q_sh, o_sb, o_st, o_sh;
+  int64_t k_sb, k_st, k_sh, v_sb, v_st, v_sh;
   int64_t kp_sp, kp_sh, kp_st, vp_sp, vp_sh, vp_st;
   const int32_t* table;
   int64_t table_sb;
@@ -141,9 +142,70 @@ struct Shares {
     return pieces ? make_int2(first, first + pieces - 1) : make_int2(owner(u), owner(u + n - 1));
   }
 };
+// Up to 32 batch rows: every warp finds the share by itself, a lane a batch
+// row, without a barrier (1.0 us of 1.9 at the start of a call).
+FXB_DEV int64_t warp_scan(int64_t v) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += y;
+  }
+  return v;
+}
+template <int BLOCK_KEYS, bool WHOLE>
+FXB_DEV Cursor share_small(const Params& a, int64_t* start, Shares* shares) {
+  const int per = a.Hkv * a.RT, lane = threadIdx.x & 31, G = gridDim.x;
+  Row row = {0, 0, 0};
+  if (lane < a.B) row = row_of<BLOCK_KEYS>(a, lane);
+  int unit = row.blocks;  // of an item, in what u counts
+  int64_t incl = warp_scan((int64_t)unit * per);
+  shares->even(__shfl_sync(0xffffffffu, incl, 31));
+  int64_t u = *start = shares->begin(blockIdx.x);
+  Cursor c;
+  c.left = (int)(shares->begin(blockIdx.x + 1) - u);
+  int part = 0;
+  const int least = (int)shares->each + (shares->more != 0);
+  if (WHOLE && (int64_t)a.B * per <= G / 2 && least > 2) {
+    for (int more = 0; more <= 4 && !part; more = more ? 2 * more : 1) {
+      const int q = least + more, cuts = (row.blocks + q - 1) / q;
+      const int64_t x = warp_scan((int64_t)cuts * per), all = __shfl_sync(0xffffffffu, x, 31);
+      if (all <= G) {
+        part = q;
+        unit = cuts;
+        incl = x;
+        u = blockIdx.x;
+        c.left = u < all;
+      }
+    }
+  }
+  if (c.left == 0) return c;
+  const int at = __popc(__ballot_sync(0xffffffffu, incl <= u));  // rows that end at or before u
+  c.b = at;
+  c.row.len = __shfl_sync(0xffffffffu, row.len, at);
+  c.row.n = __shfl_sync(0xffffffffu, row.n, at);
+  c.row.blocks = __shfl_sync(0xffffffffu, row.blocks, at);
+  unit = __shfl_sync(0xffffffffu, unit, at);
+  const int64_t rest = u - (__shfl_sync(0xffffffffu, incl, at) - (int64_t)unit * per);
+  const int hr = rest >> 32 ? (int)(rest / unit) : (int)((uint32_t)rest / (uint32_t)unit);
+  c.j = (int)(rest - (int64_t)hr * unit);
+  if (part) {
+    const int k = c.j;
+    shares->first = blockIdx.x - k;
+    shares->pieces = unit;
+    c.j = (int)((int64_t)c.row.blocks * k / unit);
+    c.left = (int)((int64_t)c.row.blocks * (k + 1) / unit) - c.j;
+    *start = c.j;
+  }
+  c.hk = hr / a.RT;
+  c.rt = hr - c.hk * a.RT;
+  return c;
+}
+
 // This thread block's share. Its first block has number *start: in all (even),
 // or in its item (whole).
 template <int BLOCK_KEYS, int THREADS, bool WHOLE> FXB_DEV Cursor share(const Params& a, int64_t* start, Shares* shares) {
+  if (a.B <= 32) return share_small<BLOCK_KEYS, WHOLE>(a, start, shares);
   __shared__ int s_b;
   __shared__ int64_t s_rest;
   const int per = a.Hkv * a.RT, tid = threadIdx.x, G = gridDim.x;

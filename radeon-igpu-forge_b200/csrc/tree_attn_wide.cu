@@ -65,8 +65,7 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
 tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmNK,
-               const __grid_constant__ CUtensorMap tmNV, const void* new_v, int64_t v_sb, int64_t v_st, int64_t v_sh,
-               const void* new_k, int64_t k_sb, int64_t k_st, int64_t k_sh, const Params a) {
+               const __grid_constant__ CUtensorMap tmNV, const Params a) {
   using W = Wide<D>;
   constexpr int NS = W::kSlots, NBOX = W::kBoxes;
   constexpr int FMT = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
@@ -292,9 +291,9 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
             const int pg = pi < a.W ? a.table[f.b * a.table_sb + pi] : -1;
             if (pg < 0 || pg >= a.P) atomicOr(a.err, FXB_DERR_PAGES);
             else to[u] = ((int64_t)pg << a.page_shift) | (pos & ((1 << a.page_shift) - 1));
-            xk[u] = *reinterpret_cast<const uint4*>(static_cast<const T*>(new_k) + f.b * k_sb + t * k_st + hk * k_sh +
+            xk[u] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.k) + f.b * a.k_sb + t * a.k_st + hk * a.k_sh +
                                                     ch * 8);
-            xv[u] = *reinterpret_cast<const uint4*>(static_cast<const T*>(new_v) + f.b * v_sb + t * v_st + hk * v_sh +
+            xv[u] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.v) + f.b * a.v_sb + t * a.v_st + hk * a.v_sh +
                                                     ch * 8);
           }
         }
@@ -479,7 +478,7 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
 #pragma unroll
               for (int e = 0; e < D / 2; ++e) {
                 const float y =
-                    to_f<T>(static_cast<const T*>(new_v)[cur.b * v_sb + j * v_st + hk * v_sh + g * (D / 2) + e]);
+                    to_f<T>(static_cast<const T*>(a.v)[cur.b * a.v_sb + j * a.v_st + hk * a.v_sh + g * (D / 2) + e]);
                 if (!(fabsf(y) < INFINITY)) o[e] += y;
               }
 #pragma unroll
@@ -546,7 +545,7 @@ int launch(const fxb_tree_attn_args* x, Params& a, int grid, void* stream) {
           "fxb_tree_attn"))
     return r;
   fxb::pdl_launch(tree_attn_wide<T, D>, dim3(grid), dim3(kThreads), Wide<D>::kSmem, fxb::as_stream(stream), q, k, v,
-                  nk, nv, x->v, x->v_sb, x->v_st, x->v_sh, x->k, x->k_sb, x->k_st, x->k_sh, a);
+                  nk, nv, a);
   if (int r = fxb::check_launch("fxb_tree_attn")) return r;
   const int chunks = (a.NT * a.G + 31) / 32;
   fxb::pdl_launch(tree_attn_join<T, D>, dim3((unsigned)(a.B * a.Hkv * a.RT), chunks), dim3(kJoinThreads), 0,

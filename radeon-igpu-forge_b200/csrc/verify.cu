@@ -325,9 +325,11 @@ __global__ void __launch_bounds__(kMaxThreads, 2) verify_tree_kernel(const Verif
 }
 
 // Thread blocks of a cluster: one for every 4096 tokens of the vocabulary, at
-// most 8 (a portable cluster). Threads of a block: 512 while every block has
-// an SM to itself (at 50257 tokens 13 elements a thread, all under way at
-// once), else 256, four blocks an SM.
+// most 8 (a portable cluster; 64 rows of 50257: 21.4 us with 8 blocks of 256
+// threads, 27.1 with 4, 36.8 with 2, 55.8 with 1). Threads of a block: 256,
+// four blocks an SM, and a thread's 16 elements of 32768 all under way at once
+// (one row: 4.9 us, 5.6 with 512 threads); 512 for longer slices while every
+// block has an SM to itself.
 int cluster_of(int V) {
   int c = 1;
   while (c < kMaxCluster && V > c * 4096) c *= 2;
@@ -337,7 +339,8 @@ int cluster_of(int V) {
 template <bool DRAFT> int launch(const VerifyParams& a, void* stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.B * a.cluster));
-  cfg.blockDim = dim3((int64_t)a.B * a.cluster <= fxb::num_sms() ? kMaxThreads : kMaxThreads / 2);
+  const bool alone = (int64_t)a.B * a.cluster <= fxb::num_sms();
+  cfg.blockDim = dim3(alone && a.V > a.cluster * kAtOnce * kMaxThreads / 2 ? kMaxThreads : kMaxThreads / 2);
   cfg.stream = fxb::as_stream(stream);
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
