@@ -395,6 +395,7 @@ tree_attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
   __shared__ __align__(8) uint64_t bars[kWarps][ST];
   __shared__ float sm[kWarps][kRows], sl[kWarps][kRows];
   __shared__ int s_last;
+  __shared__ Scratch scratch;
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint8_t* ring = smem + warp * ST * S::kSlot;
@@ -415,7 +416,7 @@ tree_attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
   int64_t start;
   Shares shares;
   const int nodes = (int)blockIdx.x < a.B ? a.n_nodes[blockIdx.x] : 1;
-  Cursor c = share<kBlockKeys, kThreads, true>(a, &start, &shares);
+  Cursor c = share<kBlockKeys, kThreads, true>(a, &start, &shares, scratch);
   idle_rows<T, D, kThreads>(a, nodes);
   if (c.left == 0) return;
   Cursor f = c;          // the next block to fetch

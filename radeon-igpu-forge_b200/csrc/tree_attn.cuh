@@ -67,10 +67,14 @@ template <int BLOCK_KEYS> FXB_DEV Row row_of(const Params& a, int b) {
   return r;
 }
 
+struct Scratch {  // of share(), in shared memory
+  int64_t warp_total[12], rest;
+  int b;
+};
 // inclusive prefix sum over the block's threads; *total for everyone
-template <int THREADS> FXB_DEV int64_t block_scan(int64_t v, int64_t* total) {
+template <int THREADS> FXB_DEV int64_t block_scan(int64_t v, int64_t* total, int64_t* warp_total) {
   constexpr int kWarps = THREADS / 32;
-  __shared__ int64_t warp_total[kWarps];
+  static_assert(kWarps <= 12, "Scratch");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -204,10 +208,8 @@ FXB_DEV Cursor share_small(const Params& a, int64_t* start, Shares* shares) {
 
 // This thread block's share. Its first block has number *start: in all (even),
 // or in its item (whole).
-template <int BLOCK_KEYS, int THREADS, bool WHOLE> FXB_DEV Cursor share(const Params& a, int64_t* start, Shares* shares) {
+template <int BLOCK_KEYS, int THREADS, bool WHOLE> FXB_DEV Cursor share(const Params& a, int64_t* start, Shares* shares, Scratch& s) {
   if (a.B <= 32) return share_small<BLOCK_KEYS, WHOLE>(a, start, shares);
-  __shared__ int s_b;
-  __shared__ int64_t s_rest;
   const int per = a.Hkv * a.RT, tid = threadIdx.x, G = gridDim.x;
   int64_t n = 0, mine = 0, incl = 0;
   int blocks = 0;
@@ -216,7 +218,7 @@ template <int BLOCK_KEYS, int THREADS, bool WHOLE> FXB_DEV Cursor share(const Pa
     blocks = b < a.B ? row_of<BLOCK_KEYS>(a, b).blocks : 0;
     mine = (int64_t)blocks * per;
     int64_t all;
-    incl = block_scan<THREADS>(mine, &all) + n;
+    incl = block_scan<THREADS>(mine, &all, s.warp_total) + n;
     n += all;
   }
   shares->even(n);
@@ -229,7 +231,7 @@ template <int BLOCK_KEYS, int THREADS, bool WHOLE> FXB_DEV Cursor share(const Pa
     for (int more = 0; more <= 4 && !part; more = more ? 2 * more : 1) {
       const int q = least + more, cuts = (blocks + q - 1) / q;
       int64_t all;
-      const int64_t x = block_scan<THREADS>((int64_t)cuts * per, &all);
+      const int64_t x = block_scan<THREADS>((int64_t)cuts * per, &all, s.warp_total);
       if (all <= G) {
         part = q;
         mine = (int64_t)cuts * per;
@@ -246,19 +248,19 @@ template <int BLOCK_KEYS, int THREADS, bool WHOLE> FXB_DEV Cursor share(const Pa
     if (a.B > THREADS) {
       mine = b < a.B ? (int64_t)row_of<BLOCK_KEYS>(a, b).blocks * per : 0;
       int64_t all;
-      incl = block_scan<THREADS>(mine, &all) + n;
+      incl = block_scan<THREADS>(mine, &all, s.warp_total) + n;
       n += all;
     }
     if (u < incl && u >= incl - mine) {
-      s_b = b;
-      s_rest = u - (incl - mine);
+      s.b = b;
+      s.rest = u - (incl - mine);
     }
     if (a.B > THREADS && n > u) break;
   }
   __syncthreads();
-  c.b = s_b;
+  c.b = s.b;
   c.row = row_of<BLOCK_KEYS>(a, c.b);
-  const int64_t rest = s_rest;
+  const int64_t rest = s.rest;
   const int unit = part ? (c.row.blocks + part - 1) / part : c.row.blocks;  // of an item, in what u counts
   const int hr = rest >> 32 ? (int)(rest / unit) : (int)((uint32_t)rest / (uint32_t)unit);
   c.j = (int)(rest - (int64_t)hr * unit);

@@ -16,7 +16,12 @@
 // at 384. Scores are free as soon as they are in registers, so that the tensor
 // cores and the softmax run side by side.
 // Keys and values go through one ring of operands in the order of their use
-// (K0 K1 V0 K2 V1 ...).
+// (K0 K1 V0 K2 V1 ...). A wait tells a phase from the one before it by parity
+// alone, so whoever waits for a slot has to know that its previous use is over.
+// The ring's length is even: a slot is used by keys only or by values only (but
+// for the first keys and the last values), so each of the two issuing warps
+// waits for every use of its slots. With an odd length the warp that issues S
+// took a slot for filled whose older values were still under way.
 #include "tree_attn.cuh"
 
 namespace {
@@ -29,14 +34,15 @@ constexpr int kThreads = 384;
 constexpr int kWarpS = 8, kWarpTma = 9, kWarpStore = 10, kWarpPV = 11;
 constexpr int kSoftmax = 256;  // threads of both groups
 
+constexpr int kSmall = 3072;   // shared memory behind the operands
 template <int D> struct Wide {
   static constexpr int kBoxes = D / 64;
   static constexpr int kOperand = kTileRows * D * 2;  // Q, K or V of a tile: D / 64 blocks of [128 rows][128 bytes]
-  static constexpr int kSlots = D == 128 ? 5 : 11;    // ring of keys and values
-  static constexpr int kSmem = 1024 + (1 + kSlots) * kOperand;
+  static constexpr int kSlots = D == 128 ? 6 : 12;    // ring of keys and values: an even number, see the top
+  static constexpr int kSmem = (1 + kSlots) * kOperand + kSmall;
   static constexpr int kPart = kTileRows * (D + 2);   // floats of a state in the workspace
 };
-static_assert(Wide<128>::kSmem + 5120 <= 232448 && Wide<64>::kSmem + 5120 <= 232448, "shared memory");
+static_assert(Wide<128>::kSmem <= 232448 && Wide<64>::kSmem <= 232448, "shared memory of a block");
 
 // byte offset of 16-byte piece c of row r of an operand (128-byte swizzle)
 FXB_DEV uint32_t sw(int r, int c) { return (c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4); }
@@ -56,10 +62,14 @@ FXB_DEV void tmem_wait_ld32(uint32_t* r) {
                : "memory");
 }
 
-struct Exchange {
-  float m[2][2][kTileRows];  // [tile parity][half]: a row's maximum over half a tile
-  float l[2][2][kTileRows];  // [item parity][half]: its sum over the item
+struct Small {
+  float x[2][2][kTileRows];  // [tile parity][half]: a row's maximum over half a tile; its sum at an item's end
+  uint64_t bars[36];
+  Scratch scratch;
+  int odd_value[3];          // an item's node has a value that is not finite (items in turn)
+  uint32_t tmem_slot;
 };
+static_assert(sizeof(Small) <= kSmall, "shared memory behind the operands");
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -69,15 +79,17 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
   using W = Wide<D>;
   constexpr int NS = W::kSlots, NBOX = W::kBoxes;
   constexpr int FMT = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
-  extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t bars[2 * NS + 12];
-  __shared__ Exchange xch;
-  __shared__ int odd_value[3];  // an item's node has a value that is not finite (items in turn)
-  __shared__ uint32_t tmem_slot;
-  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
-  uint8_t* gbase = smem_raw + (base - raw);
+  // All of it dynamic, so that six operands fit beside Q: it begins on a 1024-byte boundary, as the swizzle needs
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t base = smem_u32(smem_raw);
+  uint8_t* gbase = smem_raw;
+  Small& sm = *reinterpret_cast<Small*>(smem_raw + (1 + NS) * W::kOperand);
+  if (base & 1023) {  // (not met: there is no static shared memory)
+    if (threadIdx.x == 0) atomicOr(a.err, FXB_DERR_ATTN_WAIT);
+    return;
+  }
   const uint32_t sQ = base, sKV = base + W::kOperand;
-  const uint32_t bar0 = smem_u32(bars);
+  const uint32_t bar0 = smem_u32(sm.bars);
   auto full = [&](int s) { return bar0 + 8u * s; };
   auto empty = [&](int s) { return bar0 + 8u * (NS + s); };
   const uint32_t q_full = bar0 + 8u * (2 * NS), q_empty = bar0 + 8u * (2 * NS + 1);
@@ -99,7 +111,7 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
       mbar_init(p_full(i), kSoftmax);
       mbar_init(pv_done(i), 1);
     }
-    odd_value[0] = odd_value[1] = odd_value[2] = 0;
+    sm.odd_value[0] = sm.odd_value[1] = sm.odd_value[2] = 0;
     mbar_init(q_full, 1);
     mbar_init(q_empty, 1);
     mbar_init(o_free, kSoftmax);
@@ -107,20 +119,20 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
     fence_mbar_init();
   }
   if (warp == kWarpS) {
-    tmem_alloc(smem_u32(&tmem_slot), 512);
+    tmem_alloc(smem_u32(&sm.tmem_slot), 512);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tmem_slot;
+  const uint32_t tmem = sm.tmem_slot;
   pdl_wait();
   pdl_trigger();  // after the wait: what the joining kernel reads before its own is then complete
 
   int64_t start;
   Shares shares;
   const int nodes = (int)blockIdx.x < a.B ? a.n_nodes[blockIdx.x] : 1;
-  Cursor c = share<kBlockKeys, kThreads, false>(a, &start, &shares);
+  Cursor c = share<kBlockKeys, kThreads, false>(a, &start, &shares, sm.scratch);
   idle_rows<T, D, kThreads>(a, nodes);
   const int n_tiles = c.left;
   // places in the ring's order of use
@@ -146,11 +158,10 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
       const bool has = f.left > 0 && f.j < f.row.blocks - 1 && lane < per_tile && slot0 < f.row.len;
       return has ? a.table[f.b * a.table_sb + (slot0 >> a.page_shift)] : 0;
     };
-    auto load = [&](const Cursor& f, int pg, const CUtensorMap* ctx, const CUtensorMap* nodes) -> bool {
+    auto load = [&](bool values, const Cursor& f, int pg) -> bool {
       const int s = issued % NS;
       if (!mbar_wait_warp(empty(s), ((issued / NS) & 1) ^ 1, a.err, FXB_DERR_ATTN_WAIT)) return false;
       const bool tree = f.j == f.row.blocks - 1;
-      const int hk = f.hk;
       const int pages = tree ? 1 : (min(f.row.len - f.j * kBlockKeys, kBlockKeys) + box_rows - 1) / box_rows;
       if (lane == 0) mbar_expect_tx(full(s), pages * (tree ? kMaxTree : box_rows) * 128 * NBOX);
       __syncwarp();
@@ -159,11 +170,11 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
           atomicOr(a.err, FXB_DERR_PAGES);
           pg = 0;
         }
+        const CUtensorMap* map = values ? (tree ? &tmNV : &tmV) : (tree ? &tmNK : &tmK);
         const uint32_t dst = sKV + s * W::kOperand + (tree ? 0 : lane * box_rows * 128);
         const int row = tree ? 0 : (f.j * kBlockKeys) & (page - 1);  // 0 unless a page holds several tiles
 #pragma unroll
-        for (int x = 0; x < NBOX; ++x)
-          tma_load_4d(dst + x * 16384, tree ? nodes : ctx, full(s), x * 64, row, hk, tree ? f.b : pg);
+        for (int x = 0; x < NBOX; ++x) tma_load_4d(dst + x * 16384, map, full(s), x * 64, row, f.hk, tree ? f.b : pg);
       }
       ++issued;
       return true;
@@ -194,7 +205,7 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
         }
 #pragma unroll 1
         for (int kv = q < n_tiles ? 0 : 1; kv < (q ? 2 : 1) && ok; ++kv)
-          ok = load(kv ? fv : fk, kv ? pv : pk, kv ? &tmV : &tmK, kv ? &tmNV : &tmNK);
+          ok = load(kv != 0, kv ? fv : fk, kv ? pv : pk);
         fv = fk;
         pv = pk;
       }
@@ -334,13 +345,15 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
         dead = !__any_sync(0xffffffffu, live);
       }
       if (ok && !uwait(s_full(par), (q >> 1) & 1)) ok = false;
+      const int cols = tree ? kMaxTree : kBlockKeys;
+      const int c0 = g * (cols / 2);  // this thread's columns: 64, or 32 of the nodes
+      uint32_t v[64];
+      float mx = -INFINITY;
+      // After an expired wait a warp goes on through the tiles without work, so that every barrier is met.
       if (ok) {
         tc_fence_after();
         const int valid = tree ? c.row.n : min(c.row.len - c.j * kBlockKeys, kBlockKeys);
-        const int cols = tree ? kMaxTree : kBlockKeys;
-        const int c0 = g * (cols / 2);  // this thread's columns: 64, or 32 of the nodes
         const bool some = valid < cols || tree;
-        uint32_t v[64];
         tmem_ld32(tS + par * 128 + c0, v);
         tmem_ld32(tS + par * 128 + min(c0 + 32, 96), v + 32);
         tmem_wait_ld32(v);
@@ -380,7 +393,7 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
               odd |= any;
             }
           }
-          if (odd) atomicExch(&odd_value[item % 3], 1);
+          if (odd) atomicExch(&sm.odd_value[item % 3], 1);
           fence_proxy_async_smem();
           __syncwarp();
         }
@@ -389,10 +402,18 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
 #pragma unroll
           for (int i = 0; i < 32; ++i)
             mv[i & 3] = fmaxf(fmaxf(mv[i & 3], __uint_as_float(v[i])), __uint_as_float(v[32 + i]));
-          float mx = fmaxf(fmaxf(mv[0], mv[1]), fmaxf(mv[2], mv[3]));
-          xch.m[par][g][r] = mx;
-          named_bar_sync(2 + (warp & 3), 64);  // the row's two threads
-          mx = fmaxf(mx, xch.m[par][g ^ 1][r]) * a.scale_log2;
+          mx = fmaxf(fmaxf(mv[0], mv[1]), fmaxf(mv[2], mv[3]));
+          sm.x[par][g][r] = mx;
+        }
+      }
+      if (!dead) {
+        __syncwarp();
+        named_bar_sync(2 + (warp & 3), 64);  // the row's two threads
+      }
+      if (ok) {
+        if (!dead) {
+          // (a row that is no node's holds whatever was in shared memory: it must not ask for a rescaling)
+          mx = live ? fmaxf(mx, sm.x[par][g ^ 1][r]) * a.scale_log2 : -INFINITY;
           // the reference maximum m moves only when a tile exceeds it by more than 2^8: probabilities stay
           // below 2^8, which 16 bits hold as well as [0, 1], and O is rarely rescaled
           if (begins) {
@@ -448,47 +469,62 @@ tree_attn_wide(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
       if (!tree && q + 1 < n_tiles) continue;
       // ---- the item ends here
       if (ok && !uwait(pv_done(par), (q >> 1) & 1)) ok = false;
-      xch.l[item & 1][g][r] = live ? l : 0.f;
-      // the next item's flag, last read two items ago (every thread has passed the barrier since); the
-      // exchange of sums is written again two items on, likewise
-      if (threadIdx.x == 0) odd_value[(item + 1) % 3] = 0;
+      if (!dead) sm.x[par ^ 1][g][r] = live ? l : 0.f;  // (the maxima of tile q - 1 have been read)
+      // the next item's flag, last read two items ago (every thread has passed the barrier since)
+      if (threadIdx.x == 0) sm.odd_value[(item + 1) % 3] = 0;
       __syncwarp();
       named_bar_sync(1, kSoftmax);
       const bool begun = u_first >= start, whole = begun && tree;
-      const float mj = live ? m : -INFINITY, lj = xch.l[item & 1][0][r] + xch.l[item & 1][1][r];
+      const float mj = live ? m : -INFINITY, lj = live ? sm.x[par ^ 1][0][r] + sm.x[par ^ 1][1][r] : 0.f;
+      if (!dead) named_bar_sync(2 + (warp & 3), 64);  // both have read: tile q + 1 writes there
       const int rows = min(a.NT, a.T - t0) * a.G;
       float* part = part_of<kTileRows, D>(a, blockIdx.x, begun);
-      // Accesses to tensor memory are collective: all of them here, where the warp is together, and none below,
-      // where lanes without a row part from the others
+      // 16 columns at a time, rolled (this code runs once an item, out of a cold instruction cache). Accesses to
+      // tensor memory are collective: the warp is brought together before each, and the lanes' own condition is
+      // kept opaque, so that the loop cannot be split by lanes.
+      const int t = (t0 * a.G + r) / a.G, h = hk * a.G + (t0 * a.G + r - t * a.G);
+      T* out = static_cast<T*>(a.o) + cur.b * a.o_sb + t * a.o_st + h * a.o_sh + g * (D / 2);
+      float4* to = reinterpret_cast<float4*>(part + 2 * kTileRows) + g * (D / 8) * kTileRows + r;
+      const float inv = lj > 0.f ? 1.f / lj : (lj == 0.f ? 0.f : lj);  // no visible key: zeros; NaN stays
+      const bool odd = tree && sm.odd_value[item % 3];
+      int mine = r < rows && ok;
       tc_fence_after();
-      uint32_t ov[D / 2];
+#pragma unroll 1
+      for (int i = 0; i < D / 2; i += 16) {
+        asm volatile("" : "+r"(mine));
+        __syncwarp();
+        uint32_t ov[16];
+        tmem_ld16(tO + i, ov);
+        tmem_wait_ld();
+        float o[16];
 #pragma unroll
-      for (int i = 0; i < D / 2; i += 16) tmem_ld16(tO + i, ov + i);
-      tmem_wait_ld();
-      tc_fence_before();
-      mbar_arrive(o_free);
-      if (r < rows && ok) {
-        float o[D / 2];
-#pragma unroll
-        for (int e = 0; e < D / 2; ++e) o[e] = live ? __uint_as_float(ov[e]) : 0.f;
-        if (tree && odd_value[item % 3])
+        for (int e = 0; e < 16; ++e) o[e] = live ? __uint_as_float(ov[e]) : 0.f;
+        if (odd && live)
 #pragma unroll 1
           for (int j = 0; j < cur.row.n; ++j)
             if ((see >> j) & 1)
 #pragma unroll
-              for (int e = 0; e < D / 2; ++e) {
-                const float y =
-                    to_f<T>(static_cast<const T*>(a.v)[cur.b * a.v_sb + j * a.v_st + hk * a.v_sh + g * (D / 2) + e]);
+              for (int e = 0; e < 16; ++e) {
+                const float y = to_f<T>(
+                    static_cast<const T*>(a.v)[cur.b * a.v_sb + j * a.v_st + hk * a.v_sh + g * (D / 2) + i + e]);
                 if (!(fabsf(y) < INFINITY)) o[e] += y;
               }
+        if (mine) {
+          if (whole) {
 #pragma unroll
-        for (int e = 0; e < D / 2; e += 4) {
-          const float4 o4 = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-          const int d = g * (D / 2) + e;
-          if (whole) write_out<T, D>(a, cur.b, hk, t0 * a.G + r, d, o4, lj);
-          else reinterpret_cast<float4*>(part + 2 * kTileRows)[(d / 4) * kTileRows + r] = o4;
+            for (int e = 0; e < 16; ++e) o[e] *= inv;
+            store8<T>(out + i, o);
+            store8<T>(out + i + 8, o + 8);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 16; e += 4)
+              to[(i + e) / 4 * kTileRows] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          }
         }
+        __syncwarp();
       }
+      tc_fence_before();
+      mbar_arrive(o_free);
       if (!whole && g == 0 && r < rows) {
         part[r] = mj;
         part[kTileRows + r] = lj;
