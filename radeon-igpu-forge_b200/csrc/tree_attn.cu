@@ -7,19 +7,18 @@ namespace {
 
 using namespace fxb_tree;
 
-constexpr int kBlockKeys = 64;          // keys of a block
-constexpr int kWarps = 4;               // each takes 16 keys of a block
-constexpr int kThreads = kWarps * 32;
+constexpr int kBlockKeys = 64;          // keys of a block, dealt out to the warps
 constexpr int kRows = 16;               // rows of a tile
-constexpr int kTile = 16;               // keys a warp takes at once
 
-// ------------------------------------------------------------------ few rows: a warp takes 16 keys at once
+// ------------------------------------------------------------------ few rows
 template <typename T, int D> struct Shape {
+  static constexpr int kTile = sizeof(T) == 4 && D == 128 ? 8 : 16;  // keys a warp takes at once
+  static constexpr int kWarps = kBlockKeys / kTile, kThreads = kWarps * 32;
   static constexpr int kBoxCols = 128 / sizeof(T);           // columns of a 128-byte swizzled row
   static constexpr int kBoxes = D / kBoxCols;
   static constexpr int kOperand = kTile * D * sizeof(T);      // one warp's keys (or values)
   static constexpr int kSlot = 2 * kOperand;                  // of one stage; >= 16 rows of O in fp32
-  static constexpr int kStages = sizeof(T) == 4 ? 3 : (D == 128 ? 3 : 6);
+  static constexpr int kStages = sizeof(T) == 4 || D == 128 ? 3 : 6;
   static constexpr int kQPitch = D + 4;                       // fp32: rows of Q in shared memory
   static constexpr int kQBytes = sizeof(T) == 4 ? kRows * kQPitch * 4 : 0;
   static constexpr int kPBytes = sizeof(T) == 4 ? kWarps * (kTile * kRows + kRows) * 4 : 0;
@@ -57,12 +56,15 @@ template <> FXB_DEV void mma16816<__half>(float* c, const uint32_t* a, uint32_t 
 }
 
 // byte offset of 16-byte piece c of row r of an operand in shared memory (128-byte swizzle)
-FXB_DEV uint32_t sw(int r, int c) { return (c >> 3) * (kTile * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4); }
+template <int ROWS> FXB_DEV uint32_t sw(int r, int c) {
+  return (c >> 3) * (ROWS * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+}
 
 // 16-bit types: m16n8k16 products. A lane holds, of rows lane / 4 and lane / 4
 // + 8, two columns of every eight.
 template <typename T, int D>
 struct Rows16 {
+  static constexpr int kHeld = kRows, kTile = Shape<T, D>::kTile;
   uint32_t q[D / 16][4];
   float o[D / 8][4];
   float m[2], l[2];
@@ -101,7 +103,7 @@ struct Rows16 {
 #pragma unroll
     for (int k = 0; k < D / 16; ++k) {
       uint32_t f[4];
-      ldmatrix4(sk + sw((lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)), f);
+      ldmatrix4(sk + sw<kTile>((lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)), f);
       mma16816<T>(k & 1 ? s1[0] : s[0], q[k], f[0], f[1]);
       mma16816<T>(k & 1 ? s1[1] : s[1], q[k], f[2], f[3]);
     }
@@ -164,7 +166,7 @@ struct Rows16 {
       bool odd = false;
       for (int i = lane; i < kTile * (D / 8); i += 32) {
         const int r = i / (D / 8), c = i - r * (D / 8);
-        uint4* x = reinterpret_cast<uint4*>(vs + sw(r, c));
+        uint4* x = reinterpret_cast<uint4*>(vs + sw<kTile>(r, c));
         if (r >= valid) {
           *x = make_uint4(0, 0, 0, 0);
         } else if (tree) {
@@ -179,7 +181,7 @@ struct Rows16 {
         for (int j = 0; j < valid; ++j)
 #pragma unroll
           for (int i = 0; i < D / 8; ++i) {
-            const float2 f = unpack2<T>(*reinterpret_cast<const uint32_t*>(vs + sw(j, i) + 4 * (lane & 3)));
+            const float2 f = unpack2<T>(*reinterpret_cast<const uint32_t*>(vs + sw<kTile>(j, i) + 4 * (lane & 3)));
 #pragma unroll
             for (int h = 0; h < 2; ++h)
               if ((see[h] >> (node0 + j)) & 1) {
@@ -189,7 +191,7 @@ struct Rows16 {
           }
         __syncwarp();
         for (int i = lane; i < valid * D; i += 32) {
-          T* x = reinterpret_cast<T*>(vs + sw(i / D, (i % D) / 8)) + i % 8;
+          T* x = reinterpret_cast<T*>(vs + sw<kTile>(i / D, (i % D) / 8)) + i % 8;
           if (!(fabsf(to_f<T>(*x)) < INFINITY)) *x = from_f<T>(0.f);
         }
       }
@@ -199,7 +201,7 @@ struct Rows16 {
 #pragma unroll
     for (int c = 0; c < D / 16; ++c) {
       uint32_t f[4];
-      ldmatrix4t(sv + sw((lane & 7) + (((lane >> 3) & 1) << 3), 2 * c + (lane >> 4)), f);
+      ldmatrix4t(sv + sw<kTile>((lane & 7) + (((lane >> 3) & 1) << 3), 2 * c + (lane >> 4)), f);
       mma16816<T>(o[2 * c], p, f[0], f[1]);
       mma16816<T>(o[2 * c + 1], p, f[2], f[3]);
     }
@@ -223,20 +225,42 @@ struct Rows16 {
   }
 };
 
-// fp32: FMA. For the scores a lane holds rows 4 (lane / 8) .. + 3 and keys
-// lane % 8 and + 8; for O all 16 rows and D / 32 columns.
-template <int D>
+// fp32: FMA, two at once (fma.rn.f32x2). A warp holds the first N rows of a
+// tile. The scores, summed in parts of D, lie four rows and every eighth key
+// to a lane (with N < 16 in kSplit copies). For O a lane has all N rows, two
+// to a register pair, and D / 32 columns.
+FXB_DEV uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+FXB_DEV uint64_t pair_of(float x, float y) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(x), "f"(y));
+  return d;
+}
+FXB_DEV float2 halves(uint64_t x) {
+  float2 d;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(x));
+  return d;
+}
+template <int D, int N>
 struct Rows32 {
-  static constexpr int C = D / 32;
-  float o[kRows][C];
+  static constexpr int kHeld = N, kTile = Shape<float, D>::kTile;
+  static constexpr int C = D / 32, kKeys = kTile / 8, kGroups = N / 4, kSplit = 4 / kGroups;
+  uint64_t o[N / 2][C];
   float m[4], l[4];
   uint64_t see[4];
   bool live[4];
 
+  FXB_DEV static int group() { return (threadIdx.x & 31) / 8 % kGroups; }
+  FXB_DEV static int split() { return (threadIdx.x & 31) / 8 / kGroups; }
+  // Probabilities lie by key, pieces of four rows exchanged by key: a lane's stores then fall into different banks
+  FXB_DEV static float* p_at(float* sp, int j, int r) { return sp + j * N + ((r / 4) ^ (j / (32 / N) & (N / 4 - 1))) * 4; }
+
   FXB_DEV void begin(const Params& a, int b, int hk, int row0, int n, float* sq) {
-    const int lane = threadIdx.x & 31;
     __syncthreads();  // the previous item's Q has been read
-    for (int i = threadIdx.x; i < kRows * (D / 4); i += kThreads) {
+    for (int i = threadIdx.x; i < N * (D / 4); i += Shape<float, D>::kThreads) {
       const int rr = i / (D / 4), d = (i - rr * (D / 4)) * 4, r = row0 + rr, t = r / a.G;
       float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
       if (r < a.R && t < n)
@@ -246,45 +270,95 @@ struct Rows32 {
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int r = row0 + (lane >> 3) * 4 + i, t = r / a.G;
+      const int r = row0 + group() * 4 + i, t = r / a.G;
       live[i] = r < a.R && t < n;
       see[i] = live[i] ? (uint64_t)a.mask[b * a.mask_sb + t] : 0;
       m[i] = -INFINITY;
       l[i] = 0.f;
     }
 #pragma unroll
-    for (int r = 0; r < kRows; ++r)
+    for (int r = 0; r < N / 2; ++r)
 #pragma unroll
-      for (int c = 0; c < C; ++c) o[r][c] = 0.f;
+      for (int c = 0; c < C; ++c) o[r][c] = 0;
     __syncthreads();
   }
 
   FXB_DEV void tile(const Params& a, uint8_t* slot, int valid, bool tree, int node0, const float* sq, float* sp) {
-    const int lane = threadIdx.x & 31, rg = (lane >> 3) * 4, kg = lane & 7;
+    const int lane = threadIdx.x & 31, rg = group() * 4, kg = lane & 7;
     const uint8_t* vs = slot + Shape<float, D>::kOperand;
-    float s[4][2] = {};
+    float s[4][kKeys];
+    if constexpr (kKeys == 2) {  // four rows x keys kg and kg + 8 x every kSplit-th piece of D
+      uint64_t acc[4][2] = {};
 #pragma unroll 4
-    for (int c = 0; c < D / 4; ++c) {
-      const float4 k0 = *reinterpret_cast<const float4*>(slot + sw(kg, c));
-      const float4 k1 = *reinterpret_cast<const float4*>(slot + sw(kg + 8, c));
+      for (int x = 0; x < D / 4 / kSplit; ++x) {
+        const int c = x * kSplit + split();
+        const ulonglong2 k0 = *reinterpret_cast<const ulonglong2*>(slot + sw<kTile>(kg, c));
+        const ulonglong2 k1 = *reinterpret_cast<const ulonglong2*>(slot + sw<kTile>(kg + 8, c));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(sq + (rg + i) * (D + 4) + c * 4);
+          acc[i][0] = fma2(q.y, k0.y, fma2(q.x, k0.x, acc[i][0]));
+          acc[i][1] = fma2(q.y, k1.y, fma2(q.x, k1.x, acc[i][1]));
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float2 h = halves(acc[i][e]);
+          s[i][e] = h.x + h.y;
+#pragma unroll
+          for (int w = 8 * kGroups; w < 32; w *= 2) s[i][e] += __shfl_xor_sync(0xffffffffu, s[i][e], w);
+        }
+    } else {
+      // kIn rows x keys lane % 4 and + 4 x one of kParts parts of D; bit 2 of the lane is bit 2 of the piece,
+      // which keeps eight lanes' pieces of K in different banks
+      constexpr int kIn = N < 8 ? N : 8, kParts = 8 * kIn / N < 8 ? 4 : 8, kPieces = D / 4 / kParts;
+      const int s0 = (lane >> 2) & 1, s1 = (lane >> 3) & 1, hi = lane >> 4;
+      const int c0 = 4 * s0 + 8 * s1 + (kParts == 8 ? hi * 16 : 0);
+      const float* rows = sq + (kParts == 8 ? 0 : hi * 8) * (D + 4);
+      uint64_t acc[kIn][2] = {};
+#pragma unroll(kIn == 8 ? 2 : 4)
+      for (int x = 0; x < kPieces; ++x) {
+        const int c = c0 + (x & 3) + (x >> 2) * 16;
+        const ulonglong2 k0 = *reinterpret_cast<const ulonglong2*>(slot + sw<kTile>(lane & 3, c));
+        const ulonglong2 k1 = *reinterpret_cast<const ulonglong2*>(slot + sw<kTile>((lane & 3) + 4, c));
+#pragma unroll
+        for (int i = 0; i < kIn; ++i) {
+          const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(rows + i * (D + 4) + c * 4);
+          acc[i][0] = fma2(q.y, k0.y, fma2(q.x, k0.x, acc[i][0]));
+          acc[i][1] = fma2(q.y, k1.y, fma2(q.x, k1.x, acc[i][1]));
+        }
+      }
+      // the parts add up: a lane keeps one of its two keys, then four of its rows
+      float w[kIn];
+#pragma unroll
+      for (int i = 0; i < kIn; ++i) {
+        const float2 x0 = halves(acc[i][0]), x1 = halves(acc[i][1]);
+        const float y0 = x0.x + x0.y, y1 = x1.x + x1.y;
+        w[i] = (s0 ? y1 : y0) + __shfl_xor_sync(0xffffffffu, s0 ? y0 : y1, 4);
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float4 x = *reinterpret_cast<const float4*>(sq + (rg + i) * (D + 4) + c * 4);
-        s[i][0] = fmaf(x.x, k0.x, fmaf(x.y, k0.y, fmaf(x.z, k0.z, fmaf(x.w, k0.w, s[i][0]))));
-        s[i][1] = fmaf(x.x, k1.x, fmaf(x.y, k1.y, fmaf(x.z, k1.z, fmaf(x.w, k1.w, s[i][1]))));
+        if constexpr (kIn == 8)
+          s[i][0] = (s1 ? w[4 + i] : w[i]) + __shfl_xor_sync(0xffffffffu, s1 ? w[i] : w[4 + i], 8);
+        else
+          s[i][0] = w[i] + __shfl_xor_sync(0xffffffffu, w[i], 8);
+        if constexpr (kParts == 8) s[i][0] += __shfl_xor_sync(0xffffffffu, s[i][0], 16);
       }
     }
-    float r[4], p[4][2];
+    float r[4], p[4][kKeys];
     bool moved = false;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
+      float x = -INFINITY;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
+      for (int e = 0; e < kKeys; ++e) {
         const int j = kg + 8 * e;
         const bool in = j < valid && (tree ? (see[i] >> (node0 + j)) & 1 : live[i]);
         s[i][e] = in ? s[i][e] * a.scale_log2 : -INFINITY;
+        x = fmaxf(x, s[i][e]);
       }
-      float x = fmaxf(s[i][0], s[i][1]);
       x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
       x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
       x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
@@ -292,47 +366,74 @@ struct Rows32 {
       r[i] = up ? ex2(m[i] - x) : 1.f;
       if (up) m[i] = x;
       moved |= up;
-      const float z = m[i] == -INFINITY ? 0.f : m[i];
-      p[i][0] = ex2(s[i][0] - z);
-      p[i][1] = ex2(s[i][1] - z);
-      l[i] = fmaf(l[i], r[i], p[i][0] + p[i][1]);
+      l[i] *= r[i];
+#pragma unroll
+      for (int e = 0; e < kKeys; ++e) {
+        p[i][e] = ex2(s[i][e] - (m[i] == -INFINITY ? 0.f : m[i]));
+        l[i] += p[i][e];
+      }
     }
-    // probabilities by key, then the factors of the rows
-    *reinterpret_cast<float4*>(sp + kg * kRows + rg) = make_float4(p[0][0], p[1][0], p[2][0], p[3][0]);
-    *reinterpret_cast<float4*>(sp + (kg + 8) * kRows + rg) = make_float4(p[0][1], p[1][1], p[2][1], p[3][1]);
+    float* factors = sp + kTile * N;
+    if (split() == 0) {
+#pragma unroll
+      for (int e = 0; e < kKeys; ++e)
+        *reinterpret_cast<float4*>(p_at(sp, kg + 8 * e, rg)) = make_float4(p[0][e], p[1][e], p[2][e], p[3][e]);
+    }
     moved = __any_sync(0xffffffffu, moved);
-    if (moved && kg == 0) *reinterpret_cast<float4*>(sp + kTile * kRows + rg) = make_float4(r[0], r[1], r[2], r[3]);
+    if (moved && kg == 0 && split() == 0) *reinterpret_cast<float4*>(factors + rg) = make_float4(r[0], r[1], r[2], r[3]);
     __syncwarp();
     if (moved) {
 #pragma unroll
-      for (int i = 0; i < kRows; ++i) {
-        const float f = sp[kTile * kRows + i];
+      for (int i = 0; i < N; i += 4) {
+        const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(factors + i);
 #pragma unroll
-        for (int c = 0; c < C; ++c) o[i][c] *= f;
+        for (int c = 0; c < C; ++c) {
+          o[i / 2][c] = fma2(o[i / 2][c], f.x, 0);
+          o[i / 2 + 1][c] = fma2(o[i / 2 + 1][c], f.y, 0);
+        }
       }
     }
-    const bool some = valid < kTile || tree;  // values that count for some rows only: weight 0 is no product
-#pragma unroll 2
-    for (int j = 0; j < kTile; ++j) {
-      float v[C];
+    auto values = [&](int j, float* v) {
       if constexpr (C == 4) {
-        const float4 x = *reinterpret_cast<const float4*>(vs + sw(j, lane));
+        const float4 x = *reinterpret_cast<const float4*>(vs + sw<kTile>(j, lane));
         v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
       } else {
-        const float2 x = *reinterpret_cast<const float2*>(vs + sw(j, lane >> 1) + 8 * (lane & 1));
+        const float2 x = *reinterpret_cast<const float2*>(vs + sw<kTile>(j, lane >> 1) + 8 * (lane & 1));
         v[0] = x.x; v[1] = x.y;
       }
+    };
+    if (valid == kTile && !tree) {
 #pragma unroll
-      for (int i0 = 0; i0 < kRows; i0 += 4) {
-        const float4 w = *reinterpret_cast<const float4*>(sp + j * kRows + i0);
-        const float pw[4] = {w.x, w.y, w.z, w.w};
+      for (int j = 0; j < kTile; ++j) {
+        float v[C];
+        values(j, v);
+        uint64_t vv[C];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int c = 0; c < C; ++c) vv[c] = pair_of(v[c], v[c]);
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+          const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(p_at(sp, j, i));
 #pragma unroll
           for (int c = 0; c < C; ++c) {
-            const float x = fmaf(pw[i], v[c], o[i0 + i][c]);
-            o[i0 + i][c] = some && pw[i] == 0.f ? o[i0 + i][c] : x;
+            o[i / 2][c] = fma2(w.x, vv[c], o[i / 2][c]);
+            o[i / 2 + 1][c] = fma2(w.y, vv[c], o[i / 2 + 1][c]);
           }
+        }
+      }
+    } else {  // values that count for some rows only: weight 0 is no product
+#pragma unroll 1
+      for (int j = 0; j < valid; ++j) {
+        float v[C];
+        values(j, v);
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+          const float2 w = *reinterpret_cast<const float2*>(p_at(sp, j, i) + (i & 2));
+#pragma unroll
+          for (int c = 0; c < C; ++c) {
+            const float2 x = halves(o[i / 2][c]);
+            o[i / 2][c] = pair_of(w.x != 0.f ? fmaf(w.x, v[c], x.x) : x.x, w.y != 0.f ? fmaf(w.y, v[c], x.y) : x.y);
+          }
+        }
       }
     }
     __syncwarp();
@@ -345,24 +446,29 @@ struct Rows32 {
       float x = l[i] + __shfl_xor_sync(0xffffffffu, l[i], 1);
       x += __shfl_xor_sync(0xffffffffu, x, 2);
       x += __shfl_xor_sync(0xffffffffu, x, 4);
-      if ((lane & 7) == 0) {
-        sm[(lane >> 3) * 4 + i] = m[i];
-        sl[(lane >> 3) * 4 + i] = x;
+      if ((lane & 7) == 0 && split() == 0) {
+        sm[group() * 4 + i] = m[i];
+        sl[group() * 4 + i] = x;
       }
     }
 #pragma unroll
-    for (int r = 0; r < kRows; ++r)
+    for (int r = 0; r < N; r += 2)
 #pragma unroll
-      for (int c = 0; c < C; ++c) slot[o_at<D>(r, lane * C + c)] = o[r][c];
+      for (int c = 0; c < C; ++c) {
+        const float2 x = halves(o[r / 2][c]);
+        slot[o_at<D>(r, lane * C + c)] = x.x;
+        slot[o_at<D>(r + 1, lane * C + c)] = x.y;
+      }
   }
 };
 
-// The nodes' keys and values into the cache. Up to 16 nodes leave the first
-// warp to the products: the other three copy.
+// The nodes' keys and values into the cache. Nodes that one warp takes
+// leave the first to the products: the others copy.
 template <typename T, int D>
 FXB_DEV void store_nodes(const Params& a, int b, int hk, const Row& row) {
   constexpr int kPer = 16 / sizeof(T), CH = D / kPer;  // 16-byte pieces of a row
-  const int skip = row.n <= kTile ? 32 : 0, tid = (int)threadIdx.x - skip;
+  constexpr int kThreads = Shape<T, D>::kThreads;
+  const int skip = row.n <= Shape<T, D>::kTile ? 32 : 0, tid = (int)threadIdx.x - skip;
   if (tid < 0) return;
   const T* k = static_cast<const T*>(a.k) + b * a.k_sb + hk * a.k_sh;
   const T* v = static_cast<const T*>(a.v) + b * a.v_sb + hk * a.v_sh;
@@ -382,15 +488,15 @@ FXB_DEV void store_nodes(const Params& a, int b, int hk, const Row& row) {
   }
 }
 
-template <typename T, int D> struct RowsOf { using type = Rows16<T, D>; };
-template <int D> struct RowsOf<float, D> { using type = Rows32<D>; };
+template <typename T, int D, int N> struct RowsOf { using type = Rows16<T, D>; };
+template <int D, int N> struct RowsOf<float, D, N> { using type = Rows32<D, N>; };
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads)
+template <typename T, int D, int N>
+__global__ void __launch_bounds__(Shape<T, D>::kThreads, Shape<T, D>::kCtas)
 tree_attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                const __grid_constant__ CUtensorMap tmNK, const __grid_constant__ CUtensorMap tmNV, const Params a) {
   using S = Shape<T, D>;
-  constexpr int ST = S::kStages;
+  constexpr int ST = S::kStages, kTile = S::kTile, kWarps = S::kWarps, kThreads = S::kThreads;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t bars[kWarps][ST];
   __shared__ float sm[kWarps][kRows], sl[kWarps][kRows];
@@ -466,7 +572,7 @@ tree_attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       window = front;
     }
   };
-  typename RowsOf<T, D>::type rows;
+  typename RowsOf<T, D, N>::type rows;
   rows.begin(a, c.b, c.hk, c.rt * kRows, c.row.n, sq);  // the loads of Q are under way while the ring fills
   for (int i = 0; i < ST; ++i) fetch();
 
@@ -503,8 +609,9 @@ tree_attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       const bool begun = u_begin >= start;  // this block has the item's first keys
       const bool whole = begun && tree;
       float* part = part_of<kRows, D>(a, blockIdx.x, begun);
-      for (int i = threadIdx.x; i < kRows * (D / 4); i += kThreads) {
-        const int r = i % kRows, d = i / kRows * 4;
+      constexpr int kHeld = decltype(rows)::kHeld;
+      for (int i = threadIdx.x; i < kHeld * (D / 4); i += kThreads) {
+        const int r = i % kHeld, d = i / kHeld * 4;
         float mx = sm[0][r];
 #pragma unroll
         for (int w = 1; w < kWarps; ++w) mx = fmaxf(mx, sm[w][r]);
@@ -584,23 +691,23 @@ size_t workspace_bytes(const fxb_tree_attn_args* x) {
   return kCounters + (size_t)rows_grid(x->dtype, x->D) * 2 * kRows * (x->D + 2) * sizeof(float);
 }
 
-template <typename T, int D>
+template <typename T, int D, int N = kRows>
 int launch(const fxb_tree_attn_args* x, Params& a, void* stream) {
+  using S = Shape<T, D>;
   CUtensorMap k, v, nk, nv;
   const auto t = map_type<T>();
   const int e = sizeof(T);
-  if (int r = encode_rows(&k, t, e, x->k_pages, D, x->page, x->kp_st, x->Hkv, x->kp_sh, x->P, x->kp_sp, kTile, 1)) return r;
-  if (int r = encode_rows(&v, t, e, x->v_pages, D, x->page, x->vp_st, x->Hkv, x->vp_sh, x->P, x->vp_sp, kTile, 1)) return r;
-  if (int r = encode_rows(&nk, t, e, x->k, D, x->T, x->k_st, x->Hkv, x->k_sh, x->B, x->k_sb, kTile, 1)) return r;
-  if (int r = encode_rows(&nv, t, e, x->v, D, x->T, x->v_st, x->Hkv, x->v_sh, x->B, x->v_sb, kTile, 1)) return r;
+  if (int r = encode_rows(&k, t, e, x->k_pages, D, x->page, x->kp_st, x->Hkv, x->kp_sh, x->P, x->kp_sp, S::kTile, 1)) return r;
+  if (int r = encode_rows(&v, t, e, x->v_pages, D, x->page, x->vp_st, x->Hkv, x->vp_sh, x->P, x->vp_sp, S::kTile, 1)) return r;
+  if (int r = encode_rows(&nk, t, e, x->k, D, x->T, x->k_st, x->Hkv, x->k_sh, x->B, x->k_sb, S::kTile, 1)) return r;
+  if (int r = encode_rows(&nv, t, e, x->v, D, x->T, x->v_st, x->Hkv, x->v_sh, x->B, x->v_sb, S::kTile, 1)) return r;
   a.RT = (a.R + kRows - 1) / kRows;
   const int grid = grid_of(x, a, kBlockKeys, rows_grid(x->dtype, D));
-  using S = Shape<T, D>;
   if (int r = fxb::check_cuda(
-          cudaFuncSetAttribute(tree_attn_rows<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem),
+          cudaFuncSetAttribute(tree_attn_rows<T, D, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem),
           "fxb_tree_attn"))
     return r;
-  fxb::pdl_launch(tree_attn_rows<T, D>, dim3(grid), dim3(kThreads), S::kSmem, fxb::as_stream(stream), k, v, nk, nv, a);
+  fxb::pdl_launch(tree_attn_rows<T, D, N>, dim3(grid), dim3(S::kThreads), S::kSmem, fxb::as_stream(stream), k, v, nk, nv, a);
   return fxb::check_launch("fxb_tree_attn");
 }
 
@@ -692,8 +799,11 @@ int fxb_tree_attn(const fxb_tree_attn_args* a, void* stream) {
   p.parts = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + kCounters);
   p.err = err;
   if (many_rows(a->dtype, a->T, G)) return launch_wide(a, p, stream);
-  if (a->dtype == FXB_DTYPE_F32)
+  if (a->dtype == FXB_DTYPE_F32) {
+    if (p.R <= 4) return a->D == 64 ? launch<float, 64, 4>(a, p, stream) : launch<float, 128, 4>(a, p, stream);
+    if (p.R <= 8) return a->D == 64 ? launch<float, 64, 8>(a, p, stream) : launch<float, 128, 8>(a, p, stream);
     return a->D == 64 ? launch<float, 64>(a, p, stream) : launch<float, 128>(a, p, stream);
+  }
   if (a->dtype == FXB_DTYPE_F16)
     return a->D == 64 ? launch<__half, 64>(a, p, stream) : launch<__half, 128>(a, p, stream);
   return a->D == 64 ? launch<__nv_bfloat16, 64>(a, p, stream)
