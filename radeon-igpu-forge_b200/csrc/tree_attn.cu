@@ -1,6 +1,16 @@
 // Attention of a tree of drafted tokens over a paged KV cache (fxb_tree_attn):
 // the kernel for few rows and the entry point. No reference counterpart: its
 // sampler keeps no cache (ml/fxlm/sample.py:63-73).
+//
+// Every warp works by itself on its own keys of each block (16 of 64; 8 in
+// fp32 with D = 128), from copies that it starts by itself, so that nothing but
+// an item's end makes one warp wait for another. What bounds it: HBM while the
+// cache is long (48 rows of 4 nodes x 32 heads over 8 key heads, up to 8192
+// slots, D = 128: 191 us, 6.1 TB/s, 0.94 of the rate of a copy); a chain of
+// latencies where it is short (one token of 12 heads at 1023 slots: 8.6 us: the
+// launch, the share of the work, the first copies, the join of the parts); in
+// fp32 from 16 rows on the FMA pipe and shared memory, which are busy 0.41 and
+// 0.52 of the time (8 rows of 24 at 39062 slots, D = 64).
 #include "tree_attn.cuh"
 
 namespace {
@@ -23,6 +33,7 @@ template <typename T, int D> struct Shape {
   static constexpr int kQBytes = sizeof(T) == 4 ? kRows * kQPitch * 4 : 0;
   static constexpr int kPBytes = sizeof(T) == 4 ? kWarps * (kTile * kRows + kRows) * 4 : 0;
   static constexpr int kSmem = 1024 + kWarps * kStages * kSlot + kQBytes + kPBytes;
+  // 98 KB under way in a thread block, two blocks an SM; fp32 with D = 128 takes 196 KB for as many keys
   static constexpr int kCtas = kSmem <= 112 * 1024 ? 2 : 1;   // thread blocks of an SM
 };
 // offset of element d of row r of O in a slot: 32-byte pieces exchanged by row, so that the
@@ -226,9 +237,14 @@ struct Rows16 {
 };
 
 // fp32: FMA, two at once (fma.rn.f32x2). A warp holds the first N rows of a
-// tile. The scores, summed in parts of D, lie four rows and every eighth key
-// to a lane (with N < 16 in kSplit copies). For O a lane has all N rows, two
-// to a register pair, and D / 32 columns.
+// tile: 4, 8 or 16, the fewest that hold the call's rows (4 rows of 2 nodes x
+// 13 heads at 6009 slots, D = 128: 61 us with 4, 107 with 16; 3 rows of 5 nodes
+// at 517 slots, D = 64: 9.8 us with 8, 11.8 with 16). The scores, summed in
+// parts of D, lie four rows and every eighth key to a lane (with N < 16 in
+// kSplit copies). For O a lane has all N rows, two to a register pair, and
+// D / 32 columns. 8 keys a warp and eight warps for D = 128 (that case with 16
+// keys and four warps: 84 us), 16 keys and two blocks of four warps for D = 64
+// (8 rows of 24 at 39062 slots: 159 us; 8 keys and eight warps: 237 us).
 FXB_DEV uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   uint64_t d;
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
@@ -676,7 +692,13 @@ template <typename T> constexpr CUtensorMapDataType map_type() {
 }
 // Few or many rows of a key head. The first kernel reads the cache once for
 // every 16 rows and leaves 16 x 16 products to a warp; the second takes up to
-// 128 rows with one reading, in tiles of 128 whatever the number of rows.
+// 128 rows with one reading, in tiles of 128 whatever the number of rows. From
+// 17 rows on the second reading costs more than the empty rows (16 rows of 24
+// at 6000 slots, D = 128: 57.5 us against 84.8; 4 rows of 32 at 30000: 78
+// against 125; 8 rows of 48 at 1000, D = 64: 20.1 against 22.5), but for short
+// caches, where both are near a launch (2 rows of 18 at 100 slots: 9.3 against
+// 8.6). The lengths lie on the device, so the rule cannot ask for them. More
+// than 128 query heads a key head do not fit a tile of whole nodes.
 bool many_rows(int dtype, int T, int G) { return dtype != FXB_DTYPE_F32 && T * G > kRows && G <= 128; }
 
 template <typename T, int D> constexpr int rows_ctas() { return Shape<T, D>::kCtas; }

@@ -8,6 +8,11 @@
 // ends. Every sum is taken over floor(w * 2^36) in 64-bit integers, so it does
 // not depend on how the row is divided, and every other step is one rounded
 // fp32 operation per element in a fixed order.
+//
+// What bounds it: latency. One row of 8 nodes and 32768 tokens takes 4.9 us
+// (131 kB), 64 rows of 32 nodes and 50257 tokens 21.4 us (25.8 MB, 3.9 us at a
+// copy's rate): up to four rejections in a row, each of which needs the sum
+// that the one before it left, and the same row again, from L2.
 #include "common.cuh"
 #include "internal.h"
 
