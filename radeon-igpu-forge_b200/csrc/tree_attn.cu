@@ -467,14 +467,17 @@ struct Rows32 {
         sl[group() * 4 + i] = x;
       }
     }
+    __syncwarp();
 #pragma unroll
-    for (int r = 0; r < N; r += 2)
+    for (int r = 0; r < N; r += 2) {
+      const bool any0 = sm[r] != -INFINITY, any1 = sm[r + 1] != -INFINITY;  // (weights of 0 times infinity are NaN)
 #pragma unroll
       for (int c = 0; c < C; ++c) {
         const float2 x = halves(o[r / 2][c]);
-        slot[o_at<D>(r, lane * C + c)] = x.x;
-        slot[o_at<D>(r + 1, lane * C + c)] = x.y;
+        slot[o_at<D>(r, lane * C + c)] = any0 ? x.x : 0.f;
+        slot[o_at<D>(r + 1, lane * C + c)] = any1 ? x.y : 0.f;
       }
+    }
   }
 };
 

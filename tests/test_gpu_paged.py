@@ -727,3 +727,20 @@ def test_attention_many_batch_rows(dev, T, Hq, Hkv):
     from fxlm import tree_attention
     a["n_nodes"].zero_()
     assert not tree_attention(**a).any()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("T,G,D", [(3, 1, 128), (7, 1, 64), (5, 3, 64), (30, 4, 128)])
+def test_attention_context_infinity_leaves_empty_rows_zero(dev, dtype, T, G, D):
+    # an infinite value in the context: infinity for every node, zeros still for rows that are no node's
+    from fxlm import tree_attention
+    a = make(dev, dtype, 2, T, 2 * G, 2, D, [200, 70], 16, seed=5, n_nodes=[1, T], spread=0.2)
+    ref, tol = attention_64(a)
+    for b, at in ((0, 3), (0, 150), (1, 64)):
+        a["v_pages"][int(a["page_table"][b, at // 16]), :, at % 16, 9] = float("inf")
+    o = tree_attention(**a).double()
+    hit = torch.zeros_like(o, dtype=torch.bool)
+    hit[0, :1, :, 9] = hit[1, :, :, 9] = True
+    assert (o[hit] == float("inf")).all()
+    assert ((o - ref).abs() <= tol)[~hit].all()
+    assert (o[0, 1:] == 0).all()
