@@ -9,6 +9,8 @@ library's message. There is no fallback: if the library is missing or fails to
 load, every op raises.
 """
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 import threading
 
@@ -165,6 +167,18 @@ def load():
     return _LIB
 
 
+def load_binding():
+    """The extension module lib/_fxbind.so (csrc/bind.cpp), which calls the
+    library with torch tensors in hand; raises if it has not been built."""
+    path = os.path.join(_PKG_ROOT, "lib", "_fxbind.so")
+    if not os.path.exists(path):
+        raise RuntimeError(f"_fxbind.so not found at {path}: build it with `python -m fxb200.build`")
+    loader = importlib.machinery.ExtensionFileLoader("_fxbind", path)
+    module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_fxbind", loader))
+    loader.exec_module(module)
+    return module
+
+
 def last_error():
     return load().fxb_last_error().decode(errors="replace")
 
@@ -181,12 +195,6 @@ def call(name, *args):
 
 def stream_ptr(device=None):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
-
-
-def raw_stream(device_index):
-    """Handle of torch's current stream of a device as an integer, without the
-    Stream object that stream_ptr makes (2.4 us a call)."""
-    return torch._C._cuda_getCurrentRawStream(device_index)
 
 
 def ptr(t):

@@ -14,6 +14,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG_ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(PKG_ROOT, "csrc")
@@ -57,6 +58,28 @@ def _compile(src, verbose=False):
     return obj, r.stderr
 
 
+def _build_binding(force=False):
+    """lib/_fxbind.so from csrc/bind.cpp, against torch's headers (host code)."""
+    src, out = os.path.join(CSRC, "bind.cpp"), os.path.join(LIB_DIR, "_fxbind.so")
+    newest = max(os.path.getmtime(src), os.path.getmtime(os.path.join(INCLUDE, "fxb200.h")))
+    if not force and os.path.exists(out) and os.path.getmtime(out) >= newest:
+        return
+    import torch
+    home = os.path.dirname(torch.__file__)
+    cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(_nvcc()))), "include")
+    headers = os.path.join(home, "include")
+    paths = [INCLUDE, headers, os.path.join(headers, "torch", "csrc", "api", "include"), cuda,
+             sysconfig.get_path("include")]
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *("-I" + p for p in paths), src, "-o", out + ".tmp", "-L" + os.path.join(home, "lib"),
+           "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for bind.cpp:\n{r.stdout}\n{r.stderr}")
+    os.replace(out + ".tmp", out)
+
+
 def build(force=False, verbose=False, jobs=None):
     """Compile stale objects and relink; returns the library path."""
     os.makedirs(OBJ_DIR, exist_ok=True)
@@ -82,6 +105,7 @@ def build(force=False, verbose=False, jobs=None):
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
         os.replace(tmp, LIB_PATH)
+    _build_binding(force)
     return LIB_PATH
 
 

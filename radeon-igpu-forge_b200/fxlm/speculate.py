@@ -2,23 +2,32 @@
 import torch
 
 from fxb200 import _lib
-from .paged import MAX_NODES, _i32
+from .paged import MAX_NODES, _native, _refuse_i32
 
 
-def _refuse_probs(t, name, shape):
-    if t.dtype != torch.float32 or not t.is_cuda:
-        raise TypeError(f"{name} must be a cuda fp32 tensor, got {t.dtype} on {t.device}")
-    raise ValueError(f"{name} must be {shape} with unit stride on the vocabulary, got {tuple(t.shape)}")
-
-
-def _probs(t, name, shape):
-    """(address, row stride, node stride)."""
-    if not (t.dtype == torch.float32 and t.is_cuda and t.shape == shape):
-        _refuse_probs(t, name, shape)
-    sb, st, s1 = t.stride()
-    if s1 != 1 and shape[2] > 1:
-        _refuse_probs(t, name, shape)
-    return t.data_ptr(), sb, st
+def _refuse(tokens, parents, n_nodes, target_probs, u, draft_probs):
+    if tokens.dim() != 2:
+        raise ValueError(f"tokens must be (B,T), got {tuple(tokens.shape)}")
+    B, T = tokens.shape
+    if not 1 <= T <= MAX_NODES:
+        raise ValueError(f"T={T}: 1 to {MAX_NODES} nodes")
+    if tokens.dtype != torch.int64 or not tokens.is_cuda:
+        raise TypeError("tokens must be a cuda int64 tensor")
+    if not tokens.is_contiguous():
+        raise ValueError("tokens must be contiguous")
+    shape = (B, T, target_probs.shape[-1])
+    for t, name in ((target_probs, "target_probs"), (draft_probs, "draft_probs")):
+        if t is None:
+            continue
+        if t.dtype != torch.float32 or not t.is_cuda:
+            raise TypeError(f"{name} must be a cuda fp32 tensor, got {t.dtype} on {t.device}")
+        if t.shape != shape or (shape[2] > 1 and t.stride(2) != 1):
+            raise ValueError(f"{name} must be {shape} with unit stride on the vocabulary, got {tuple(t.shape)}")
+    _refuse_i32(parents, "parents", (B, T))
+    _refuse_i32(n_nodes, "n_nodes", (B,))
+    if u.dtype != torch.float32 or not u.is_cuda:
+        raise TypeError("u must be a cuda fp32 tensor")
+    raise ValueError(f"u must be contiguous ({B},{T}), got {tuple(u.shape)}")
 
 
 def verify_tree(tokens, parents, n_nodes, target_probs, u, draft_probs=None):
@@ -39,28 +48,9 @@ def verify_tree(tokens, parents, n_nodes, target_probs, u, draft_probs=None):
     path (B, T) int32: accepted nodes, node 0 first, then -1; n_path (B,) int32;
     next_token (B,) int64, -1 where n_nodes is 0 or the row has no mass.
     """
-    if tokens.dim() != 2:
-        raise ValueError(f"tokens must be (B,T), got {tuple(tokens.shape)}")
-    B, T = tokens.shape
-    if not 1 <= T <= MAX_NODES:
-        raise ValueError(f"T={T}: 1 to {MAX_NODES} nodes")
-    if tokens.dtype != torch.int64 or not tokens.is_cuda:
-        raise TypeError("tokens must be a cuda int64 tensor")
-    if not tokens.is_contiguous():
-        raise ValueError("tokens must be contiguous")
-    V = target_probs.shape[-1]
-    p, p_sb, p_st = _probs(target_probs, "target_probs", (B, T, V))
-    q, q_sb, q_st = (None, 0, 0) if draft_probs is None else _probs(draft_probs, "draft_probs", (B, T, V))
-    par, nn = _i32(parents, "parents", (B, T)), _i32(n_nodes, "n_nodes", (B,))
-    if u.dtype != torch.float32 or not u.is_cuda:
-        raise TypeError("u must be a cuda fp32 tensor")
-    if u.shape != (B, T) or not u.is_contiguous():
-        raise ValueError(f"u must be contiguous ({B},{T}), got {tuple(u.shape)}")
-    path, n_path, nxt = torch.empty_like(parents), torch.empty_like(n_nodes), tokens.new_empty(B)
-    if B:
-        rc = _lib.load().fxb_verify_tree(
-            tokens.data_ptr(), par, nn, p, p_sb, p_st, q, q_sb, q_st, u.data_ptr(), path.data_ptr(),
-            n_path.data_ptr(), nxt.data_ptr(), B, T, V, _lib.raw_stream(tokens.get_device()))
-        if rc:
-            _lib.check(rc, "fxb_verify_tree")
-    return path, n_path, nxt
+    r = _native().verify_tree(tokens, parents, n_nodes, target_probs, u, draft_probs)
+    if r is None:
+        _refuse(tokens, parents, n_nodes, target_probs, u, draft_probs)
+    if type(r) is int:
+        _lib.check(r, "fxb_verify_tree")
+    return r

@@ -39,11 +39,6 @@ def test_struct_layouts_match(lib):
     from fxb200 import _lib
     assert lib.fxb_abi_struct_size(2) == ctypes.sizeof(_lib.TreeAttnArgs)
     assert lib.fxb_abi_struct_size(3) == ctypes.sizeof(_lib.KvArgs)
-    from fxlm import paged
-    for packed, mirror in ((paged._TREE_ARGS, _lib.TreeAttnArgs), (paged._KV_ARGS, _lib.KvArgs)):
-        assert packed.size == ctypes.sizeof(mirror)
-        m = mirror.from_buffer_copy(packed.pack(*range(1, len(mirror._fields_) + 1)))
-        assert [getattr(m, f[0]) for f in mirror._fields_] == list(range(1, len(mirror._fields_) + 1))
 
 
 @pytest.mark.parametrize("change,word", [
@@ -200,3 +195,20 @@ def test_next_probs():
     p = next_probs(x, 0.5, 2)
     assert p[0, 1] == p[0, 2] == 0.5 and p[0, 0] == p[0, 3] == p[0, 4] == 0
     assert torch.allclose(next_probs(x, 1.0, 0), torch.softmax(x, -1))
+
+
+def test_wrappers_take_tensors_and_say_what_is_wrong():
+    from fxlm import kv_commit, kv_fork, kv_reserve, verify_tree
+    i = torch.zeros(1, dtype=torch.int32)
+    pool = torch.zeros(2, 4, 2, 16, 64, dtype=torch.bfloat16)
+    args = (i[:, None], i, i, torch.zeros(4, dtype=torch.int32))
+    with pytest.raises(AttributeError):
+        kv_commit(pool, pool, None, i, i, i, i[:, None], i)
+    with pytest.raises(TypeError, match="page_table"):
+        kv_commit(pool, pool, i.long()[:, None], *args[1:], i[:, None], i)
+    with pytest.raises(TypeError, match="page_table"):
+        kv_fork(pool, pool, *args, [0])
+    with pytest.raises(TypeError):
+        kv_reserve(*args, i, "16")
+    with pytest.raises(TypeError, match="int64"):
+        verify_tree(torch.zeros(1, 2), i, i, torch.zeros(1, 2, 8), torch.zeros(1, 2))
