@@ -30,9 +30,11 @@
 // exponentials take 1024 of their unit and the products 1024 of theirs). Without
 // the copies that case takes 57.9 us, without the exponentials 55.8, without
 // seven of eight products 57.9, without all three 46.8: no unit is the limit.
-// Not faster: a group of warps for each of two tiles in flight (63.7 us), 16
-// softmax warps with 32 keys a thread (62.1), packed fp32 pairs and three-way
-// maxima (59.8), one arrival a warp (61.2).
+// The copying warp (1300 cycles an operand) and the softmax warps (2500 a tile)
+// keep the same pace. Not faster: a group of warps for each of two tiles in
+// flight (63.7 us), 16 softmax warps with 32 keys a thread (62.1), packed fp32
+// pairs and three-way maxima (59.8), one arrival a warp (61.2), a ring and a
+// copying warp each for keys and values (59.7 to 63.1: the softmax's pace).
 #include "tree_attn.cuh"
 
 namespace {
