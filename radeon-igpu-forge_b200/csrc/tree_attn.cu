@@ -9,8 +9,8 @@
 // slots, D = 128: 191 us, 6.1 TB/s, 0.94 of the rate of a copy); a chain of
 // latencies where it is short (one token of 12 heads at 1023 slots: 8.6 us: the
 // launch, the share of the work, the first copies, the join of the parts); in
-// fp32 from 16 rows on the FMA pipe and shared memory, which are busy 0.41 and
-// 0.52 of the time (8 rows of 24 at 39062 slots, D = 64).
+// fp32 from 16 rows on the issue of FMA and shared-memory loads by two warps a
+// scheduler (8 rows of 24 at 39062 slots, D = 64: 141 us, 16.5 TFLOP/s).
 #include "tree_attn.cuh"
 
 namespace {
@@ -244,7 +244,8 @@ struct Rows16 {
 // kSplit copies). For O a lane has all N rows, two to a register pair, and
 // D / 32 columns. 8 keys a warp and eight warps for D = 128 (that case with 16
 // keys and four warps: 84 us), 16 keys and two blocks of four warps for D = 64
-// (8 rows of 24 at 39062 slots: 159 us; 8 keys and eight warps: 237 us).
+// (8 rows of 24 at 39062 slots: 159 us, 237 with 8 keys and eight warps; 141 us
+// now that the swizzle's places are found once a tile).
 FXB_DEV uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   uint64_t d;
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
@@ -260,6 +261,7 @@ FXB_DEV float2 halves(uint64_t x) {
   asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(x));
   return d;
 }
+FXB_DEV ulonglong2 load2(const uint8_t* p) { return *reinterpret_cast<const ulonglong2*>(p); }
 template <int D, int N>
 struct Rows32 {
   static constexpr int kHeld = N, kTile = Shape<float, D>::kTile;
@@ -269,6 +271,9 @@ struct Rows32 {
   uint64_t see[4];
   bool live[4];
 
+  // The swizzle's places, found once a tile: where a lane reads pieces i = 0 .. 7 of a key, and where in row j of
+  // the values its columns lie (xor of the piece and the row; everything else is a constant)
+  FXB_DEV static uint32_t key_at(int row, int piece) { return row * 128 + ((piece ^ (row & 7)) << 4); }
   FXB_DEV static int group() { return (threadIdx.x & 31) / 8 % kGroups; }
   FXB_DEV static int split() { return (threadIdx.x & 31) / 8 / kGroups; }
   // Probabilities lie by key, pieces of four rows exchanged by key: a lane's stores then fall into different banks
@@ -305,14 +310,18 @@ struct Rows32 {
     float s[4][kKeys];
     if constexpr (kKeys == 2) {  // four rows x keys kg and kg + 8 x every kSplit-th piece of D
       uint64_t acc[4][2] = {};
-#pragma unroll 4
+      const float* qs = sq + rg * (D + 4) + split() * 4;
+      uint32_t at[8 / kSplit];
+#pragma unroll
+      for (int x = 0; x < 8 / kSplit; ++x) at[x] = key_at(kg, x * kSplit + split());
+#pragma unroll
       for (int x = 0; x < D / 4 / kSplit; ++x) {
-        const int c = x * kSplit + split();
-        const ulonglong2 k0 = *reinterpret_cast<const ulonglong2*>(slot + sw<kTile>(kg, c));
-        const ulonglong2 k1 = *reinterpret_cast<const ulonglong2*>(slot + sw<kTile>(kg + 8, c));
+        const int box = x * kSplit / 8;
+        const ulonglong2 k0 = load2(slot + at[x % (8 / kSplit)] + box * kTile * 128);
+        const ulonglong2 k1 = load2(slot + at[x % (8 / kSplit)] + box * kTile * 128 + 8 * 128);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(sq + (rg + i) * (D + 4) + c * 4);
+          const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(qs + i * (D + 4) + x * kSplit * 4);
           acc[i][0] = fma2(q.y, k0.y, fma2(q.x, k0.x, acc[i][0]));
           acc[i][1] = fma2(q.y, k1.y, fma2(q.x, k1.x, acc[i][1]));
         }
@@ -332,13 +341,17 @@ struct Rows32 {
       constexpr int kIn = N < 8 ? N : 8, kParts = 8 * kIn / N < 8 ? 4 : 8, kPieces = D / 4 / kParts;
       const int s0 = (lane >> 2) & 1, s1 = (lane >> 3) & 1, hi = lane >> 4;
       const int c0 = 4 * s0 + 8 * s1 + (kParts == 8 ? hi * 16 : 0);
-      const float* rows = sq + (kParts == 8 ? 0 : hi * 8) * (D + 4);
+      const float* rows = sq + (kParts == 8 ? 0 : hi * 8) * (D + 4) + c0 * 4;
+      uint32_t at[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        at[x] = (c0 >> 3) * kTile * 128 + key_at(lane & 3, (c0 & 7) + x);
       uint64_t acc[kIn][2] = {};
-#pragma unroll(kIn == 8 ? 2 : 4)
+#pragma unroll
       for (int x = 0; x < kPieces; ++x) {
-        const int c = c0 + (x & 3) + (x >> 2) * 16;
-        const ulonglong2 k0 = *reinterpret_cast<const ulonglong2*>(slot + sw<kTile>(lane & 3, c));
-        const ulonglong2 k1 = *reinterpret_cast<const ulonglong2*>(slot + sw<kTile>((lane & 3) + 4, c));
+        const int c = (x & 3) + (x >> 2) * 16;  // behind c0
+        const ulonglong2 k0 = load2(slot + at[x & 3] + (x >> 2) * 2 * kTile * 128);
+        const ulonglong2 k1 = load2(slot + (at[x & 3] ^ 64) + 4 * 128 + (x >> 2) * 2 * kTile * 128);
 #pragma unroll
         for (int i = 0; i < kIn; ++i) {
           const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(rows + i * (D + 4) + c * 4);
@@ -378,7 +391,7 @@ struct Rows32 {
       x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
       x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
       x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-      const bool up = x > m[i];
+      const bool up = x > m[i] + kRescaleLog2;  // (as in Rows16: O is rarely rescaled)
       r[i] = up ? ex2(m[i] - x) : 1.f;
       if (up) m[i] = x;
       moved |= up;
@@ -409,20 +422,25 @@ struct Rows32 {
         }
       }
     }
-    auto values = [&](int j, float* v) {
+    const int piece = C == 4 ? lane : lane >> 1;
+    const uint8_t* vp = vs + (piece >> 3) * (kTile * 128) + (C == 4 ? 0 : 8 * (lane & 1));
+    auto values = [&](const uint8_t* at, float* v) {
       if constexpr (C == 4) {
-        const float4 x = *reinterpret_cast<const float4*>(vs + sw<kTile>(j, lane));
+        const float4 x = *reinterpret_cast<const float4*>(at);
         v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
       } else {
-        const float2 x = *reinterpret_cast<const float2*>(vs + sw<kTile>(j, lane >> 1) + 8 * (lane & 1));
+        const float2 x = *reinterpret_cast<const float2*>(at);
         v[0] = x.x; v[1] = x.y;
       }
     };
     if (valid == kTile && !tree) {
+      uint32_t at[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) at[j] = ((piece & 7) ^ j) << 4;
 #pragma unroll
       for (int j = 0; j < kTile; ++j) {
         float v[C];
-        values(j, v);
+        values(vp + at[j & 7] + j * 128, v);
         uint64_t vv[C];
 #pragma unroll
         for (int c = 0; c < C; ++c) vv[c] = pair_of(v[c], v[c]);
@@ -440,7 +458,7 @@ struct Rows32 {
 #pragma unroll 1
       for (int j = 0; j < valid; ++j) {
         float v[C];
-        values(j, v);
+        values(vp + (((piece & 7) ^ (j & 7)) << 4) + j * 128, v);
 #pragma unroll
         for (int i = 0; i < N; i += 2) {
           const float2 w = *reinterpret_cast<const float2*>(p_at(sp, j, i) + (i & 2));
