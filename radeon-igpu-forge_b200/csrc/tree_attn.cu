@@ -271,8 +271,8 @@ struct Rows32 {
   uint64_t see[4];
   bool live[4];
 
-  // The swizzle's places, found once a tile: where a lane reads pieces i = 0 .. 7 of a key, and where in row j of
-  // the values its columns lie (xor of the piece and the row; everything else is a constant)
+  // place of a piece of a key's row in a box (128-byte swizzle); a tile's few places are found once, everything
+  // else is a constant
   FXB_DEV static uint32_t key_at(int row, int piece) { return row * 128 + ((piece ^ (row & 7)) << 4); }
   FXB_DEV static int group() { return (threadIdx.x & 31) / 8 % kGroups; }
   FXB_DEV static int split() { return (threadIdx.x & 31) / 8 / kGroups; }

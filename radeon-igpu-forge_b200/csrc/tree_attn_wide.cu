@@ -47,7 +47,7 @@ constexpr int kThreads = 384;
 constexpr int kWarpS = 8, kWarpTma = 9, kWarpStore = 10, kWarpPV = 11;
 constexpr int kSoftmax = 256;  // threads of both groups
 
-constexpr int kSmall = 3072;   // shared memory behind the operands
+constexpr int kSmall = 3 * 1024; // shared memory behind the operands
 template <int D> struct Wide {
   static constexpr int kBoxes = D / 64;
   static constexpr int kOperand = kTileRows * D * 2;  // Q, K or V of a tile: D / 64 blocks of [128 rows][128 bytes]
