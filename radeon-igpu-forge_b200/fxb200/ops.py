@@ -54,18 +54,35 @@ def _gemm_workspace(device):
     return ws
 
 
+def _capturing_without_table():
+    """True in a plain CUDA-graph capture. All such captures share one default
+    stream, and a graph keeps the addresses it was given: a workspace kept by
+    stream would be zeroed by the first graph alone, shared by all of them, and
+    freed under them when a later call needs a larger one."""
+    return _CAPTURE_WS is None and torch.cuda.is_current_stream_capturing()
+
+
+def _zeroed_workspace(device, nbytes, zeroed):
+    ws = torch.empty(nbytes, device=device, dtype=torch.uint8)
+    ws[:zeroed].zero_()  # (inside a capture: a memset node of the graph)
+    return ws
+
+
 def stream_workspace(kind, device_index, stream, nbytes, zeroed):
     """Workspace of at least `nbytes` bytes for calls of one kind on a stream
     (its handle), kept like the GEMM's: one per (device, stream) for eager
-    launches, one of its own for a captured graph. Its first `zeroed` bytes are
-    zero before the first use; the kernels leave them so."""
+    launches, one of its own for a graph captured in `graph_workspaces`. In any
+    other capture each call gets one of its own, which the graph's memory pool
+    owns. Its first `zeroed` bytes are zero before the first use; the kernels
+    leave them so."""
+    device = torch.device("cuda", device_index)
+    if _capturing_without_table():
+        return _zeroed_workspace(device, nbytes, zeroed)
     table = _CAPTURE_WS if _CAPTURE_WS is not None else _STREAM_WS
     key = (kind, device_index, stream)
     ws = table.get(key)
     if ws is None or ws.numel() < nbytes:
-        ws = torch.empty(nbytes, device=torch.device("cuda", device_index), dtype=torch.uint8)
-        ws[:zeroed].zero_()
-        table[key] = ws
+        ws = table[key] = _zeroed_workspace(device, nbytes, zeroed)
     return ws
 
 

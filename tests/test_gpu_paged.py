@@ -744,3 +744,45 @@ def test_attention_context_infinity_leaves_empty_rows_zero(dev, dtype, T, G, D):
     assert (o[hit] == float("inf")).all()
     assert ((o - ref).abs() <= tol)[~hit].all()
     assert (o[0, 1:] == 0).all()
+
+
+def test_attention_plain_captures(dev):
+    # graphs captured without ops.graph_workspaces: replayed in another order than captured, with larger calls
+    # (whose workspaces are larger) and other allocations in between, and on two streams at once
+    from fxlm import tree_attention
+    few = [make(dev, BF16, 3, 4, 8, 8, 64, [500, 900, 3], 32, seed=6), make(dev, F16, 2, 2, 6, 2, 128, [4000, 70], 16, seed=7)]
+    wide = make(dev, BF16, 2, 64, 8, 1, 64, [2000, 900], 16, seed=2)
+    calls = few + [wide]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    want = []
+    with torch.cuda.stream(side):  # warm-up on the stream of the captures: the small calls' eager workspace
+        for a in few:
+            want.append(tree_attention(**a).clone())
+    side.synchronize()
+    graphs, outs = [], []
+    for a in calls:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=side):
+            outs.append(tree_attention(**a))
+    want.append(tree_attention(**wide).clone())
+    for i in (2, 1, 0, 1, 2):
+        outs[i].fill_(7)
+        with torch.cuda.stream(side):
+            side.wait_stream(torch.cuda.current_stream())
+            tree_attention(**wide)
+            noise = [torch.full((1 << 20,), 3, dtype=torch.int32, device=dev) for _ in range(8)]
+        torch.cuda.current_stream().wait_stream(side)
+        graphs[i].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[i], want[i])
+        assert all((x == 3).all() for x in noise)
+    for _ in range(5):
+        for out in outs[:2]:
+            out.fill_(7)
+        side.wait_stream(torch.cuda.current_stream())
+        graphs[0].replay()
+        with torch.cuda.stream(side):
+            graphs[1].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])

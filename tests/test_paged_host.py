@@ -212,3 +212,55 @@ def test_wrappers_take_tensors_and_say_what_is_wrong():
         kv_reserve(*args, i, "16")
     with pytest.raises(TypeError, match="int64"):
         verify_tree(torch.zeros(1, 2), i, i, torch.zeros(1, 2, 8), torch.zeros(1, 2))
+
+
+class _Buffer:
+    """Stands in for a tensor of the allocator and records its memsets."""
+
+    def __init__(self, n, log):
+        self.n, self.log = n, log
+        log.append(("new", self))
+
+    def numel(self):
+        return self.n
+
+    def __getitem__(self, part):
+        return self
+
+    def zero_(self):
+        self.log.append(("zero", self))
+
+
+@pytest.fixture
+def allocations(monkeypatch):
+    from fxb200 import ops
+    log = []
+    monkeypatch.setattr(torch, "empty", lambda n, **kw: _Buffer(n, log))
+    monkeypatch.setattr(ops, "_STREAM_WS", {})
+    return log
+
+
+def test_workspaces_of_plain_captures_are_their_own(monkeypatch, allocations):
+    # plain captures share one capture stream: each call's buffer is new and zeroed in its own graph, and none
+    # of them is handed to another call or kept where a larger request could drop it
+    from fxb200 import ops
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    eager = ops.stream_workspace("k", 0, 7, 100, 16)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    first = ops.stream_workspace("k", 0, 7, 100, 16)
+    second = ops.stream_workspace("k", 0, 7, 100, 16)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    assert len({id(x) for x in (eager, first, second)}) == 3
+    assert [x for what, x in allocations if what == "zero"] == [eager, first, second]
+    assert ops.stream_workspace("k", 0, 7, 50, 16) is eager
+    assert list(ops._STREAM_WS.values()) == [eager]
+
+
+def test_workspaces_of_a_table_are_kept(monkeypatch, allocations):
+    from fxb200 import ops
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    table = {}
+    with ops.graph_workspaces(table):
+        ws = ops.stream_workspace("k", 0, 7, 100, 16)
+        assert ops.stream_workspace("k", 0, 7, 100, 16) is ws and list(table.values()) == [ws]
+    assert not ops._STREAM_WS
