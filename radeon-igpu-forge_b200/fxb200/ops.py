@@ -31,27 +31,15 @@ def set_gemm_timing(records):
 
 # GEMM workspace (tail split, see fxb_gemm_args.workspace): one buffer per
 # (device, stream) for eager launches, allocated on first use and kept. A
-# captured CUDA graph gets workspaces of its own (see `graph_workspaces`), so
-# two graphs, or a graph and eager launches, never share arrival counters.
+# captured CUDA graph gets workspaces of its own (see `graph_workspaces`; in a
+# plain capture each call has one), so two graphs, or a graph and eager
+# launches, never share arrival counters.
 # The first 4096 bytes are arrival counters that must be zero before a GEMM
 # starts; GEMMs reset them themselves, except after an expired wait (device
 # error word bit 1), when `_reset_workspaces` zeroes them.
 _GEMM_WS = {}
 _STREAM_WS = {}      # the same for stream_workspace
 _CAPTURE_WS = None  # dict of the graph being captured, or None
-
-
-def _gemm_workspace(device):
-    st = torch.cuda.current_stream(device)
-    key = (device.index, st.cuda_stream)
-    table = _CAPTURE_WS if _CAPTURE_WS is not None else _GEMM_WS
-    ws = table.get(key)
-    if ws is None:
-        n = int(_lib.load().fxb_gemm_workspace_size())
-        ws = torch.empty(n, device=device, dtype=torch.uint8)
-        ws[:4096].zero_()  # the arrival counters (inside a capture: a memset node of the graph)
-        table[key] = ws
-    return ws
 
 
 def _capturing_without_table():
@@ -65,6 +53,21 @@ def _capturing_without_table():
 def _zeroed_workspace(device, nbytes, zeroed):
     ws = torch.empty(nbytes, device=device, dtype=torch.uint8)
     ws[:zeroed].zero_()  # (inside a capture: a memset node of the graph)
+    return ws
+
+
+def _gemm_workspace(device):
+    def new():
+        return _zeroed_workspace(device, int(_lib.load().fxb_gemm_workspace_size()), 4096)
+
+    if _capturing_without_table():
+        return new()
+    st = torch.cuda.current_stream(device)
+    key = (device.index, st.cuda_stream)
+    table = _CAPTURE_WS if _CAPTURE_WS is not None else _GEMM_WS
+    ws = table.get(key)
+    if ws is None:
+        ws = table[key] = new()
     return ws
 
 

@@ -544,3 +544,25 @@ def test_config3_cross_entropy_full_shape(dev):
     err = (buf[rows].float() - gref).abs().max().item()
     assert err <= 2e-2 * gref.abs().max().item(), err
     assert not torch.isnan(buf[rows].float()).any()
+
+
+def test_gemm_plain_captures(dev):
+    # graphs captured without ops.graph_workspaces, the one captured last replayed first: each split-tail GEMM has
+    # counters of its own, zeroed in its own graph
+    from fxb200 import _lib, ops
+    M, N, K = 1024, 768, 2304
+    assert _lib.gemm_plan(M, N, K)[2] > 1
+    g = torch.Generator(device=dev).manual_seed(3)
+    A, B = (torch.randn(*s, generator=g, device=dev).to(torch.bfloat16) for s in ((M, K), (N, K)))
+    want = torch.empty(M, N, device=dev, dtype=torch.bfloat16)
+    ops.gemm(A, B, want)
+    graphs, outs = [], [torch.zeros_like(want) for _ in range(2)]
+    for out in outs:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            ops.gemm(A, B, out)
+    for i in (1, 0, 1):
+        outs[i].zero_()
+        graphs[i].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[i], want)

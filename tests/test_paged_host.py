@@ -264,3 +264,20 @@ def test_workspaces_of_a_table_are_kept(monkeypatch, allocations):
         ws = ops.stream_workspace("k", 0, 7, 100, 16)
         assert ops.stream_workspace("k", 0, 7, 100, 16) is ws and list(table.values()) == [ws]
     assert not ops._STREAM_WS
+
+
+def test_gemm_workspaces_of_plain_captures_are_their_own(monkeypatch, allocations):
+    from fxb200 import ops
+
+    class Stream:
+        cuda_stream = 7
+
+    monkeypatch.setattr(ops, "_GEMM_WS", {})
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: Stream)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    device = torch.device("cuda", 0)
+    first, second = ops._gemm_workspace(device), ops._gemm_workspace(device)
+    assert first is not second and not ops._GEMM_WS
+    assert [x for what, x in allocations if what == "zero"] == [first, second]
+    with ops.graph_workspaces({}):
+        assert ops._gemm_workspace(device) is ops._gemm_workspace(device)
