@@ -176,8 +176,7 @@ __global__ void __launch_bounds__(kThreads) kv_commit_kernel(KvParams c, const i
     int all;
     const int before = block_scan(add, &all);
     if (s < c.S) off[s] = total + before;
-    total = all > c.P - total ? c.P + 1 : total + all;  // more than the pool has: no need to count on
-    if (total > c.P) break;
+    total = all > c.P - total ? c.P + 1 : total + all;  // more than the pool has: stays so (every length is written)
   }
   if (total == 0) return;
   __syncthreads();

@@ -786,3 +786,27 @@ def test_attention_plain_captures(dev):
             graphs[1].replay()
         torch.cuda.synchronize()
         assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+
+
+def test_commit_lengths_when_the_pool_is_too_small(dev):
+    # more rows than a thread block has threads, the first of which want more than the pool has: every length is
+    # returned and every token moved, no page is handed out
+    from fxb200 import _lib
+    from fxlm import kv_commit
+    rng = np.random.RandomState(3)
+    S, T, page = 1300, 5, 16
+    lens = [int(rng.randint(0, 40)) for _ in range(S)]
+    held = sum(-(-(n + T) // page) for n in lens)
+    c = cache(dev, BF16, S, 2, 1, 8, page, lens, T, P=held + 3, W=20, seed=3)
+    want = PlainPages(c)
+    n = [int(rng.randint(0, T + 1)) for _ in range(S)]
+    path = [sorted(rng.permutation(T)[:k].tolist()) + [-1] * (T - k) for k in n]
+    room = [250] * S
+    assert not want.commit(path, n, room)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    out = i32([-7] * S)
+    assert kv_commit(c["k"], c["v"], c["table"], c["n_pages"], c["lens"], c["ref"], i32(path), i32(n),
+                     room=i32(room), out=out) is not None
+    same(c, want, out)
+    with pytest.raises(RuntimeError, match="KV cache"):
+        _lib.raise_on_device_error()
