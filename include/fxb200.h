@@ -441,8 +441,10 @@ typedef struct fxb_kv_args {
  * strictly; path == NULL: nothing moves and n_path counts as 0), then
  * lens_out[s] = lens[s] + n_path[s], and where room[s] > 0 (room may be NULL)
  * the row is given pages for lens_out[s] + room[s] slots: the lowest-numbered
- * free ones, rows in order. If the pool lacks them no row is given any (bit 16
- * of the device error word). lens_out must not be lens. */
+ * free ones, rows in order. If the pool lacks them no row is given any. A token
+ * whose entry does not ascend, or whose slot the row does not hold, stays where
+ * it is, the others move; n_path outside [0, T] counts as the nearer end (bit
+ * 16 of the device error word in each case). lens_out must not be lens. */
 int fxb_kv_commit(const fxb_kv_args* args, const int32_t* path, int64_t path_ss, int32_t T,
                   const int32_t* n_path, const int32_t* room, int32_t* lens_out, void* stream);
 

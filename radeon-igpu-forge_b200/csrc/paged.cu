@@ -161,7 +161,9 @@ __global__ void __launch_bounds__(kThreads) kv_commit_kernel(KvParams c, const i
     const int s = s0 + threadIdx.x;
     int add = 0;
     if (s < c.S) {
-      const int len = c.lens[s] + (path ? min(max(n_path[s], 0), T) : 0);
+      const int n_in = path ? n_path[s] : 0, n = min(max(n_in, 0), T);
+      if (n != n_in) atomicOr(c.err, FXB_DERR_PAGES);
+      const int len = c.lens[s] + n;
       lens_out[s] = len;
       const int want = room ? room[s] : 0;
       if (want > 0) {

@@ -810,3 +810,43 @@ def test_commit_lengths_when_the_pool_is_too_small(dev):
     same(c, want, out)
     with pytest.raises(RuntimeError, match="KV cache"):
         _lib.raise_on_device_error()
+
+
+@pytest.mark.parametrize("n", [[3, 1], [1, -1]])
+def test_commit_reports_counts_outside_the_tree(dev, n):
+    from fxb200 import _lib
+    from fxlm import kv_commit
+    c = cache(dev, BF16, 2, 1, 1, 8, 16, [4, 5], 2, seed=1)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    got = kv_commit(c["k"], c["v"], c["table"], c["n_pages"], c["lens"], c["ref"], i32([[0, 1], [0, 1]]), i32(n))
+    assert got.tolist() == [4 + min(n[0], 2), 5 + max(n[1], 0)]
+    with pytest.raises(RuntimeError, match="KV cache"):
+        _lib.raise_on_device_error()
+
+
+def test_commit_moves_what_fits_of_a_path(dev):
+    # entries of a path that do not ascend, or lie outside the tree or the row's pages, are left out, each by
+    # itself; the lengths are those of the whole path; a path longer than the tree counts as the tree's length
+    from fxb200 import _lib
+    from fxlm import kv_commit
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    T, page, lens = 4, 16, [20, 30, 7]
+    for path, n in (([[2, 1, 3, -1], [1, 2, 3, -1], [0, 0, 3, -1]], [3, 3, 3]),
+                    ([[0, 2, 4, 5], [-1, 1, 3, -1], [3, 2, 1, 0]], [4, 3, 4]),
+                    ([[1, 2, 3, 3], [0, 2, 3, -1], [2, -1, -1, -1]], [9, 3, -2])):
+        c = cache(dev, BF16, 3, 2, 2, 64, page, lens, T, seed=1)
+        want = PlainPages(c)
+        for s, row in enumerate(path):
+            count = min(max(n[s], 0), T)
+            for i in range(count):
+                p = row[i]
+                if not (max(i, row[i - 1] + 1 if i else 0) <= p < T):
+                    continue
+                a, b = lens[s] + p, lens[s] + i
+                for x in (want.k, want.v):
+                    x[:, want.rows[s][b // page], :, b % page] = x[:, want.rows[s][a // page], :, a % page].clone()
+            want.lens[s] += count
+        got = kv_commit(c["k"], c["v"], c["table"], c["n_pages"], c["lens"], c["ref"], i32(path), i32(n))
+        same(c, want, got)
+        with pytest.raises(RuntimeError, match="KV cache"):
+            _lib.raise_on_device_error()
