@@ -444,7 +444,8 @@ typedef struct fxb_kv_args {
  * free ones, rows in order. If the pool lacks them no row is given any. A token
  * whose entry does not ascend, or whose slot the row does not hold, stays where
  * it is, the others move; n_path outside [0, T] counts as the nearer end (bit
- * 16 of the device error word in each case). lens_out must not be lens. */
+ * 16 of the device error word in each case). lens_out must be an array of its
+ * own, neither lens nor another argument. */
 int fxb_kv_commit(const fxb_kv_args* args, const int32_t* path, int64_t path_ss, int32_t T,
                   const int32_t* n_path, const int32_t* room, int32_t* lens_out, void* stream);
 

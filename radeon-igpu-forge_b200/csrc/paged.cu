@@ -406,11 +406,13 @@ int fxb_kv_commit(const fxb_kv_args* args, const int32_t* path, int64_t path_ss,
                   const int32_t* room, int32_t* lens_out, void* stream) {
   KvParams c = {};
   if (int r = params("fxb_kv_commit", args, path != nullptr, &c)) return r;
-  if (!lens_out || lens_out == args->lens)
-    return fxb::set_error(FXB_EINVAL, "fxb_kv_commit: lens_out must be another array than lens");
   if (path && (T < 1 || T > kMaxTree || path_ss < T || !n_path))
     return fxb::set_error(FXB_EINVAL, "fxb_kv_commit: path needs n_path, 1 <= T=%d <= %d and a row stride >= T", T,
                           kMaxTree);
+  for (const int32_t* x : {(const int32_t*)args->lens, (const int32_t*)args->n_pages, (const int32_t*)args->ref,
+                           (const int32_t*)args->table, path, n_path, room})
+    if (!lens_out || lens_out == x)  // (the token movers read these while the lengths are written)
+      return fxb::set_error(FXB_EINVAL, "fxb_kv_commit: lens_out must be an array of its own");
   if (!(c.err = fxb::dev_error_ptr())) return FXB_ECUDA;
   int64_t gx = 0;
   if (path) {

@@ -173,7 +173,8 @@ def kv_commit(k, v, page_table, n_pages, lens, ref, path, n_path, room=None, out
     the returned lengths are lens + n_path, and rows with room[s] > 0 are given
     pages for that many slots behind the new length: the lowest-numbered free
     ones, rows in order, none at all if the pool does not have enough.
-    page_table, n_pages and ref are updated in place, lens is not.
+    page_table, n_pages and ref are updated in place, lens is not; `out`, where
+    given, receives the lengths and is none of the other arguments.
     """
     r = _native().kv_commit(k, v, page_table, n_pages, lens, ref, path, n_path, room, out, 0)
     if r is None:

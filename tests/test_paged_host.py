@@ -281,3 +281,13 @@ def test_gemm_workspaces_of_plain_captures_are_their_own(monkeypatch, allocation
     assert [x for what, x in allocations if what == "zero"] == [first, second]
     with ops.graph_workspaces({}):
         assert ops._gemm_workspace(device) is ops._gemm_workspace(device)
+
+
+def test_commit_refuses_lengths_written_over_its_arguments(lib):
+    a = kv_args()
+    a.n_pages, a.ref, a.table = 1024, 2048, 4096
+    path, n_path, room = (ctypes.c_void_p(x) for x in (512, 768, 8192))
+    for out in (256, 1024, 2048, 4096, 512, 768, 8192):
+        assert lib.fxb_kv_commit(ctypes.byref(a), path, 4, 4, n_path, room, ctypes.c_void_p(out), None) == -1
+        assert "lens_out" in err()
+    assert lib.fxb_kv_commit(ctypes.byref(a), path, 4, 4, n_path, room, None, None) == -1 and "lens_out" in err()
