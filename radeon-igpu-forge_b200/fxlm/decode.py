@@ -134,7 +134,8 @@ class DecodeStep:
 
     def __call__(self, trees, u):
         """Accepted node indices and the next token of every slot: a list of
-        (path, next), ([], -1) where the tree is empty. u (slots, nodes) fp32."""
+        (path, next), ([], -1) where the tree is empty; next is -1 too where the
+        model's probabilities are (NaN logits). u (slots, nodes) fp32."""
         self.x.copy_(_pack(trees, self.T))
         self.u.copy_(u)
         self.calls += 1
@@ -229,6 +230,10 @@ def generate_cached(model, ids, max_new, temperature=0.8, top_k=50, generator=No
             u = torch.rand(samples, draft + 1, device=dev, generator=generator)
             for s, (t, _), (path, nxt) in zip(seqs, trees, step(trees, u)):
                 if path:
+                    if nxt < 0:
+                        cache.check()
+                        raise RuntimeError("generate_cached: the model's probabilities of the next token are empty "
+                                           "(NaN or infinite logits)")
                     s.extend([t[i] for i in path[1:]] + [nxt])
                     given += len(path)
             steps += 1

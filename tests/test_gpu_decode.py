@@ -115,3 +115,12 @@ def test_sample_command(dev, tmp_path):
     assert sample.main(args) == sample.main(args + ["--draft", "4"])
     two = sample.main(args + ["--draft", "4", "--num-samples", "2"])
     assert two == "\n".join([sample.main(args)] * 2)
+
+
+def test_logits_without_probabilities_raise(dev):
+    from fxlm import generate_cached
+    m = model_of(dev, torch.float32)
+    with torch.no_grad():
+        m.lnf_w.fill_(float("nan"))
+    with pytest.raises(RuntimeError, match="probabilit"):
+        generate_cached(m, torch.tensor([3, 1, 4], device=dev), 6, draft=2, samples=2)
