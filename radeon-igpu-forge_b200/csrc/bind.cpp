@@ -12,6 +12,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/object_ptr.h>
 
+#include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
 #include <c10/cuda/CUDAStream.h>
@@ -107,6 +108,9 @@ PyObject* tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (t[i]->dim() != 4 || t[i]->scalar_type() != type || !t[i]->is_cuda() || t[i]->stride(3) != 1) Py_RETURN_NONE;
   const auto s = q.sizes(), sp = t[3]->sizes();
   const int64_t B = s[0], T = s[1], Hq = s[2], D = s[3], Hkv = t[1]->size(2), page = sp[2];
+  if (at::GradMode::is_enabled())  // no backward pass: a result without one would cut gradients silently
+    for (int i = 0; i < 5; ++i)
+      if (t[i]->requires_grad()) Py_RETURN_NONE;
   const int64_t node_shape[4] = {B, T, Hkv, D}, page_shape[4] = {sp[0], Hkv, page, D};
   if ((D != 64 && D != 128) || T > kMaxNodes || Hkv < 1 || Hq % Hkv || t[1]->sizes() != at::IntArrayRef(node_shape) ||
       t[2]->sizes() != at::IntArrayRef(node_shape) || sp != at::IntArrayRef(page_shape) || t[4]->sizes() != sp)

@@ -63,7 +63,7 @@ def tree_logits(model, cache, tokens, n_nodes, mask, depth):
     continue the sequences of `cache`: tokens, mask, depth (S, T) int64 (what
     each node sees, see tree_masks, and its distance from the root), n_nodes
     (S,) int32. Writes the nodes' keys and values behind the sequences
-    (cache.reserve first)."""
+    (cache.reserve first). Not differentiable: call it under torch.no_grad()."""
     cfg = model.cfg
     if cfg.linear_impl != "fused":
         raise ValueError("tree_logits needs linear_impl='fused'")
@@ -124,6 +124,7 @@ class DecodeStep:
         self.u = torch.zeros(cache.slots, nodes, device=dev)
         self.calls, self.graph, self.out, self._ws = 0, None, None, {}
 
+    @torch.no_grad()
     def _run(self):
         tokens, parents, n, mask, depth = _unpack(self.x)
         self.cache.reserve(n)

@@ -93,6 +93,9 @@ def _refuse_tree(q, k, v, kp, vp, page_table, ctx_lens, n_nodes, tree_mask, out)
         raise ValueError(f"pages must share (P,{Hkv},page,{D}): {tuple(kp.shape)} {tuple(vp.shape)}")
     if not (q.is_cuda and k.is_cuda and v.is_cuda and kp.is_cuda and vp.is_cuda):
         raise TypeError("q, k, v and the pages must be cuda tensors")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, kp, vp)):
+        raise ValueError("tree_attention has no backward pass: call it under torch.no_grad(), or with tensors that "
+                         "require no gradient")
     _refuse_table(page_table)
     if page_table.shape[0] != B:
         raise ValueError(f"page_table has {page_table.shape[0]} rows for a batch of {B}")
@@ -118,7 +121,9 @@ def tree_attention(q, k, v, k_pages, v_pages, page_table, ctx_lens, n_nodes, tre
     in tree_mask[b, t] (int64). k and v of the nodes j < n_nodes[b] are written
     to the slots ctx_lens[b] + j, which the row has to hold (kv_reserve or
     kv_commit's room). Rows t >= n_nodes[b], and rows that see nothing, are
-    zeros. T <= 64, D 64 or 128, bf16 / fp16 / fp32.
+    zeros. T <= 64, D 64 or 128, bf16 / fp16 / fp32; scale (1 / sqrt(D) by
+    default) positive. There is no backward pass: tensors that require a
+    gradient are refused while gradients are enabled.
     """
     o = _native().tree_attention(q, k, v, k_pages, v_pages, page_table, ctx_lens, n_nodes, tree_mask, scale, out)
     if o is None:

@@ -124,3 +124,19 @@ def test_logits_without_probabilities_raise(dev):
         m.lnf_w.fill_(float("nan"))
     with pytest.raises(RuntimeError, match="probabilit"):
         generate_cached(m, torch.tensor([3, 1, 4], device=dev), 6, draft=2, samples=2)
+
+
+def test_gradients_are_not_cut_silently(dev):
+    # a decoding step works with gradients enabled; logits that would carry a graph without attention are refused
+    from fxlm.decode import DecodeStep, PagedKVCache, tree_batch, tree_logits
+    m = model_of(dev, torch.float32)
+    cache = PagedKVCache(3, 2, 64, 1, 160, dev, torch.float32)
+    tok, par, n, mask, depth = tree_batch([([1, 2], [-1, 0])], dev)
+    cache.reserve(n)
+    with pytest.raises(ValueError, match="no_grad"):
+        tree_logits(m, cache, tok, n, mask, depth)
+    step = DecodeStep(m, cache, 2, 1.0, 1)
+    for _ in range(4):
+        (path, nxt), = step([([1], [-1])], torch.zeros(1, 2, device=dev))
+        assert path == [0] and nxt >= 0
+    cache.check()

@@ -850,3 +850,15 @@ def test_commit_moves_what_fits_of_a_path(dev):
         same(c, want, got)
         with pytest.raises(RuntimeError, match="KV cache"):
             _lib.raise_on_device_error()
+
+
+def test_attention_refuses_inputs_that_need_a_gradient(dev):
+    from fxlm import tree_attention
+    a = make(dev, BF16, 1, 3, 4, 4, 64, [40], 16, seed=9)
+    want = tree_attention(**a).clone()
+    for name in ("q", "k", "v", "k_pages", "v_pages"):
+        b = dict(a, **{name: a[name].detach().clone().requires_grad_()})
+        with pytest.raises(ValueError, match="gradient"):
+            tree_attention(**b)
+        with torch.no_grad():
+            assert torch.equal(tree_attention(**b), want)
