@@ -46,9 +46,12 @@ bool ints(std::initializer_list<int64_t> sizes) {  // the C structs take 32 bits
 
 const at::Tensor* tensor(PyObject* x) { return THPVariable_Check(x) ? &THPVariable_Unpack(x) : nullptr; }
 
-// a contiguous int32 tensor of this shape on the GPU
-int32_t* i32(const at::Tensor* t, at::IntArrayRef shape) {
-  if (!t || t->scalar_type() != at::kInt || !t->is_cuda() || t->sizes() != shape || !t->is_contiguous()) return nullptr;
+// on the GPU of this index: a kernel runs on one, and would take another's address for its own
+bool on(const at::Tensor& t, int64_t device) { return t.is_cuda() && t.get_device() == device; }
+
+// a contiguous int32 tensor of this shape on this GPU
+int32_t* i32(const at::Tensor* t, at::IntArrayRef shape, int64_t device) {
+  if (!t || t->scalar_type() != at::kInt || !on(*t, device) || t->sizes() != shape || !t->is_contiguous()) return nullptr;
   return static_cast<int32_t*>(t->data_ptr());
 }
 
@@ -56,8 +59,8 @@ struct Table {
   int32_t* p;
   int64_t rows, entries, stride;
 };
-bool table(const at::Tensor* t, Table* out) {
-  if (!t || t->scalar_type() != at::kInt || !t->is_cuda() || t->dim() != 2 || t->stride(1) != 1) return false;
+bool table(const at::Tensor* t, Table* out, int64_t device) {
+  if (!t || t->scalar_type() != at::kInt || !on(*t, device) || t->dim() != 2 || t->stride(1) != 1) return false;
   *out = {static_cast<int32_t*>(t->data_ptr()), t->size(0), t->size(1), t->size(0) > 1 ? t->stride(0) : t->size(1)};
   return true;
 }
@@ -104,8 +107,9 @@ PyObject* tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const auto type = q.scalar_type();
   const int code = dtype_code(type);
   if (code < 0) Py_RETURN_NONE;
+  const int64_t dev = q.get_device();
   for (int i = 0; i < 5; ++i)
-    if (t[i]->dim() != 4 || t[i]->scalar_type() != type || !t[i]->is_cuda() || t[i]->stride(3) != 1) Py_RETURN_NONE;
+    if (t[i]->dim() != 4 || t[i]->scalar_type() != type || !on(*t[i], dev) || t[i]->stride(3) != 1) Py_RETURN_NONE;
   const auto s = q.sizes(), sp = t[3]->sizes();
   const int64_t B = s[0], T = s[1], Hq = s[2], D = s[3], Hkv = t[1]->size(2), page = sp[2];
   if (at::GradMode::is_enabled())  // no backward pass: a result without one would cut gradients silently
@@ -117,8 +121,8 @@ PyObject* tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Py_RETURN_NONE;
   Table tab;
   const int64_t rows[1] = {B};
-  const int32_t *lens = i32(t[6], rows), *nodes = i32(t[7], rows);
-  if (!table(t[5], &tab) || tab.rows != B || mask.scalar_type() != at::kLong || !mask.is_cuda() || mask.dim() != 2 ||
+  const int32_t *lens = i32(t[6], rows, dev), *nodes = i32(t[7], rows, dev);
+  if (!table(t[5], &tab, dev) || tab.rows != B || mask.scalar_type() != at::kLong || !on(mask, dev) || mask.dim() != 2 ||
       mask.size(0) != B || mask.size(1) != T || (T > 1 && mask.stride(1) != 1))
     Py_RETURN_NONE;
   if ((B && (!lens || !nodes)) || !ints({B, Hq, page, sp[0], tab.entries})) Py_RETURN_NONE;
@@ -129,7 +133,7 @@ PyObject* tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     out = at::empty(s, q.options());
   } else {
     const at::Tensor* o = tensor(a[10]);
-    if (!o || o->sizes() != s || o->scalar_type() != type || !o->is_cuda() || o->stride(3) != 1) Py_RETURN_NONE;
+    if (!o || o->sizes() != s || o->scalar_type() != type || !on(*o, dev) || o->stride(3) != 1) Py_RETURN_NONE;
     out = *o;
   }
   if (B && T) {
@@ -164,7 +168,7 @@ PyObject* tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     x.mask_sb = B > 1 ? mask.stride(0) : T;
     const cudaStream_t stream = stream_of(q);
     const size_t bytes = lib.tree_attn_workspace(code, x.B, x.T, x.Hq, x.Hkv, x.D);
-    THPObjectPtr device(PyLong_FromLong(q.get_device())), handle(PyLong_FromVoidPtr(stream)),
+    THPObjectPtr device(PyLong_FromLong(dev)), handle(PyLong_FromVoidPtr(stream)),
         size(PyLong_FromSize_t(bytes)),
         zeroed(PyLong_FromSize_t(lib.tree_attn_zeroed(code, x.B, x.T, x.Hq, x.Hkv, x.D)));
     PyObject* const w[5] = {tree_kind, device.get(), handle.get(), size.get(), zeroed.get()};
@@ -191,15 +195,15 @@ PyObject* verify_tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Py_RETURN_NONE;
   const int64_t B = tokens.size(0), T = tokens.size(1), V = p.size(2);
   if (T < 1 || T > kMaxNodes || !ints({B, V})) Py_RETURN_NONE;
-  const int64_t shape[3] = {B, T, V}, rows[1] = {B};
+  const int64_t shape[3] = {B, T, V}, rows[1] = {B}, dev = tokens.get_device();
   const at::IntArrayRef nodes(shape, 2);
   for (const at::Tensor* x : {t[3], t[5]})
-    if (x && (x->scalar_type() != at::kFloat || !x->is_cuda() || x->sizes() != at::IntArrayRef(shape) ||
+    if (x && (x->scalar_type() != at::kFloat || !on(*x, dev) || x->sizes() != at::IntArrayRef(shape) ||
               (V > 1 && x->stride(2) != 1)))
       Py_RETURN_NONE;
-  const int32_t *parents = i32(t[1], nodes), *count = i32(t[2], rows);
+  const int32_t *parents = i32(t[1], nodes, dev), *count = i32(t[2], rows, dev);
   if (B && (!parents || !count)) Py_RETURN_NONE;
-  if (u.scalar_type() != at::kFloat || !u.is_cuda() || u.sizes() != nodes || !u.is_contiguous()) Py_RETURN_NONE;
+  if (u.scalar_type() != at::kFloat || !on(u, dev) || u.sizes() != nodes || !u.is_contiguous()) Py_RETURN_NONE;
   at::Tensor path = at::empty_like(*t[1]), n_path = at::empty_like(*t[2]), next = at::empty(rows, tokens.options());
   if (B) {
     const cudaStream_t stream = stream_of(tokens);
@@ -222,7 +226,9 @@ bool cache(PyObject* const* a, int page, fxb_kv_args* x, const at::Tensor** lens
   Table tab;
   const at::Tensor* ref = tensor(a[5]);
   *lens = tensor(a[4]);
-  if (!table(tensor(a[2]), &tab) || !ref || ref->dim() != 1 || !ints({tab.rows, tab.entries, ref->size(0)})) return false;
+  const at::Tensor* pages = tensor(a[2]);
+  const int64_t dev = pages ? pages->get_device() : -1;
+  if (!table(pages, &tab, dev) || !ref || ref->dim() != 1 || !ints({tab.rows, tab.entries, ref->size(0)})) return false;
   const int64_t S[1] = {tab.rows}, P[1] = {ref->size(0)};
   *x = {};
   x->S = (int)tab.rows;
@@ -231,15 +237,15 @@ bool cache(PyObject* const* a, int page, fxb_kv_args* x, const at::Tensor** lens
   x->page = page;
   x->table = tab.p;
   x->table_ss = tab.stride;
-  x->n_pages = i32(tensor(a[3]), S);
-  x->lens = i32(*lens, S);
-  x->ref = i32(ref, P);
+  x->n_pages = i32(tensor(a[3]), S, dev);
+  x->lens = i32(*lens, S, dev);
+  x->ref = i32(ref, P, dev);
   if (S[0] && (!x->n_pages || !x->lens)) return false;
   if (P[0] && !x->ref) return false;
   if (a[0] == Py_None) return true;
   const at::Tensor *k = tensor(a[0]), *v = tensor(a[1]);
   if (!k || !v || k->dim() != 5 || v->sizes() != k->sizes() || k->size(1) != P[0] || dtype_code(k->scalar_type()) < 0 ||
-      v->scalar_type() != k->scalar_type() || !k->is_cuda() || !v->is_cuda() || k->stride(4) != 1 || v->stride(4) != 1)
+      v->scalar_type() != k->scalar_type() || !on(*k, dev) || !on(*v, dev) || k->stride(4) != 1 || v->stride(4) != 1)
     return false;
   x->elem_size = (int)k->element_size();
   x->L = (int)k->size(0);
@@ -262,24 +268,24 @@ PyObject* kv_commit(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const long page = PyLong_AsLong(a[10]);
   if (page == -1 && PyErr_Occurred()) return nullptr;
   if (!cache(a, (int)page, &x, &lens)) Py_RETURN_NONE;
-  const int64_t S[1] = {x.S};
+  const int64_t S[1] = {x.S}, dev = lens->get_device();
   const int32_t *path = nullptr, *n_path = nullptr, *room = nullptr;
   int64_t T = 0;
   if (a[6] != Py_None) {
     const at::Tensor* t = tensor(a[6]);
     if (!t || t->dim() != 2 || (T = t->size(1)) < 1 || T > kMaxNodes) Py_RETURN_NONE;
     const int64_t shape[2] = {S[0], T};
-    path = i32(t, shape);
-    n_path = i32(tensor(a[7]), S);
+    path = i32(t, shape, dev);
+    n_path = i32(tensor(a[7]), S, dev);
     if (S[0] && (!path || !n_path)) Py_RETURN_NONE;
   }
-  if (a[8] != Py_None && !(room = i32(tensor(a[8]), S)) && S[0]) Py_RETURN_NONE;
+  if (a[8] != Py_None && !(room = i32(tensor(a[8]), S, dev)) && S[0]) Py_RETURN_NONE;
   at::Tensor out;
   if (a[9] == Py_None) {
     out = at::empty_like(*lens);
   } else {
     const at::Tensor* o = tensor(a[9]);
-    if (!o || (!i32(o, S) && S[0])) Py_RETURN_NONE;
+    if (!o || (!i32(o, S, dev) && S[0])) Py_RETURN_NONE;
     out = *o;
   }
   if (S[0]) {
@@ -300,7 +306,7 @@ PyObject* kv_fork(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const at::Tensor* lens;
   if (!cache(a, 0, &x, &lens)) Py_RETURN_NONE;
   const int64_t S[1] = {x.S};
-  const int32_t* parents = i32(tensor(a[6]), S);
+  const int32_t* parents = i32(tensor(a[6]), S, lens->get_device());
   if (S[0] && !parents) Py_RETURN_NONE;
   if (S[0]) {
     const int64_t words[1] = {(int64_t)((lib.kv_fork_workspace(x.S, x.W) + 3) / 4)};

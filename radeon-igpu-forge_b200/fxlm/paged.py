@@ -51,6 +51,12 @@ def _refuse_i32(t, name, shape):
         raise ValueError(f"{name} must be contiguous {shape}, got {tuple(t.shape)}")
 
 
+def _refuse_devices(first, **others):
+    for name, t in others.items():
+        if t is not None and t.device != first.device:
+            raise ValueError(f"{name} is on {t.device}, other arguments on {first.device}")
+
+
 def _refuse_table(t):
     if t.dtype != torch.int32 or not t.is_cuda:
         raise TypeError(f"page_table must be a cuda int32 tensor, got {t.dtype} on {t.device}")
@@ -107,6 +113,8 @@ def _refuse_tree(q, k, v, kp, vp, page_table, ctx_lens, n_nodes, tree_mask, out)
         raise ValueError(f"out must be {(B, T, Hq, D)} {dt} on the GPU")
     _refuse_i32(ctx_lens, "ctx_lens", (B,))
     _refuse_i32(n_nodes, "n_nodes", (B,))
+    _refuse_devices(q, k=k, v=v, k_pages=kp, v_pages=vp, page_table=page_table, ctx_lens=ctx_lens, n_nodes=n_nodes,
+                    tree_mask=tree_mask, out=out)
     raise ValueError("the last axis of every tensor must be contiguous")
 
 
@@ -142,6 +150,7 @@ def _refuse_cache(k, v, page_table, n_pages, lens, ref):
     P = ref.shape[0]
     for t, name, n in ((n_pages, "n_pages", S), (lens, "lens", S), (ref, "ref", P)):
         _refuse_i32(t, name, (n,))
+    _refuse_devices(page_table, n_pages=n_pages, lens=lens, ref=ref, k=k, v=v)
     if k is None:
         return S
     if k.dim() != 5 or v.shape != k.shape or k.shape[1] != P:
@@ -167,6 +176,7 @@ def _refuse_commit(k, v, page_table, n_pages, lens, ref, path, n_path, room, out
     for t, name in ((room, "room"), (out, "out")):
         if t is not None:
             _refuse_i32(t, name, (S,))
+    _refuse_devices(page_table, path=path, n_path=n_path, room=room, out=out)
     raise ValueError("sizes of 2^31 and more")
 
 
@@ -208,6 +218,7 @@ def kv_fork(k, v, page_table, n_pages, lens, ref, parents):
     r = _native().kv_fork(k, v, page_table, n_pages, lens, ref, parents)
     if r is None:
         _refuse_i32(parents, "parents", (_refuse_cache(k, v, page_table, n_pages, lens, ref),))
+        _refuse_devices(page_table, parents=parents)
         raise ValueError("sizes of 2^31 and more")
     if type(r) is int:
         _lib.check(r, "fxb_kv_fork")

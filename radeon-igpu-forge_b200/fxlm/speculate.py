@@ -2,7 +2,7 @@
 import torch
 
 from fxb200 import _lib
-from .paged import MAX_NODES, _native, _refuse_i32
+from .paged import MAX_NODES, _native, _refuse_devices, _refuse_i32
 
 
 def _refuse(tokens, parents, n_nodes, target_probs, u, draft_probs):
@@ -27,6 +27,7 @@ def _refuse(tokens, parents, n_nodes, target_probs, u, draft_probs):
     _refuse_i32(n_nodes, "n_nodes", (B,))
     if u.dtype != torch.float32 or not u.is_cuda:
         raise TypeError("u must be a cuda fp32 tensor")
+    _refuse_devices(tokens, parents=parents, n_nodes=n_nodes, target_probs=target_probs, u=u, draft_probs=draft_probs)
     raise ValueError(f"u must be contiguous ({B},{T}), got {tuple(u.shape)}")
 
 

@@ -291,3 +291,31 @@ def test_commit_refuses_lengths_written_over_its_arguments(lib):
         assert lib.fxb_kv_commit(ctypes.byref(a), path, 4, 4, n_path, room, ctypes.c_void_p(out), None) == -1
         assert "lens_out" in err()
     assert lib.fxb_kv_commit(ctypes.byref(a), path, 4, 4, n_path, room, None, None) == -1 and "lens_out" in err()
+
+
+@pytest.mark.filterwarnings("ignore:Accessing the data pointer")
+def test_arguments_on_several_devices_are_refused():
+    # tensors without storage stand in for those of two GPUs: one argument on the other GPU at a time
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from fxlm import kv_commit, kv_fork, kv_reserve, tree_attention, verify_tree
+    bf, i32, i64, f32 = torch.bfloat16, torch.int32, torch.int64, torch.float32
+
+    def refused(fn, shapes, **kw):
+        for odd in shapes:
+            args = {n: torch.empty(*s, dtype=d, device="cuda:1" if n == odd else "cuda:0") for n, (s, d) in shapes.items()}
+            with pytest.raises(ValueError, match="cuda:1"):
+                fn(**args, **kw)
+
+    cache = dict(page_table=((1, 4), i32), n_pages=((1,), i32), lens=((1,), i32), ref=((4,), i32))
+    pools = dict(k=((2, 4, 2, 16, 64), bf), v=((2, 4, 2, 16, 64), bf))
+    with FakeTensorMode():
+        refused(tree_attention, dict(
+            q=((1, 2, 4, 64), bf), k=((1, 2, 2, 64), bf), v=((1, 2, 2, 64), bf), k_pages=((4, 2, 16, 64), bf),
+            v_pages=((4, 2, 16, 64), bf), page_table=((1, 4), i32), ctx_lens=((1,), i32), n_nodes=((1,), i32),
+            tree_mask=((1, 2), i64), out=((1, 2, 4, 64), bf)))
+        refused(verify_tree, dict(
+            tokens=((1, 2), i64), parents=((1, 2), i32), n_nodes=((1,), i32), target_probs=((1, 2, 8), f32),
+            u=((1, 2), f32), draft_probs=((1, 2, 8), f32)))
+        refused(kv_commit, dict(**pools, **cache, path=((1, 2), i32), n_path=((1,), i32), room=((1,), i32), out=((1,), i32)))
+        refused(kv_reserve, dict(**cache, room=((1,), i32)), page=16)
+        refused(kv_fork, dict(**pools, **cache, parents=((1,), i32)))
