@@ -385,7 +385,7 @@ typedef struct fxb_tree_attn_args {
   const int32_t* table; int64_t table_sb;              /* (B,W) */
   const int32_t* lens;                                 /* (B,) */
   const int32_t* n_nodes;                              /* (B,) in [0,T] */
-  const int64_t* mask; int64_t mask_sb;                /* (B,T) */
+  const int64_t* mask; int64_t mask_sb;                /* (B,T); mask_sb 0: one tree for all rows */
   void* workspace; int64_t workspace_bytes;            /* fxb_tree_attn_workspace bytes */
 } fxb_tree_attn_args;
 

@@ -785,7 +785,8 @@ int fxb_tree_attn(const fxb_tree_attn_args* a, void* stream) {
   for (int s = 4; s <= 8; ++s)
     if (a->page == 1 << s) shift = s;
   if (!shift) return fxb::set_error(FXB_EINVAL, "fxb_tree_attn: page %d (16, 32, 64, 128 or 256)", a->page);
-  if (a->P < 1 || a->W < 1 || a->table_sb < a->W || a->mask_sb < a->T)
+  // a mask's row stride of 0: one tree for all batch rows (a table's would put all rows' nodes into the same slots)
+  if (a->P < 1 || a->W < 1 || a->table_sb < a->W || (a->mask_sb < a->T && a->mask_sb != 0))
     return fxb::set_error(FXB_EINVAL, "fxb_tree_attn: P=%d W=%d, or a row stride of table or mask too small", a->P,
                           a->W);
   const void* ptr[6] = {a->q, a->k, a->v, a->o, a->k_pages, a->v_pages};

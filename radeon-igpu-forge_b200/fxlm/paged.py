@@ -126,10 +126,10 @@ def tree_attention(q, k, v, k_pages, v_pages, page_table, ctx_lens, n_nodes, tre
     k_pages, v_pages (P, Hkv, page, D) of one layer: views with unit stride on
     D (slices of a fused projection need no copy). Node t of row b sees the
     cache slots [0, ctx_lens[b]) and the nodes j < n_nodes[b] whose bit is set
-    in tree_mask[b, t] (int64). k and v of the nodes j < n_nodes[b] are written
-    to the slots ctx_lens[b] + j, which the row has to hold (kv_reserve or
-    kv_commit's room). Rows t >= n_nodes[b], and rows that see nothing, are
-    zeros. T <= 64, D 64 or 128, bf16 / fp16 / fp32; scale (1 / sqrt(D) by
+    in tree_mask[b, t] (int64; one tree for all rows: tree_mask.expand(B, T)).
+    k and v of the nodes j < n_nodes[b] are written to the slots
+    ctx_lens[b] + j, which the row has to hold (kv_reserve or kv_commit's room).
+    Rows t >= n_nodes[b], and rows that see nothing, are zeros. T <= 64, D 64 or 128, bf16 / fp16 / fp32; scale (1 / sqrt(D) by
     default) positive. There is no backward pass: tensors that require a
     gradient are refused while gradients are enabled.
     """

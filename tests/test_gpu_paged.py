@@ -862,3 +862,12 @@ def test_attention_refuses_inputs_that_need_a_gradient(dev):
             tree_attention(**b)
         with torch.no_grad():
             assert torch.equal(tree_attention(**b), want)
+
+
+@pytest.mark.parametrize("T,dtype", [(2, BF16), (2, F32), (24, BF16)])
+def test_attention_one_tree_for_all_rows(dev, T, dtype):
+    from fxlm import tree_attention
+    a = make(dev, dtype, 5, T, 4, 2, 64, [30, 0, 7, 200, 64], 16, seed=4)
+    one = a["tree_mask"][1:2]
+    want = check(dict(a, tree_mask=one.repeat(5, 1))).clone()
+    assert torch.equal(tree_attention(**dict(a, tree_mask=one.expand(5, T))), want)

@@ -319,3 +319,10 @@ def test_arguments_on_several_devices_are_refused():
         refused(kv_commit, dict(**pools, **cache, path=((1, 2), i32), n_path=((1,), i32), room=((1,), i32), out=((1,), i32)))
         refused(kv_reserve, dict(**cache, room=((1,), i32)), page=16)
         refused(kv_fork, dict(**pools, **cache, parents=((1,), i32)))
+
+
+def test_tree_attn_takes_one_mask_for_all_rows(lib):
+    # (a row stride of 0 passes; the next check, of the workspace, stops the call here)
+    assert lib.fxb_tree_attn(ctypes.byref(tree_args(B=3, mask_sb=0)), None) == -1 and "workspace" in err()
+    for kw in (dict(mask_sb=-4), dict(table_sb=0)):
+        assert lib.fxb_tree_attn(ctypes.byref(tree_args(B=3, **kw)), None) == -1 and "row stride" in err()
