@@ -375,7 +375,8 @@ typedef struct fxb_tree_attn_args {
   int32_t B, T, Hq, Hkv, D; /* T <= 64; Hq a multiple of Hkv; D = 64 or 128 */
   int32_t page, P, W;       /* slots per page, pages of the pool, entries of a table row */
   float scale;
-  /* element strides, unit stride on D; strides multiples of 16 bytes, 16-byte aligned bases */
+  /* element strides, unit stride on D; strides multiples of 16 bytes (that of an axis of one entry may be
+   * anything), 16-byte aligned bases */
   const void* q; int64_t q_sb, q_st, q_sh;             /* (B,T,Hq,D) */
   const void* k; int64_t k_sb, k_st, k_sh;             /* (B,T,Hkv,D) */
   const void* v; int64_t v_sb, v_st, v_sh;

@@ -376,9 +376,11 @@ int params(const char* fn, const fxb_kv_args* a, bool pools, KvParams* c) {
       return fxb::set_error(FXB_EINVAL, "%s: L=%d H=%d D=%d (rows of a multiple of 16 bytes)", fn, a->L, a->H, a->D);
     if (!a->k || !a->v || !fxb::aligned16(a->k) || !fxb::aligned16(a->v))
       return fxb::set_error(FXB_EINVAL, "%s: k and v must be 16-byte aligned", fn);
-    const int64_t st[8] = {a->k_sl, a->k_sp, a->k_sh, a->k_st, a->v_sl, a->v_sp, a->v_sh, a->v_st};
-    for (int64_t x : st)
-      if (x < 0 || (x * e) % 16)
+    const struct { int64_t entries, stride; } st[8] = {  // the stride of an axis of one entry is not used
+        {a->L, a->k_sl}, {a->P, a->k_sp}, {a->H, a->k_sh}, {a->page, a->k_st},
+        {a->L, a->v_sl}, {a->P, a->v_sp}, {a->H, a->v_sh}, {a->page, a->v_st}};
+    for (const auto& x : st)
+      if (x.entries > 1 && (x.stride < 0 || (x.stride * e) % 16))
         return fxb::set_error(FXB_EINVAL, "%s: strides must be multiples of 16 bytes", fn);
     c->k = {static_cast<uint8_t*>(a->k), a->k_sl * e, a->k_sp * e, a->k_sh * e, a->k_st * e};
     c->v = {static_cast<uint8_t*>(a->v), a->v_sl * e, a->v_sp * e, a->v_sh * e, a->v_st * e};

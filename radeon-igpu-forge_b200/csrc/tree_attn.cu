@@ -795,10 +795,12 @@ int fxb_tree_attn(const fxb_tree_attn_args* a, void* stream) {
       return fxb::set_error(FXB_EINVAL, "fxb_tree_attn: q, k, v, o and the pages must be 16-byte aligned");
   if (!a->table || !a->lens || !a->n_nodes || !a->mask)
     return fxb::set_error(FXB_EINVAL, "fxb_tree_attn: table, lens, n_nodes or mask is NULL");
-  const int64_t st[18] = {a->q_sb, a->q_st, a->q_sh, a->k_sb, a->k_st, a->k_sh, a->v_sb, a->v_st, a->v_sh,
-                          a->o_sb, a->o_st, a->o_sh, a->kp_sp, a->kp_sh, a->kp_st, a->vp_sp, a->vp_sh, a->vp_st};
-  for (int64_t s : st)
-    if (s < 0 || (s * e) % 16)
+  const struct { int64_t entries, stride; } st[18] = {  // the stride of an axis of one entry is not used
+      {a->B, a->q_sb}, {a->T, a->q_st}, {a->Hq, a->q_sh}, {a->B, a->k_sb}, {a->T, a->k_st}, {a->Hkv, a->k_sh},
+      {a->B, a->v_sb}, {a->T, a->v_st}, {a->Hkv, a->v_sh}, {a->B, a->o_sb}, {a->T, a->o_st}, {a->Hq, a->o_sh},
+      {a->P, a->kp_sp}, {a->Hkv, a->kp_sh}, {a->page, a->kp_st}, {a->P, a->vp_sp}, {a->Hkv, a->vp_sh}, {a->page, a->vp_st}};
+  for (const auto& s : st)
+    if (s.entries > 1 && (s.stride < 0 || (s.stride * e) % 16))
       return fxb::set_error(FXB_EINVAL, "fxb_tree_attn: strides must be multiples of 16 bytes");
   if (!(a->scale > 0.f) || !(a->scale < INFINITY))
     return fxb::set_error(FXB_EINVAL, "fxb_tree_attn: scale must be positive and finite");

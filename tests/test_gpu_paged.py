@@ -871,3 +871,35 @@ def test_attention_one_tree_for_all_rows(dev, T, dtype):
     one = a["tree_mask"][1:2]
     want = check(dict(a, tree_mask=one.repeat(5, 1))).clone()
     assert torch.equal(tree_attention(**dict(a, tree_mask=one.expand(5, T))), want)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_attention_strides_of_single_entries(dev, dtype):
+    # one batch row, one node, one key head: the strides of those axes are not used and may be anything
+    from fxlm import tree_attention
+    for T, Hq, P in ((1, 4, 3), (1, 24, 3)):
+        a = make(dev, dtype, 1, T, Hq, 1, 64, [30], 32, seed=4, layout="nhd")
+        want = tree_attention(**a).clone()
+
+        def odd(t, *strides):
+            return t.as_strided(t.shape, strides)
+
+        b = dict(a, q=odd(a["q"], 7, 3, 64, 1), k=odd(a["k"], 5, 3, 1, 1), v=odd(a["v"], 3, 5, 7, 1))
+        for name in ("k_pages", "v_pages"):
+            b[name] = odd(a[name], a[name].stride(0), 3, 64, 1)
+        assert torch.equal(tree_attention(**b), want)
+
+
+def test_commit_strides_of_single_entries(dev):
+    from fxlm import kv_commit, kv_fork
+    c = cache(dev, BF16, 2, 1, 1, 64, 16, [5, 9], 4, seed=1)
+    want = PlainPages(c)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    args = (c["table"], c["n_pages"], c["lens"], c["ref"])
+    k, v = (x.as_strided(x.shape, (7, x.stride(1), 3, 64, 1)) for x in (c["k"], c["v"]))
+    assert want.commit([[1, 3], [0, 2]], [2, 2], [0, 0])
+    c["lens"].copy_(kv_commit(k, v, *args, i32([[1, 3, -1, -1], [0, 2, -1, -1]]), i32([2, 2])))
+    same(c, want, c["lens"])
+    assert want.fork([1, 1])
+    kv_fork(k, v, *args, i32([1, 1]))
+    same(c, want, c["lens"])

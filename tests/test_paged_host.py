@@ -326,3 +326,12 @@ def test_tree_attn_takes_one_mask_for_all_rows(lib):
     assert lib.fxb_tree_attn(ctypes.byref(tree_args(B=3, mask_sb=0)), None) == -1 and "workspace" in err()
     for kw in (dict(mask_sb=-4), dict(table_sb=0)):
         assert lib.fxb_tree_attn(ctypes.byref(tree_args(B=3, **kw)), None) == -1 and "row stride" in err()
+
+
+def test_strides_of_single_entries_may_be_anything(lib):
+    odd = {f"{n}_{s}": 7 for n in ("q", "k", "v", "o") for s in ("sb", "st", "sh")}
+    a = tree_args(T=1, Hq=1, Hkv=1, P=1, **odd, kp_sp=3, kp_sh=-5, vp_sp=9, vp_sh=1)
+    assert lib.fxb_tree_attn(ctypes.byref(a), None) == -1 and "workspace" in err()
+    p = ctypes.c_void_p(512)
+    k = kv_args(L=1, P=1, H=1, k_sl=7, k_sp=3, k_sh=1, v_sl=-9, v_sp=5, v_sh=3)
+    assert lib.fxb_kv_fork(ctypes.byref(k), p, ctypes.c_void_p(8), None) == -1 and "workspace" in err()
