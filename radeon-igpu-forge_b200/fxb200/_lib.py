@@ -20,6 +20,7 @@ _PKG_ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 LIB_PATH = os.environ.get("FXB200_LIB", os.path.join(_PKG_ROOT, "lib", "libfxb200.so"))
 
 FXB_OK = 0
+FXB_EINVAL = -1
 DTYPE_CODE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 EPI_STORE, EPI_RESIDUAL, EPI_GELU, EPI_DGELU = 0, 1, 2, 3

@@ -44,6 +44,13 @@ def _native():
     return module
 
 
+def _failed(rc, what):
+    """Raises for the library's error code: ValueError for arguments that it refuses before any launch."""
+    if rc == _lib.FXB_EINVAL:
+        raise ValueError(_lib.last_error())
+    _lib.check(rc, what)
+
+
 def _refuse_i32(t, name, shape):
     if t.dtype != torch.int32 or not t.is_cuda:
         raise TypeError(f"{name} must be a cuda int32 tensor, got {t.dtype} on {t.device}")
@@ -137,7 +144,7 @@ def tree_attention(q, k, v, k_pages, v_pages, page_table, ctx_lens, n_nodes, tre
     if o is None:
         _refuse_tree(q, k, v, k_pages, v_pages, page_table, ctx_lens, n_nodes, tree_mask, out)
     if type(o) is int:
-        _lib.check(o, "fxb_tree_attn")
+        _failed(o, "fxb_tree_attn")
     return o
 
 
@@ -195,7 +202,7 @@ def kv_commit(k, v, page_table, n_pages, lens, ref, path, n_path, room=None, out
     if r is None:
         _refuse_commit(k, v, page_table, n_pages, lens, ref, path, n_path, room, out)
     if type(r) is int:
-        _lib.check(r, "fxb_kv_commit")
+        _failed(r, "fxb_kv_commit")
     return r
 
 
@@ -206,7 +213,7 @@ def kv_reserve(page_table, n_pages, lens, ref, room, page):
     if r is None:
         _refuse_commit(None, None, page_table, n_pages, lens, ref, None, None, room, None)
     if type(r) is int:
-        _lib.check(r, "fxb_kv_commit")
+        _failed(r, "fxb_kv_commit")
 
 
 def kv_fork(k, v, page_table, n_pages, lens, ref, parents):
@@ -221,4 +228,4 @@ def kv_fork(k, v, page_table, n_pages, lens, ref, parents):
         _refuse_devices(page_table, parents=parents)
         raise ValueError("sizes of 2^31 and more")
     if type(r) is int:
-        _lib.check(r, "fxb_kv_fork")
+        _failed(r, "fxb_kv_fork")

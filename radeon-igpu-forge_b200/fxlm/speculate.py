@@ -1,8 +1,7 @@
 """fxlm.speculate: verification of drafted tokens against the target's probabilities."""
 import torch
 
-from fxb200 import _lib
-from .paged import MAX_NODES, _native, _refuse_devices, _refuse_i32
+from .paged import MAX_NODES, _failed, _native, _refuse_devices, _refuse_i32
 
 
 def _refuse(tokens, parents, n_nodes, target_probs, u, draft_probs):
@@ -53,5 +52,5 @@ def verify_tree(tokens, parents, n_nodes, target_probs, u, draft_probs=None):
     if r is None:
         _refuse(tokens, parents, n_nodes, target_probs, u, draft_probs)
     if type(r) is int:
-        _lib.check(r, "fxb_verify_tree")
+        _failed(r, "fxb_verify_tree")
     return r

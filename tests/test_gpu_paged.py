@@ -903,3 +903,33 @@ def test_commit_strides_of_single_entries(dev):
     assert want.fork([1, 1])
     kv_fork(k, v, *args, i32([1, 1]))
     same(c, want, c["lens"])
+
+
+def test_refusals_are_value_errors(dev):
+    from fxlm import kv_commit, kv_fork, kv_reserve, tree_attention, verify_tree
+    a = make(dev, BF16, 2, 3, 4, 4, 64, [40, 20], 16, seed=9)
+
+    def refused(match, **kw):
+        with pytest.raises(ValueError, match=match):
+            tree_attention(**dict(a, **kw))
+
+    pages = torch.zeros(4, 4, 24, 64, dtype=BF16, device=dev)
+    refused("page 24", k_pages=pages, v_pages=pages)
+    refused("scale", scale=-1.0)
+    refused("scale", scale=float("nan"))
+    refused("aligned", q=torch.zeros(2 * 3 * 4 * 64 + 1, dtype=BF16, device=dev)[1:].view(2, 3, 4, 64))
+    refused("strides", q=torch.zeros(2, 3, 4, 68, dtype=BF16, device=dev)[..., :64])
+    refused("row stride", tree_mask=torch.zeros(8, dtype=torch.int64, device=dev).as_strided((2, 3), (2, 1)))
+    refused("row stride", page_table=a["page_table"][:1].expand(2, -1))
+    i = torch.zeros(1, dtype=torch.int32, device=dev)
+    args = (i[:, None], i, i.clone(), torch.zeros(4, dtype=torch.int32, device=dev))
+    with pytest.raises(ValueError, match="page 24"):
+        kv_reserve(*args, i, 24)
+    k = torch.zeros(2, 4, 2, 16, 4, dtype=BF16, device=dev)
+    with pytest.raises(ValueError, match="D=4"):
+        kv_commit(k, k, *args, i[:, None], i)
+    with pytest.raises(ValueError, match="D=4"):
+        kv_fork(k, k, *args, i)
+    p = torch.zeros(1, 1, 8, device=dev)
+    with pytest.raises(ValueError, match="V=0"):
+        verify_tree(i[:, None].long(), i[:, None], i, p[..., :0], p[:, :, 0])
