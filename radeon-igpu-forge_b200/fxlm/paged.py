@@ -73,13 +73,15 @@ def _refuse_table(t):
 
 def tree_masks(parents):
     """(B, T) int64 masks of a tree given by `parents` (B, T; -1 for the root,
-    parents[b, c] < c): bit j of mask[b, c] is set for c itself and its ancestors."""
+    parents[b, c] < c): bit j of mask[b, c] is set for c itself and its ancestors.
+    A parent outside [0, c) counts as none, as in verify_tree."""
     B, T = parents.shape
     if T > MAX_NODES:
         raise ValueError(f"T={T}: at most {MAX_NODES} nodes")
     up = parents.long()
     mask = torch.ones((), dtype=torch.int64, device=parents.device) << torch.arange(T, device=parents.device)
     mask = mask.expand(B, T)
+    up = torch.where(up < torch.arange(T, device=parents.device), up, -1)
     for _ in range(max(T - 1, 0).bit_length()):  # doubling: after k steps the 2^k nearest ancestors are in
         has = up >= 0
         at = up.clamp(min=0)

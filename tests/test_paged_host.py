@@ -335,3 +335,10 @@ def test_strides_of_single_entries_may_be_anything(lib):
     p = ctypes.c_void_p(512)
     k = kv_args(L=1, P=1, H=1, k_sl=7, k_sp=3, k_sh=1, v_sl=-9, v_sp=5, v_sh=3)
     assert lib.fxb_kv_fork(ctypes.byref(k), p, ctypes.c_void_p(8), None) == -1 and "workspace" in err()
+
+
+def test_tree_masks_of_parents_that_are_none():
+    # forward, to itself, outside the tree: on the GPU an index outside would end the process's context
+    from fxlm import tree_masks
+    par = torch.tensor([[-1, 1, 3, 0, 2], [7, 0, -9, 2 ** 31 - 1, 3]], dtype=torch.int32)
+    assert tree_masks(par).tolist() == [[1, 2, 4, 9, 20], [1, 3, 4, 8, 24]]
