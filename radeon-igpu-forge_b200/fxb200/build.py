@@ -10,6 +10,8 @@ without libcuda (symbol checks on CPU) and runs wherever the driver is present.
     python -m fxb200.build          # from radeon-igpu-forge_b200/
 """
 import concurrent.futures as cf
+import importlib.metadata
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -58,11 +60,27 @@ def _compile(src, verbose=False):
     return obj, r.stderr
 
 
+def _binding_key():
+    """What lib/_fxbind.so depends on besides its sources: the versions of torch and Python; None without torch."""
+    if importlib.util.find_spec("torch") is None:
+        return None
+    return f"torch {importlib.metadata.version('torch')}, Python {sys.version}"
+
+
 def _build_binding(force=False):
-    """lib/_fxbind.so from csrc/bind.cpp, against torch's headers (host code)."""
+    """lib/_fxbind.so from csrc/bind.cpp, against torch's headers (host code).
+    Only the generation operators need it: without torch it is left out."""
     src, out = os.path.join(CSRC, "bind.cpp"), os.path.join(LIB_DIR, "_fxbind.so")
+    key, stamp = _binding_key(), out + ".key"
+    if key is None:
+        sys.stderr.write("torch is not installed: libfxb200.so is built, _fxbind.so (generation over a KV cache) not\n")
+        return
+    built_for = None
+    if os.path.exists(out) and os.path.exists(stamp):
+        with open(stamp) as f:
+            built_for = f.read()
     newest = max(os.path.getmtime(src), os.path.getmtime(os.path.join(INCLUDE, "fxb200.h")))
-    if not force and os.path.exists(out) and os.path.getmtime(out) >= newest:
+    if not force and built_for == key and os.path.getmtime(out) >= newest:
         return
     import torch
     home = os.path.dirname(torch.__file__)
@@ -78,6 +96,8 @@ def _build_binding(force=False):
     if r.returncode != 0:
         raise RuntimeError(f"g++ failed for bind.cpp:\n{r.stdout}\n{r.stderr}")
     os.replace(out + ".tmp", out)
+    with open(stamp, "w") as f:
+        f.write(key)
 
 
 def build(force=False, verbose=False, jobs=None):

@@ -342,3 +342,42 @@ def test_tree_masks_of_parents_that_are_none():
     from fxlm import tree_masks
     par = torch.tensor([[-1, 1, 3, 0, 2], [7, 0, -9, 2 ** 31 - 1, 3]], dtype=torch.int32)
     assert tree_masks(par).tolist() == [[1, 2, 4, 9, 20], [1, 3, 4, 8, 24]]
+
+
+@pytest.fixture
+def binding_build(monkeypatch, tmp_path):
+    """fxb200.build with an empty lib folder and a compiler that only writes its output; the commands it was given."""
+    import importlib
+    import subprocess
+    build = importlib.import_module("fxb200.build")
+    ran = []
+
+    def run(cmd, **kw):
+        ran.append(cmd)
+        open(cmd[cmd.index("-o") + 1], "w").close()
+        return subprocess.CompletedProcess(cmd, 0, "", "")
+
+    monkeypatch.setattr(build.subprocess, "run", run)
+    monkeypatch.setattr(build, "LIB_DIR", str(tmp_path))
+    return build, ran
+
+
+def test_binding_is_rebuilt_for_another_torch(binding_build, monkeypatch):
+    # a binding made for another version of torch has another ABI, however new its file is
+    import importlib.metadata
+    build, ran = binding_build
+    build._build_binding()
+    build._build_binding()
+    assert len(ran) == 1
+    monkeypatch.setattr(importlib.metadata, "version", lambda name: "99.0")
+    build._build_binding()
+    build._build_binding()
+    assert len(ran) == 2
+
+
+def test_library_builds_without_torch(binding_build, monkeypatch, capsys):
+    import importlib.util
+    build, ran = binding_build
+    monkeypatch.setattr(importlib.util, "find_spec", lambda name: None)
+    build._build_binding()
+    assert not ran and "torch is not installed" in capsys.readouterr().err
