@@ -140,3 +140,31 @@ def test_gradients_are_not_cut_silently(dev):
         (path, nxt), = step([([1], [-1])], torch.zeros(1, 2, device=dev))
         assert path == [0] and nxt >= 0
     cache.check()
+
+
+@pytest.mark.parametrize("draft", [0, 1, 5])
+def test_generated_tokens_follow_the_model(dev, draft):
+    # the first three tokens of many samples, each continuation's count within 5 standard deviations of what the
+    # model gives it when the window is run again for every token, as the sampler's loop does. The prompt is
+    # chosen so that what is drafted from it is one of the tokens that can follow
+    from fxlm import generate_cached
+    from fxlm.decode import draft_from_text, next_probs
+    m, S, K = model_of(dev, torch.float32), 4000, 3
+    with torch.inference_mode():
+        tries = torch.tensor([[5, 6, t, 9, 8, 5, 6] for t in range(256)], device=dev)
+        p = next_probs(m(tries)[:, -1], 1.0, K)
+        t = int(p[torch.arange(256), torch.arange(256)].argmax())
+        assert 0.1 < float(p[t, t]) < 0.9
+        prompt = tries[t]
+        paths, prob = prompt[None], torch.ones(1, dtype=torch.float64, device=dev)
+        for _ in range(3):
+            top = next_probs(m(paths)[:, -1], 1.0, K).double().topk(K, -1)
+            paths = torch.cat([paths.repeat_interleave(K, 0), top.indices.reshape(-1, 1)], 1)
+            prob = (prob[:, None] * top.values).reshape(-1)
+    if draft:
+        assert draft_from_text(prompt.tolist(), draft + 1)[0][1] == t
+    g = torch.Generator(device=dev).manual_seed(2)
+    out = generate_cached(m, prompt, 3, temperature=1.0, top_k=K, generator=g, draft=draft, samples=S)
+    hits = (out[:, None] == paths[None]).all(-1).double().sum(0)
+    assert int(hits.sum()) == S
+    assert ((hits - S * prob).abs() <= 5 * (S * prob * (1 - prob)).sqrt() + 1).all()

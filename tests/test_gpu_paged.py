@@ -933,3 +933,14 @@ def test_refusals_are_value_errors(dev):
     p = torch.zeros(1, 1, 8, device=dev)
     with pytest.raises(ValueError, match="V=0"):
         verify_tree(i[:, None].long(), i[:, None], i, p[..., :0], p[:, :, 0])
+
+
+@pytest.mark.parametrize("dtype,T,Hq,Hkv,lens", [
+    (BF16, 1, 2, 1, [40, 900, 3, 300]), (BF16, 3, 2, 2, [700, 0, 130]), (F32, 2, 3, 1, [500, 64, 5]),
+    (BF16, 20, 2, 1, [700, 5, 130, 0]), (F16, 33, 4, 1, [300, 129])])
+@pytest.mark.parametrize("B", [33, 48, 128, 385])
+def test_attention_batches(dev, dtype, T, Hq, Hkv, lens, B):
+    # as many batch rows as a warp has lanes and more, up to more than a block has threads; the last row long, so
+    # that few short rows are cut into whole parts
+    lens = [lens[b % len(lens)] for b in range(B - 1)] + [3000]
+    check(make(dev, dtype, B, T, Hq, Hkv, 64, lens, 32, seed=B + T))
