@@ -165,7 +165,10 @@ struct Rows16 {
       const float p2 = ex2(fmaf(s[i][2], a.scale_log2, -z1)), p3 = ex2(fmaf(s[i][3], a.scale_log2, -z1));
       l[0] += p0 + p1;
       l[1] += p2 + p3;
-      // the probabilities enter the second product in the inputs' type, as its operands must
+      // The probabilities enter the second product in the inputs' type, as both of its operands have one type: the
+      // error against 64 bits is 1.35 times that of fp32 probabilities (bf16 2.3e-3 for 1.7e-3). A second product
+      // with what the rounding leaves brings it to 1.0 times, but takes 200 us for 190 (48 rows of up to 8192 slots,
+      // without a pause, at the clock of the power limit), and makes NaN of an infinite value where nothing, or less than 0, is left.
       p[2 * i] = pack2<T>(p0, p1);
       p[2 * i + 1] = pack2<T>(p2, p3);
     }
@@ -639,7 +642,7 @@ tree_attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     const Cursor cur = c;
     next<kBlockKeys>(a, c);
     if (tree || c.left == 0) {
-      // the four warps' states join; each lies in the stage that its warp has just used up
+      // the warps' states join; each lies in the stage that its warp has just used up
       __syncwarp();
       rows.end(reinterpret_cast<float*>(slot), sm[warp], sl[warp]);
       __syncthreads();
