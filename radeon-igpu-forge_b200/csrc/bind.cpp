@@ -2,7 +2,7 @@
 // checks that they fit, makes what is returned and launches. A decoding step
 // makes these calls once a layer for a few microseconds of GPU work, and the
 // same from Python, attribute by attribute, was what bounded small calls (host
-// time of one token's attention 14.1 us, now 5.4; of a commit 11.4, now 4.5; of
+// time of one token's attention 14.1 us, now 6.1; of a commit 11.4, now 4.5; of
 // a chain's verification 12.4, now 6.6).
 //
 // A function returns its result, None when an argument does not fit (the caller

@@ -78,14 +78,16 @@ def stream_workspace(kind, device_index, stream, nbytes, zeroed):
     other capture each call gets one of its own, which the graph's memory pool
     owns. Its first `zeroed` bytes are zero before the first use; the kernels
     leave them so."""
-    device = torch.device("cuda", device_index)
+    def new():
+        return _zeroed_workspace(torch.device("cuda", device_index), nbytes, zeroed)
+
     if _capturing_without_table():
-        return _zeroed_workspace(device, nbytes, zeroed)
+        return new()
     table = _CAPTURE_WS if _CAPTURE_WS is not None else _STREAM_WS
     key = (kind, device_index, stream)
     ws = table.get(key)
     if ws is None or ws.numel() < nbytes:
-        ws = table[key] = _zeroed_workspace(device, nbytes, zeroed)
+        ws = table[key] = new()
     return ws
 
 
