@@ -417,6 +417,8 @@ int fxb_tree_attn(const fxb_tree_attn_args* args, void* stream);
  * Sums are taken over floor(w * 2^36) in 64-bit integers, so results do not
  * depend on the order of summation; values that are not above 0 (NaN among
  * them) count as 0, values above 1 as 1.
+ * A parent that is no earlier node counts as none; n_nodes outside [0, T] counts
+ * as the nearer end (bit 16 of the device error word).
  * path (B,T): the accepted nodes in order, node 0 first, then -1; n_path (B):
  * their number; next (B): the drawn token, -1 for n_nodes == 0 or an empty row. */
 int fxb_verify_tree(const int64_t* tokens, const int32_t* parents, const int32_t* n_nodes,

@@ -274,7 +274,10 @@ __global__ void __launch_bounds__(kMaxThreads, 2) verify_tree_kernel(const Verif
     __syncthreads();  // s.part has been read
     total = row_sum();
   }
-  if (rank == 0 && tid == 0) a.n_path[b] = n ? n_path : 0;
+  if (rank == 0 && tid == 0) {
+    a.n_path[b] = n ? n_path : 0;
+    if (n != n_in) atomicOr(a.err, FXB_DERR_PAGES);
+  }
   if (total == 0 || !ok) {
     if (rank == 0 && tid == 0) a.next[b] = -1;
     return;

@@ -232,7 +232,7 @@ def device_error(clear=True):
 # bits of the device error word (csrc/common.cuh)
 DERR_NAMES = {1: "gemm (tensor-core pipeline or tail-split wait)", 2: "attention pipeline",
               4: "gather pipeline", 8: "cross-entropy row copy",
-              16: "KV cache: page ids, free pages, lengths or paths that do not fit the call",
+              16: "KV cache: page ids, free pages, lengths, numbers of nodes or paths that do not fit the call",
               32: "verification of drafted tokens"}
 DERR_GEMM_WAIT = 1
 DERR_PAGES = 16

@@ -944,3 +944,18 @@ def test_attention_batches(dev, dtype, T, Hq, Hkv, lens, B):
     # that few short rows are cut into whole parts
     lens = [lens[b % len(lens)] for b in range(B - 1)] + [3000]
     check(make(dev, dtype, B, T, Hq, Hkv, 64, lens, 32, seed=B + T))
+
+
+@pytest.mark.parametrize("draft", [False, True])
+def test_verify_reports_numbers_of_nodes_outside_the_tree(dev, draft):
+    from fxb200 import _lib
+    from fxlm import verify_tree
+    tokens, par, n, p, u, q = (None if x is None else x.to(dev) for x in verify_inputs(3, 4, 60, draft, seed=2))
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    want = verify_tree(tokens, par, i32([4, 0, 2]), p, u, draft_probs=q)
+    _lib.raise_on_device_error()
+    got = verify_tree(tokens, par, i32([9, -3, 2]), p, u, draft_probs=q)
+    for x, y in zip(want, got):
+        assert torch.equal(x, y)
+    with pytest.raises(RuntimeError, match="KV cache"):
+        _lib.raise_on_device_error()
