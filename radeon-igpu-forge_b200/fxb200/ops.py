@@ -92,16 +92,19 @@ def stream_workspace(kind, device_index, stream, nbytes, zeroed):
 
 
 class graph_workspaces:
-    """Context manager used around a CUDA-graph capture: GEMMs captured inside
-    it use workspaces stored in `table` (owned by the graph object, alive as
-    long as the graph), whose counters are zeroed by a memset node at the
-    start of every replay's first GEMM on that stream."""
+    """Context manager used around one CUDA-graph capture: calls captured inside
+    it use workspaces stored in `table` (an empty dict owned by the graph
+    object, alive as long as the graph), whose counters are zeroed by a memset
+    node at the start of every replay's first call on that stream. A second
+    graph with the same table would have no such node, so it is refused."""
 
     def __init__(self, table):
         self.table = table
 
     def __enter__(self):
         global _CAPTURE_WS
+        if self.table:
+            raise ValueError("graph_workspaces: the table has the workspaces of another capture")
         self.prev, _CAPTURE_WS = _CAPTURE_WS, self.table
         return self.table
 

@@ -381,3 +381,15 @@ def test_library_builds_without_torch(binding_build, monkeypatch, capsys):
     monkeypatch.setattr(importlib.util, "find_spec", lambda name: None)
     build._build_binding()
     assert not ran and "torch is not installed" in capsys.readouterr().err
+
+
+def test_a_table_of_workspaces_serves_one_capture(monkeypatch, allocations):
+    from fxb200 import ops
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    table = {}
+    with ops.graph_workspaces(table):
+        ops.stream_workspace("k", 0, 7, 100, 16)
+    with pytest.raises(ValueError, match="another capture"):
+        with ops.graph_workspaces(table):
+            pass
+    assert ops._CAPTURE_WS is None
